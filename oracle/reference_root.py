@@ -14,6 +14,7 @@ DEFAULT = "/root/reference"
 
 def reference_root() -> str:
     """The reference checkout: $FALCOM_REFERENCE_ROOT, else the recipe
-    default; "" when neither exists."""
+    default; "" when neither holds the reference's sources (an empty folder
+    is no checkout)."""
     root = os.environ.get("FALCOM_REFERENCE_ROOT", DEFAULT)
-    return root if os.path.isdir(root) else ""
+    return root if os.path.isfile(os.path.join(root, "momentum_compressor_openmp_simd_final.c")) else ""

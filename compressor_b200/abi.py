@@ -526,6 +526,59 @@ def bind_extensions(lib: ctypes.CDLL) -> None:
     lib.falcom_state_load.argtypes = [c_vp, ctypes.c_char_p]
     lib.falcom_state_load.restype = ctypes.c_int
     bind_replay(lib)
+    bind_optim(lib)
+
+
+TYPE_F32, TYPE_BF16, TYPE_F16 = range(3)
+ADAMW_BLOCK = 256
+
+
+class AdamWTensorC(ctypes.Structure):
+    _fields_ = [
+        ("param", ctypes.c_void_p),
+        ("grad", ctypes.c_void_p),
+        ("m", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("m_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("n", ctypes.c_size_t),
+        ("param_type", ctypes.c_int),
+        ("grad_type", ctypes.c_int),
+        ("weight_decay", ctypes.c_double),
+    ]
+
+
+class AdamWArgsC(ctypes.Structure):
+    _fields_ = [
+        ("lr", ctypes.c_double),
+        ("beta1", ctypes.c_double),
+        ("beta2", ctypes.c_double),
+        ("eps", ctypes.c_double),
+        ("grad_scale", ctypes.c_double),
+        ("seed", ctypes.c_uint64),
+        ("clip", ctypes.c_void_p),
+        ("lr_device", ctypes.c_void_p),
+    ]
+
+
+def bind_optim(lib: ctypes.CDLL) -> None:
+    """Optimiser entry points (falcom_norm_*, falcom_adamw_*); no instance needed."""
+    P = ctypes.POINTER
+    c_vp = ctypes.c_void_p
+    lib.falcom_norm_create.argtypes = [P(c_vp), P(ctypes.c_size_t), P(ctypes.c_int), ctypes.c_size_t]
+    lib.falcom_norm_create.restype = c_vp
+    lib.falcom_norm_work_bytes.argtypes = [c_vp]
+    lib.falcom_norm_work_bytes.restype = ctypes.c_size_t
+    lib.falcom_norm_run.argtypes = [c_vp, ctypes.c_double, ctypes.c_double, c_vp, c_vp, c_vp]
+    lib.falcom_norm_run.restype = ctypes.c_int
+    lib.falcom_norm_destroy.argtypes = [c_vp]
+    lib.falcom_norm_destroy.restype = None
+    lib.falcom_adamw_create.argtypes = [P(AdamWTensorC), ctypes.c_size_t, ctypes.c_int, c_vp]
+    lib.falcom_adamw_create.restype = c_vp
+    lib.falcom_adamw_step.argtypes = [c_vp, P(AdamWArgsC), c_vp]
+    lib.falcom_adamw_step.restype = ctypes.c_int
+    lib.falcom_adamw_destroy.argtypes = [c_vp]
+    lib.falcom_adamw_destroy.restype = None
 
 
 def bind_replay(lib: ctypes.CDLL) -> None:

@@ -307,6 +307,124 @@ int falcom_replay_write(const char *path, uint32_t round, const char *client_id,
 int falcom_state_save(MomentumCompressor *mc, const char *path);
 int falcom_state_load(MomentumCompressor *mc, const char *path);
 
+/* Optimiser step over many tensors.  No counterpart in the reference
+ * interface, whose server only averages the decoded updates.
+ *
+ * What comes next to the codec: a server takes the aggregate of a round
+ * (falcom_set_aggregate) as the gradient of an AdamW step on the global
+ * model, a client takes AdamW steps between two rounds.  Both work on a
+ * fixed list of tensors, so each entry point is a plan: create it once per
+ * list of addresses, then run it any number of times.
+ *
+ * Common rules.  Tensors are contiguous device memory of one device, each
+ * aligned to its element size, of any length (0 too); 16-byte alignment of
+ * all of a tensor's arrays gives the fast loads.  A plan copies the lists
+ * and keeps the addresses: the memory must stay allocated while the plan, or
+ * a CUDA graph that captured its calls, is used.  create and destroy
+ * allocate and synchronise, so they do not belong inside a stream capture;
+ * run and step only queue kernels on `stream` (cudaStream_t of the plan's
+ * device, NULL = its legacy default stream), whatever device is current, and
+ * may be captured.  Element types: */
+enum { FALCOM_TYPE_F32 = 0, FALCOM_TYPE_BF16 = 1, FALCOM_TYPE_F16 = 2 };
+
+/* Gradient norm with clipping coefficient.
+ *   norm        = |scale| * sqrt(sum of squares over every tensor)
+ *   coefficient = max_norm / norm when norm > max_norm, else 1;
+ *                 NaN when the norm is infinite or NaN
+ * Squares and sums are taken in 64 bits, in an order that depends only on
+ * the list, so repeated runs give the same bits.
+ *
+ * falcom_norm_create: tensors[i] has numels[i] elements of dtypes[i].
+ * Returns NULL (message on stderr) for a NULL or misaligned address, memory
+ * that is not device memory of one device, an unknown type, or when
+ * allocation fails.
+ * falcom_norm_run writes out[0] = norm and out[1] = coefficient (float32
+ * device memory).  max_norm > 0; INFINITY only measures.  `work` is device
+ * memory of falcom_norm_work_bytes() bytes, 8-byte aligned, zeroed before
+ * its first use; every run leaves it ready for the next.  Runs that may be
+ * in flight at the same time (two streams, two captured graphs) need a
+ * `work` and an `out` each.
+ * Returns 0; ERROR_INVALID_PARAM for bad arguments; ERROR_COMPRESSION when
+ * the launch fails or a CUDA error from earlier work is pending (nothing is
+ * launched then, and the error stays pending). */
+typedef struct falcom_norm falcom_norm;
+falcom_norm *falcom_norm_create(const void *const *tensors, const size_t *numels, const int *dtypes, size_t n);
+size_t falcom_norm_work_bytes(const falcom_norm *plan);
+int falcom_norm_run(falcom_norm *plan, double scale, double max_norm, float *out, void *work, void *stream);
+void falcom_norm_destroy(falcom_norm *plan);
+
+/* AdamW (decoupled weight decay).  With t the number of the step taken, lr
+ * the learning rate and f = grad_scale * clip coefficient:
+ *   g' = f g
+ *   m' = beta1 m + (1 - beta1) g'
+ *   v' = beta2 v + (1 - beta2) g'^2
+ *   p' = (1 - lr * weight_decay) p
+ *        - lr / (1 - beta1^t) * m' / (sqrt(v') / sqrt(1 - beta2^t) + eps)
+ * in float32 from the element types' values, each operation rounded to
+ * nearest in the order written (no contraction; the coefficients of t and lr
+ * are formed in 64 bits and rounded once), p' rounded to the parameter's
+ * type at the end.  A server whose aggregate is the sum of weight
+ * *differences* passes grad_scale = -1.
+ *
+ * state_bits = 32: m and v are float32[n].
+ * state_bits = 8: m and v are one byte per element.  Every FALCOM_ADAMW_BLOCK
+ * consecutive elements of a tensor (the last block may be short) share two
+ * float32 scales, m_scale[n_blocks] and v_scale[n_blocks]:
+ *   m = e4m3(m code) * m_scale,   sqrt(v) = e4m3(v code) * v_scale.
+ * After the step a block's scale is its largest magnitude / 448, and every
+ * value is rounded up or down to a neighbouring e4m3 value with the
+ * probability that makes the result right on average (rounding to the
+ * nearest would hold sqrt(v) still: it moves by 0.05 % a step for beta2 =
+ * 0.999, the codes are 6 to 12 % apart).  The random bits are a hash of
+ * (seed, t, position), the position being 256 * (blocks of the plan's
+ * earlier tensors) + the element's index: the same call on the same state
+ * gives the same bits on every GPU.  A v > 0 never gets code 0, so no
+ * denominator vanishes under a first moment that did not.  All-zero state
+ * (codes and scales 0) is the start.  A block in which a new value is
+ * infinite or NaN gets NaN scales and zero codes; a block whose values are
+ * all below 2^-100 gets zeros.
+ *
+ * `step` is an int64 counter in device memory (0 at the start): a step reads
+ * it, takes step number t = *step + 1 and writes it back, so a captured step
+ * can be replayed.  `clip`, when not NULL, is falcom_norm_run's output
+ * (device memory): its coefficient multiplies the gradient, and a NaN
+ * coefficient (the norm was not finite) skips the step: nothing changes, the
+ * counter included.  `lr_device`, when not NULL, is a float32 in device
+ * memory used instead of `lr`.
+ *
+ * falcom_adamw_create returns NULL (message on stderr) for state_bits other
+ * than 32 and 8, NULL or misaligned addresses (param, grad: element size; m,
+ * v: 4 bytes with 32 bits; scales: 4; step: 8), unknown types, a negative or
+ * non-finite weight decay, memory that is not device memory of one device,
+ * arrays that are written and overlap any other array, or when allocation
+ * fails.  The steps of one plan must be ordered (one stream, or events).
+ * falcom_adamw_step returns 0; ERROR_INVALID_PARAM for lr < 0 or not finite,
+ * betas outside [0, 1), eps not positive as a float32, a non-finite
+ * grad_scale, or a clip or lr_device that is not device memory of the plan's
+ * device; ERROR_COMPRESSION when a launch fails or an error is pending, as
+ * above.  One launch per pair of parameter and gradient type in the list. */
+#define FALCOM_ADAMW_BLOCK 256
+typedef struct falcom_adamw_tensor {
+    void *param;
+    const void *grad;
+    void *m, *v;
+    float *m_scale, *v_scale;   /* state_bits = 8 only */
+    size_t n;
+    int param_type, grad_type;
+    double weight_decay;
+} falcom_adamw_tensor;
+typedef struct falcom_adamw_args {
+    double lr, beta1, beta2, eps;
+    double grad_scale;
+    uint64_t seed;
+    const float *clip;
+    const float *lr_device;
+} falcom_adamw_args;
+typedef struct falcom_adamw falcom_adamw;
+falcom_adamw *falcom_adamw_create(const falcom_adamw_tensor *tensors, size_t n, int state_bits, int64_t *step);
+int falcom_adamw_step(falcom_adamw *plan, const falcom_adamw_args *args, void *stream);
+void falcom_adamw_destroy(falcom_adamw *plan);
+
 #ifdef __cplusplus
 }
 #endif

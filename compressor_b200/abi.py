@@ -577,6 +577,8 @@ def bind_optim(lib: ctypes.CDLL) -> None:
     lib.falcom_adamw_create.restype = c_vp
     lib.falcom_adamw_step.argtypes = [c_vp, P(AdamWArgsC), c_vp]
     lib.falcom_adamw_step.restype = ctypes.c_int
+    lib.falcom_adamw_errors.argtypes = [c_vp]
+    lib.falcom_adamw_errors.restype = ctypes.c_int
     lib.falcom_adamw_destroy.argtypes = [c_vp]
     lib.falcom_adamw_destroy.restype = None
 

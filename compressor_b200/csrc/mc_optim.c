@@ -28,7 +28,7 @@ struct falcom_adamw {
     int device;
     int bits;
     int64_t *step;
-    uint8_t *table;   /* ticket, op_adamw_tensor[n], op_unit[] of every type pair */
+    uint8_t *table;   /* ticket, error word, op_adamw_tensor[n], op_unit[] of every type pair */
     size_t tensors_at, units_at;
     int64_t n_units[OP_NTYPES * OP_NTYPES];   /* by param_type * OP_NTYPES + grad_type */
     int grid[OP_NTYPES * OP_NTYPES];
@@ -278,7 +278,7 @@ static int check_tensors(const char *who, const falcom_adamw_tensor *t, size_t n
             fprintf(stderr, "[ERROR] %s: tensor %zu has an unknown type\n", who, i);
             return 0;
         }
-        if (!(t[i].weight_decay >= 0.0) || !isfinite(t[i].weight_decay) || t[i].n > (size_t)1 << 40) {
+        if (!(t[i].weight_decay >= 0.0) || !isfinite(t[i].weight_decay) || t[i].n > (size_t)1 << 39) {
             fprintf(stderr, "[ERROR] %s: weight decay or length of tensor %zu is out of range\n", who, i);
             return 0;
         }
@@ -324,7 +324,7 @@ MC_EXPORT falcom_adamw *falcom_adamw_create(const falcom_adamw_tensor *tensors, 
         fprintf(stderr, "[ERROR] %s: out of memory\n", who);
         return NULL;
     }
-    const int ok = check_tensors(who, tensors, n, state_bits, step, &device, spans);
+    int ok = check_tensors(who, tensors, n, state_bits, step, &device, spans);
     free(spans);
     if (!ok) return NULL;
 
@@ -333,6 +333,10 @@ MC_EXPORT falcom_adamw *falcom_adamw_create(const falcom_adamw_tensor *tensors, 
         const int64_t k = (int64_t)((tensors[i].n + OP_ADAMW_UNIT - 1) / OP_ADAMW_UNIT);
         counts[tensors[i].param_type * OP_NTYPES + tensors[i].grad_type] += k;
         total += k;
+    }
+    if (total > (int64_t)UINT32_MAX / 2) {
+        fprintf(stderr, "[ERROR] %s: too many elements\n", who);
+        return NULL;
     }
     falcom_adamw *plan = (falcom_adamw *)calloc(1, sizeof(*plan));
     const size_t tensors_at = 256;
@@ -362,10 +366,10 @@ MC_EXPORT falcom_adamw *falcom_adamw_create(const falcom_adamw_tensor *tensors, 
         t[i].n = (int64_t)a->n;
         t[i].first_block = blocks;
         t[i].weight_decay = a->weight_decay;
-        const uintptr_t state = state_bits == 32 ? 16 : 4;
-        t[i].vec = ((uintptr_t)a->param & (4 * g_type_size[a->param_type] - 1)) == 0 &&
-                   ((uintptr_t)a->grad & (4 * g_type_size[a->grad_type] - 1)) == 0 &&
-                   (((uintptr_t)a->m | (uintptr_t)a->v) & (state - 1)) == 0;
+        if ((((uintptr_t)a->m | (uintptr_t)a->v) & 15) != 0) t[i].how = OP_RAGGED;
+        else if (((uintptr_t)a->param & (4 * g_type_size[a->param_type] - 1)) != 0 ||
+                 ((uintptr_t)a->grad & (4 * g_type_size[a->grad_type] - 1)) != 0) t[i].how = OP_STATES;
+        else t[i].how = OP_ALIGNED;
         blocks += (int64_t)((a->n + OP_BLOCK - 1) / OP_BLOCK);
         const int c = a->param_type * OP_NTYPES + a->grad_type;
         const size_t k = (a->n + OP_ADAMW_UNIT - 1) / OP_ADAMW_UNIT;
@@ -420,11 +424,10 @@ MC_EXPORT int falcom_adamw_step(falcom_adamw *plan, const falcom_adamw_args *a, 
     L.lr = a->lr;
     L.beta1 = a->beta1;
     L.beta2 = a->beta2;
-    L.b1 = (float)a->beta1;
-    L.b1c = (float)(1.0 - a->beta1);
-    L.b2 = (float)a->beta2;
-    L.b2c = (float)(1.0 - a->beta2);
-    L.eps = (float)a->eps;
+    L.b1.x = L.b1.y = (float)a->beta1;
+    L.b2.x = L.b2.y = (float)a->beta2;
+    L.b2root = (float)sqrt(a->beta2);
+    L.eps.x = L.eps.y = (float)a->eps;
     L.scale = (float)a->grad_scale;
     L.seed_key = mc_op_hash(mc_op_hash((uint32_t)a->seed ^ 0x9E3779B9u) ^ (uint32_t)(a->seed >> 32));
     int e = 0;
@@ -439,6 +442,17 @@ MC_EXPORT int falcom_adamw_step(falcom_adamw *plan, const falcom_adamw_args *a, 
     }
     leave(prev, plan->device);
     return e == 0 ? ERROR_NONE : launch_failed(who, e);
+}
+
+MC_EXPORT int falcom_adamw_errors(falcom_adamw *plan) {
+    if (!plan) return ERROR_INVALID_PARAM;
+    const int prev = enter(plan->device);
+    if (prev == -2) return ERROR_COMPRESSION;
+    uint32_t word = 0;
+    const cudaError_t e = cudaMemcpy(&word, plan->table + 4, 4, cudaMemcpyDeviceToHost);
+    leave(prev, plan->device);
+    if (e != cudaSuccess) return ERROR_COMPRESSION;
+    return word != 0;
 }
 
 MC_EXPORT void falcom_adamw_destroy(falcom_adamw *plan) {

@@ -5,6 +5,7 @@
 #ifndef MC_OPTIM_H
 #define MC_OPTIM_H
 
+#include <cuda_runtime_api.h>
 #include <stddef.h>
 #include <stdint.h>
 
@@ -19,7 +20,12 @@ extern "C" {
 #define OP_BLOCK FALCOM_ADAMW_BLOCK   /* elements a warp holds in registers at once (8 per lane) */
 #define OP_NTYPES 3
 
-/* A unit is a run of elements of one tensor that one warp works through. */
+/* Which arrays of a tensor are aligned (16 bytes; with 32-bit states 4
+ * elements): not its states, its states only, or all. */
+enum { OP_RAGGED = 0, OP_STATES = 1, OP_ALIGNED = 2 };
+
+/* A unit is a run of elements of one tensor: one warp's work at a time for
+ * the norm, one CTA's for AdamW. */
 typedef struct {
     uint32_t tensor;   /* index into the plan's tensors */
     uint32_t index;    /* unit number inside the tensor */
@@ -40,7 +46,7 @@ typedef struct {
     int64_t n;
     int64_t first_block;   /* OP_BLOCKs of the plan's earlier tensors: the dither's position */
     double weight_decay;
-    int32_t vec;           /* 4-element loads and stores allowed on all four arrays */
+    int32_t how;           /* OP_RAGGED, OP_STATES or OP_ALIGNED */
     int32_t pad;
 } op_adamw_tensor;
 
@@ -57,19 +63,20 @@ typedef struct {
 typedef struct {
     const op_adamw_tensor *tensors;
     const op_unit *units;
-    int64_t n_units;
+    uint32_t n_units;
     int64_t *step;
     const float *clip;     /* NULL, or {norm, coefficient} */
     const float *lr_dev;   /* NULL, or the learning rate */
     uint32_t *ticket;      /* 0 between calls */
     double lr, beta1, beta2;
-    float b1, b1c, b2, b2c, eps, scale;
+    float2 b1, b2, eps;    /* twice each, for two-element operations */
+    float b2root, scale;   /* sqrt(beta2) */
     uint32_t seed_key;     /* hash of the seed */
     int32_t advance;       /* this launch's last CTA counts the step */
 } op_adamw_launch;
 
 #define OP_NORM_UNIT 2048
-#define OP_ADAMW_UNIT 1024
+#define OP_ADAMW_UNIT (OP_WARPS * OP_BLOCK)
 
 uint32_t mc_op_hash(uint32_t x);
 int mc_op_norm_grid(int64_t n_units, int sms);

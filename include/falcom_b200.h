@@ -318,7 +318,7 @@ int falcom_state_load(MomentumCompressor *mc, const char *path);
  *
  * Common rules.  Tensors are contiguous device memory of one device, each
  * aligned to its element size, of any length (0 too); 16-byte alignment of
- * all of a tensor's arrays gives the fast loads.  A plan copies the lists
+ * a tensor's arrays, of its states above all, gives the fast loads.  A plan copies the lists
  * and keeps the addresses: the memory must stay allocated while the plan, or
  * a CUDA graph that captured its calls, is used.  create and destroy
  * allocate and synchronise, so they do not belong inside a stream capture;
@@ -360,11 +360,11 @@ void falcom_norm_destroy(falcom_norm *plan);
  *   v' = beta2 v + (1 - beta2) g'^2
  *   p' = (1 - lr * weight_decay) p
  *        - lr / (1 - beta1^t) * m' / (sqrt(v') / sqrt(1 - beta2^t) + eps)
- * in float32 from the element types' values, each operation rounded to
- * nearest in the order written (no contraction; the coefficients of t and lr
- * are formed in 64 bits and rounded once), p' rounded to the parameter's
- * type at the end.  A server whose aggregate is the sum of weight
- * *differences* passes grad_scale = -1.
+ * in float32 from the element types' values (the coefficients of t, lr and
+ * the betas are formed in 64 bits and rounded once; the root and the quotient
+ * are within two units in the last place, and a v' under 2^-126 counts as 0
+ * in the root), p' rounded to the parameter's type at the end.  A server
+ * whose aggregate is the sum of weight *differences* passes grad_scale = -1.
  *
  * state_bits = 32: m and v are float32[n].
  * state_bits = 8: m and v are one byte per element.  Every FALCOM_ADAMW_BLOCK
@@ -380,9 +380,9 @@ void falcom_norm_destroy(falcom_norm *plan);
  * earlier tensors) + the element's index: the same call on the same state
  * gives the same bits on every GPU.  A v > 0 never gets code 0, so no
  * denominator vanishes under a first moment that did not.  All-zero state
- * (codes and scales 0) is the start.  A block in which a new value is
- * infinite or NaN gets NaN scales and zero codes; a block whose values are
- * all below 2^-100 gets zeros.
+ * (codes and scales 0) is the start.  Of a block in which a new value of m
+ * (of sqrt(v)) is infinite, NaN or 2^100 and more, m's (v's) scale becomes
+ * NaN and its codes 0; one whose values are all below 2^-100 gets zeros.
  *
  * `step` is an int64 counter in device memory (0 at the start): a step reads
  * it, takes step number t = *step + 1 and writes it back, so a captured step
@@ -423,6 +423,10 @@ typedef struct falcom_adamw_args {
 typedef struct falcom_adamw falcom_adamw;
 falcom_adamw *falcom_adamw_create(const falcom_adamw_tensor *tensors, size_t n, int state_bits, int64_t *step);
 int falcom_adamw_step(falcom_adamw *plan, const falcom_adamw_args *args, void *stream);
+/* 1 when a step of the plan gave up waiting for its own memory copies (about
+ * two seconds; its result is then not to be used), else 0.  Waits for the
+ * legacy default stream's work. */
+int falcom_adamw_errors(falcom_adamw *plan);
 void falcom_adamw_destroy(falcom_adamw *plan);
 
 #ifdef __cplusplus

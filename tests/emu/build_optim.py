@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import hashlib
 import os
+import re
 import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -17,6 +18,46 @@ BUILD = os.path.join(HERE, "_build_optim")
 INPUTS = [os.path.join(base.CSRC, f) for f in ("mc_optim.c", "mc_optim.cu", "mc_optim.h")] + \
          [os.path.join(base.INCLUDE, "falcom_b200.h")] + \
          [os.path.join(HERE, f) for f in ("emu.h", "emu_optim.h", "fake_cudart.cpp", "prep.py", "build_optim.py")]
+
+LD_STREAM = ' if (((uintptr_t)p) & (sizeof(*p) - 1)) abort(); return *p; '
+# host bodies of the inline-PTX helpers
+BODIES = {
+    "pdl_wait": "",
+    "pdl_release": "",
+    "smem_u32": " return emu_smem_u32(p); ",
+    "mbar_init": " emu_mbar_init(bar, count); ",
+    # copies complete at issue
+    "mbar_expect_tx": " (void)bytes; emu_mbar_arrive(bar); ",
+    "mbar_arrive": " emu_mbar_arrive(bar); ",
+    "bulk_g2s": """
+    (void)bar;
+    char *d = (char *)emu_smem_ptr(dst);
+    if ((dst & 15) || (((uintptr_t)src) & 15) || (bytes & 15) || d < (char *)emu_cta->lo ||
+        d + bytes > (char *)emu_cta->hi) abort();
+    memcpy(d, src, bytes);
+""",
+    "copy_async4": " if ((char *)dst < (char *)emu_cta->lo || (char *)(dst + 1) > (char *)emu_cta->hi) abort(); *dst = *src; ",
+    "arrive_after_copies": " emu_mbar_arrive(bar); ",
+    "mbar_try_wait": " return emu_mbar_done(bar, parity); ",
+    "mbar_wait_long": """
+    for (int i = 0; i < 50000000; i++) {
+        if (emu_mbar_done(bar, parity)) return true;
+        std::this_thread::yield();
+    }
+    fprintf(stderr, "emu: a barrier never completed\\n");
+    abort();
+""",
+    "mul2": " return make_float2(a.x * b.x, a.y * b.y); ",
+    "fma2": " return make_float2(fmaf(a.x, b.x, c.x), fmaf(a.y, b.y, c.y)); ",
+    "sqrt_fast": " return sqrtf(x); ",
+    "rcp_fast": " return 1.0f / x; ",
+    "max_abs": " a = fabsf(a); return a != a || b != b || c != c ? NAN : fmaxf(a, fmaxf(fabsf(b), fabsf(c))); ",
+    "warp_max": " for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o)); return v; ",
+    "e4m3_quad": """
+    a = make_float2(emu_e4m3(codes & 0xFF), emu_e4m3(codes >> 8 & 0xFF));
+    b = make_float2(emu_e4m3(codes >> 16 & 0xFF), emu_e4m3(codes >> 24));
+""",
+}
 
 
 def build() -> str:
@@ -30,9 +71,12 @@ def build() -> str:
     os.makedirs(BUILD, exist_ok=True)
     with open(os.path.join(base.CSRC, "mc_optim.cu")) as f:
         src = f.read()
-    s = prep.transform(src.replace("__host__ ", ""), helpers=False)
-    for name in ("pdl_wait", "pdl_release"):
-        s = prep._replace_body(s, name, "")
+    s = prep.transform(re.sub(r"extern __shared__ __align__\(\d+\) float s_stage\[\];", "", src).replace("__host__ ", "").replace("__noinline__ ", "").replace("__grid_constant__ ", ""), helpers=False)
+    for vec in ("uint32_t", "uint2", "uint4"):   # the overloads one after another
+        at = s.index(f"inline {vec} ld_stream(")
+        s = prep._replace_block(s, s.index("{", at), LD_STREAM)
+    for name, body in BODIES.items():
+        s = prep._replace_body(s, name, body)
     if "emu_run(grid, smem" not in s or "<<<" in s or "asm volatile" in s:
         raise ValueError("a launch or an inline instruction was not rewritten")
     s = s.replace('#include "emu.h"', '#include "emu.h"\n#include "emu_optim.h"')

@@ -6,3 +6,47 @@ extern "C" inline __attribute__((used)) cudaError_t cudaDeviceGetAttribute(int *
     *v = 2;   // two SMs: grids that stride over their units even in small cases
     return cudaSuccess;
 }
+
+inline float emu_e4m3(unsigned code) {
+    const int e = code >> 3 & 15, f = code & 7;
+    float v = e ? ldexpf(1.0f + f / 8.0f, e - 7) : ldexpf(f / 8.0f, -6);
+    if ((code & 0x7F) == 0x7F) v = NAN;
+    return code & 0x80 ? -v : v;
+}
+// towards zero, by way of a 64-bit value (products and sums of the scale's
+// computation fit it)
+inline float __fmaf_rz(float a, float b, float c) {
+    const double x = fma((double)a, (double)b, (double)c);
+    float r = (float)x;
+    if (fabs((double)r) > fabs(x)) r = nextafterf(r, 0.0f);
+    return r;
+}
+
+inline unsigned __byte_perm(unsigned a, unsigned b, unsigned sel) {
+    const unsigned long long ab = (unsigned long long)b << 32 | a;
+    unsigned r = 0;
+    for (int i = 0; i < 4; i++) r |= (unsigned)(ab >> 8 * (sel >> 4 * i & 7) & 0xFF) << 8 * i;
+    return r;
+}
+inline float __saturatef(float x) { return x > 0.0f ? (x < 1.0f ? x : 1.0f) : 0.0f; }
+
+template <class T>
+inline T __shfl_sync(unsigned, T v, int src) {   // emu_shfl knows lane ^ arg: from src's own side
+    return emu_shfl(v, false, (int)(threadIdx.x & 31) ^ src);
+}
+inline int __all_sync(unsigned, int p) { return __ballot_sync(0xffffffffu, p) == 0xffffffffu; }
+
+// An mbarrier: arrivals expected, arrivals missing in this phase, phase.
+inline void emu_mbar_init(uint32_t bar, uint64_t count) {
+    __atomic_store_n((uint64_t *)emu_smem_ptr(bar), count << 40 | count << 8, __ATOMIC_SEQ_CST);
+}
+inline void emu_mbar_arrive(uint32_t bar) {
+    uint64_t *p = (uint64_t *)emu_smem_ptr(bar), old = __atomic_load_n(p, __ATOMIC_SEQ_CST), now;
+    do {
+        const uint64_t count = old >> 40, missing = (old >> 8 & 0xFFFFFFFF) - 1;
+        now = missing ? count << 40 | missing << 8 | (old & 1) : count << 40 | count << 8 | ((old & 1) ^ 1);
+    } while (!__atomic_compare_exchange_n(p, &old, now, false, __ATOMIC_SEQ_CST, __ATOMIC_SEQ_CST));
+}
+inline bool emu_mbar_done(uint32_t bar, uint32_t parity) {
+    return (__atomic_load_n((uint64_t *)emu_smem_ptr(bar), __ATOMIC_SEQ_CST) & 1) != parity;
+}

@@ -10,9 +10,8 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include "mc_internal.h"
 #include "mc_optim.h"
-
-#define MC_EXPORT __attribute__((visibility("default")))
 
 static const size_t g_type_size[OP_NTYPES] = {4, 2, 2};
 
@@ -39,27 +38,22 @@ static size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 /* [p, p + bytes) is device memory of one device, the plan's (*device, -1
  * before the first range); misalignment and NULL are refused too. */
-static int check_range(const char *who, const char *what, size_t i, const void *p, size_t bytes, size_t align,
-                       int *device) {
+static int check_range(mc_ptrcache *pc, const char *who, const char *what, size_t i, const void *p, size_t bytes,
+                       size_t align, int *device) {
     if (!p || ((uintptr_t)p & (align - 1)) != 0) {
         fprintf(stderr, "[ERROR] %s: %s of tensor %zu is NULL or not %zu-byte aligned\n", who, what, i, align);
         return 0;
     }
     for (int end = 0; end < 2; end++) {
-        const void *q = end ? (const void *)((const uint8_t *)p + bytes - 1) : p;
-        struct cudaPointerAttributes at;
-        if (cudaPointerGetAttributes(&at, q) != cudaSuccess) {
-            (void)cudaGetLastError();
-            at.type = cudaMemoryTypeUnregistered;
-        }
-        if (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged) {
+        int dev = -1;
+        if (!mc_classify(pc, end ? (const void *)((const uint8_t *)p + bytes - 1) : p, &dev)) {
             fprintf(stderr, "[ERROR] %s: %s of tensor %zu is not device memory\n", who, what, i);
             return 0;
         }
-        if (*device < 0) *device = at.device;
-        if (at.device != *device) {
-            fprintf(stderr, "[ERROR] %s: %s of tensor %zu is on device %d, others on device %d\n", who, what, i,
-                    at.device, *device);
+        if (*device < 0) *device = dev;
+        if (dev != *device) {
+            fprintf(stderr, "[ERROR] %s: %s of tensor %zu is on device %d, others on device %d\n", who, what, i, dev,
+                    *device);
             return 0;
         }
     }
@@ -68,9 +62,10 @@ static int check_range(const char *who, const char *what, size_t i, const void *
 
 /* One small value in device memory of `device`. */
 static int check_scalar(const char *who, const char *what, const void *p, size_t bytes, size_t align, int device) {
-    int dev = device;
-    if (!check_range(who, what, 0, p, bytes, align, &dev)) return 0;
-    return dev == device;
+    mc_ptrcache pc;
+    pc.n = MC_PTRCACHE;   /* for two looks the ranges are not worth asking for */
+    memset(pc.r, 0, sizeof(pc.r));
+    return check_range(&pc, who, what, 0, p, bytes, align, &device);
 }
 
 /* Makes `device` current; returns the device to restore, or -2 on failure. */
@@ -141,6 +136,18 @@ static int current_device(const char *who) {
 }
 
 /* ------------------------------------------------------------------- norm */
+
+/* Units of a tensor: whole ones from its first 16-byte boundary on, the
+ * elements before that (*head) go with the first. */
+static int64_t norm_units(const void *x, size_t n, size_t size, int32_t *head) {
+    const size_t unit = OP_NORM_BYTES / size;
+    size_t h = ((16 - ((uintptr_t)x & 15)) & 15) / size;
+    if (h > n) h = n;
+    if (head) *head = (int32_t)h;
+    const size_t k = (n - h + unit - 1) / unit;
+    return (int64_t)(k ? k : n > 0);
+}
+
 MC_EXPORT falcom_norm *falcom_norm_create(const void *const *tensors, const size_t *numels, const int *dtypes,
                                           size_t n) {
     static const char *who = "falcom_norm_create";
@@ -150,6 +157,8 @@ MC_EXPORT falcom_norm *falcom_norm_create(const void *const *tensors, const size
     }
     int device = -1;
     int64_t n_units = 0;
+    mc_ptrcache pc;
+    pc.n = 0;
     for (size_t i = 0; i < n; i++) {
         if (dtypes[i] < 0 || dtypes[i] >= OP_NTYPES) {
             fprintf(stderr, "[ERROR] %s: tensor %zu has unknown type %d\n", who, i, dtypes[i]);
@@ -160,8 +169,12 @@ MC_EXPORT falcom_norm *falcom_norm_create(const void *const *tensors, const size
             return NULL;
         }
         const size_t sz = g_type_size[dtypes[i]];
-        if (numels[i] && !check_range(who, "address", i, tensors[i], numels[i] * sz, sz, &device)) return NULL;
-        n_units += (int64_t)((numels[i] + OP_NORM_UNIT - 1) / OP_NORM_UNIT);
+        if (numels[i] && !check_range(&pc, who, "address", i, tensors[i], numels[i] * sz, sz, &device)) return NULL;
+        n_units += norm_units(tensors[i], numels[i], sz, NULL);
+    }
+    if (n_units > (int64_t)UINT32_MAX / 2) {
+        fprintf(stderr, "[ERROR] %s: too many elements\n", who);
+        return NULL;
     }
     if (device < 0 && (device = current_device(who)) < 0) return NULL;
     falcom_norm *plan = (falcom_norm *)calloc(1, sizeof(*plan));
@@ -179,9 +192,10 @@ MC_EXPORT falcom_norm *falcom_norm_create(const void *const *tensors, const size
         t[i].x = tensors[i];
         t[i].n = (int64_t)numels[i];
         t[i].dtype = dtypes[i];
-        t[i].vec = ((uintptr_t)tensors[i] & 15) == 0;
-        const size_t k = (numels[i] + OP_NORM_UNIT - 1) / OP_NORM_UNIT;
-        for (size_t j = 0; j < k; j++) {
+        const size_t sz = g_type_size[dtypes[i]];
+        t[i].unit = (int32_t)(OP_NORM_BYTES / sz);
+        const int64_t k = norm_units(tensors[i], numels[i], sz, &t[i].head);
+        for (int64_t j = 0; j < k; j++) {
             u->tensor = (uint32_t)i;
             u->index = (uint32_t)j;
             u++;
@@ -273,6 +287,8 @@ static int add_span(span *s, size_t *k, const void *p, size_t bytes, int written
 static int check_tensors(const char *who, const falcom_adamw_tensor *t, size_t n, int bits, int64_t *step,
                          int *device, span *spans) {
     size_t k = 0;
+    mc_ptrcache pc;
+    pc.n = 0;
     for (size_t i = 0; i < n; i++) {
         if (t[i].param_type < 0 || t[i].param_type >= OP_NTYPES || t[i].grad_type < 0 || t[i].grad_type >= OP_NTYPES) {
             fprintf(stderr, "[ERROR] %s: tensor %zu has an unknown type\n", who, i);
@@ -285,13 +301,13 @@ static int check_tensors(const char *who, const falcom_adamw_tensor *t, size_t n
         if (t[i].n == 0) continue;
         const size_t ps = g_type_size[t[i].param_type], gs = g_type_size[t[i].grad_type];
         const size_t ss = bits == 32 ? 4 : 1, blocks = (t[i].n + OP_BLOCK - 1) / OP_BLOCK;
-        if (!check_range(who, "param", i, t[i].param, t[i].n * ps, ps, device) ||
-            !check_range(who, "grad", i, t[i].grad, t[i].n * gs, gs, device) ||
-            !check_range(who, "m", i, t[i].m, t[i].n * ss, ss, device) ||
-            !check_range(who, "v", i, t[i].v, t[i].n * ss, ss, device))
+        if (!check_range(&pc, who, "param", i, t[i].param, t[i].n * ps, ps, device) ||
+            !check_range(&pc, who, "grad", i, t[i].grad, t[i].n * gs, gs, device) ||
+            !check_range(&pc, who, "m", i, t[i].m, t[i].n * ss, ss, device) ||
+            !check_range(&pc, who, "v", i, t[i].v, t[i].n * ss, ss, device))
             return 0;
-        if (bits == 8 && (!check_range(who, "m_scale", i, t[i].m_scale, 4 * blocks, 4, device) ||
-                          !check_range(who, "v_scale", i, t[i].v_scale, 4 * blocks, 4, device)))
+        if (bits == 8 && (!check_range(&pc, who, "m_scale", i, t[i].m_scale, 4 * blocks, 4, device) ||
+                          !check_range(&pc, who, "v_scale", i, t[i].v_scale, 4 * blocks, 4, device)))
             return 0;
         add_span(spans, &k, t[i].param, t[i].n * ps, 1);
         add_span(spans, &k, t[i].grad, t[i].n * gs, 0);
@@ -302,7 +318,7 @@ static int check_tensors(const char *who, const falcom_adamw_tensor *t, size_t n
             add_span(spans, &k, t[i].v_scale, 4 * blocks, 1);
         }
     }
-    if (!check_range(who, "step", n, step, sizeof(*step), 8, device)) return 0;
+    if (!check_range(&pc, who, "step", n, step, sizeof(*step), 8, device)) return 0;
     add_span(spans, &k, step, sizeof(*step), 1);
     if (!spans_disjoint(spans, k)) {
         fprintf(stderr, "[ERROR] %s: an array that is written overlaps another array\n", who);

@@ -24,8 +24,7 @@ extern "C" {
  * elements): not its states, its states only, or all. */
 enum { OP_RAGGED = 0, OP_STATES = 1, OP_ALIGNED = 2 };
 
-/* A unit is a run of elements of one tensor: one warp's work at a time for
- * the norm, one CTA's for AdamW. */
+/* A unit is a run of elements of one tensor, one CTA's work at a time. */
 typedef struct {
     uint32_t tensor;   /* index into the plan's tensors */
     uint32_t index;    /* unit number inside the tensor */
@@ -35,7 +34,9 @@ typedef struct {
     const void *x;
     int64_t n;
     int32_t dtype;
-    int32_t vec;       /* 16-byte loads allowed */
+    int32_t head;      /* elements before the first 16-byte boundary (all of a short tensor) */
+    int32_t unit;      /* elements of a unit */
+    int32_t pad;
 } op_norm_tensor;
 
 typedef struct {
@@ -53,7 +54,7 @@ typedef struct {
 typedef struct {
     const op_norm_tensor *tensors;
     const op_unit *units;
-    int64_t n_units;
+    uint32_t n_units;
     double scale, max_norm;
     float *out;
     uint32_t *ticket;      /* 0 between calls */
@@ -75,7 +76,7 @@ typedef struct {
     int32_t advance;       /* this launch's last CTA counts the step */
 } op_adamw_launch;
 
-#define OP_NORM_UNIT 2048
+#define OP_NORM_BYTES 32768   /* of a unit */
 #define OP_ADAMW_UNIT (OP_WARPS * OP_BLOCK)
 
 uint32_t mc_op_hash(uint32_t x);

@@ -33,6 +33,8 @@ from . import build as _build
 
 _TYPES = {torch.float32: abi.TYPE_F32, torch.bfloat16: abi.TYPE_BF16, torch.float16: abi.TYPE_F16}
 _libs: Dict[str, ctypes.CDLL] = {}
+# (device index) -> cudaStream_t; the public route through a Stream object takes 2 us
+_current_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _library(path: Optional[str]) -> ctypes.CDLL:
@@ -58,6 +60,7 @@ def _dense_strides(t: torch.Tensor) -> Optional[tuple]:
 
 def _check_list(tensors: Sequence[torch.Tensor], what: str) -> List[torch.Tensor]:
     tensors = list(tensors)
+    device = None
     for i, t in enumerate(tensors):
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{what} {i} is not a tensor")
@@ -65,14 +68,16 @@ def _check_list(tensors: Sequence[torch.Tensor], what: str) -> List[torch.Tensor
             raise ValueError(f"{what} {i} is {t.dtype}: float32, bfloat16 or float16 is wanted")
         if not t.is_cuda:
             raise ValueError(f"{what} {i} is on {t.device}: a CUDA device is wanted")
-        if t.device != tensors[0].device:
-            raise ValueError(f"{what} {i} is on {t.device}, the first on {tensors[0].device}")
-        if t.numel() and _dense_strides(t) is None:
+        device = t.device if device is None else device
+        if t.device != device:
+            raise ValueError(f"{what} {i} is on {t.device}, the first on {device}")
+        if not t.is_contiguous() and t.numel() and _dense_strides(t) is None:
             raise ValueError(f"{what} {i} has gaps or repeats in memory (strides {t.stride()})")
     return tensors
 
 
 def _device_of(tensors: Sequence[torch.Tensor]) -> torch.device:
+    """Their device, with its index."""
     return tensors[0].device if tensors else torch.device("cuda", torch.cuda.current_device())
 
 
@@ -105,7 +110,11 @@ class GradNorm:
         if not self._h:
             raise RuntimeError("falcom_norm_create failed")
         self._work_words = -(-self.lib.falcom_norm_work_bytes(self._h) // 8)
-        self._work: Dict[int, torch.Tensor] = {}
+        self._work: Dict[int, torch.Tensor] = {}      # by stream
+        self._captured: List[torch.Tensor] = []       # in use by graphs from then on
+        # one each for the first captured calls, so that their graphs need not clear theirs
+        self._spare = list(torch.zeros(8, self._work_words, dtype=torch.int64, device=self.device))
+        torch.cuda.current_stream(self.device).synchronize()
 
     def __call__(self, max_norm: float = math.inf, grad_scale: float = 1.0) -> torch.Tensor:
         if not self._h:
@@ -114,10 +123,13 @@ class GradNorm:
             raise ValueError(f"max_norm must be positive, got {max_norm}")
         if not math.isfinite(grad_scale):
             raise ValueError(f"grad_scale must be finite, got {grad_scale}")
-        stream = torch.cuda.current_stream(self.device).cuda_stream
+        stream = _current_stream(self.device.index)
         if torch.cuda.is_current_stream_capturing():
-            # of the graph's own memory, zeroed by the graph
-            work = torch.zeros(self._work_words, dtype=torch.int64, device=self.device)
+            if self._spare:
+                self._captured.append(self._spare.pop())
+                work = self._captured[-1]
+            else:   # of the graph's own memory, cleared by the graph
+                work = torch.zeros(self._work_words, dtype=torch.int64, device=self.device)
         else:
             work = self._work.get(stream)
             if work is None:
@@ -165,7 +177,8 @@ class AdamW:
         if len(self.grads) != n:
             raise ValueError(f"{n} parameters and {len(self.grads)} gradients")
         for i, (p, g) in enumerate(zip(self.params, self.grads)):
-            if p.shape != g.shape or (p.numel() and _dense_strides(p) != _dense_strides(g)):
+            both = p.is_contiguous() and g.is_contiguous()
+            if p.shape != g.shape or (not both and p.numel() and _dense_strides(p) != _dense_strides(g)):
                 raise ValueError(f"gradient {i} has shape {tuple(g.shape)} and strides {g.stride()}, its parameter "
                                  f"{tuple(p.shape)} and {p.stride()}")
         self.device = _device_of(self.params)
@@ -213,6 +226,8 @@ class AdamW:
         if not self._h:
             raise RuntimeError("falcom_adamw_create failed")
         self._args = abi.AdamWArgsC()
+        self._args_ref = ctypes.byref(self._args)
+        self._given = None
         self._streams = set()
 
     def _check_hyper(self, lr: float, grad_scale: float) -> None:
@@ -225,7 +240,6 @@ class AdamW:
         if not abs(grad_scale) < 3.4e38:
             raise ValueError(f"grad_scale must be finite as a float32, got {grad_scale}")
 
-    @torch.no_grad()
     def step(self, lr: Union[None, float, torch.Tensor] = None, grad_scale: float = 1.0,
              clip: Optional[torch.Tensor] = None) -> None:
         """One step on the gradients as they are now, times grad_scale and, if
@@ -237,18 +251,20 @@ class AdamW:
         a = self._args
         on_device = isinstance(lr, torch.Tensor)
         rate = self.lr if lr is None or on_device else float(lr)
-        self._check_hyper(rate, grad_scale)
-        a.lr, a.beta1, a.beta2, a.eps = rate, self.beta1, self.beta2, self.eps
-        a.grad_scale, a.seed = grad_scale, self.seed
+        given = (rate, self.beta1, self.beta2, self.eps, grad_scale, self.seed)
+        if given != self._given:
+            self._check_hyper(rate, grad_scale)
+            a.lr, a.beta1, a.beta2, a.eps, a.grad_scale, a.seed = given
+            self._given = given
         a.lr_device = _scalar_input(lr, 1, self.device, "lr") if on_device else None
         a.clip = _scalar_input(clip, 2, self.device, "clip") if clip is not None else None
-        stream = torch.cuda.current_stream(self.device)
-        if stream.cuda_stream not in self._streams and not torch.cuda.is_current_stream_capturing():
+        stream = _current_stream(self.device.index)
+        if stream not in self._streams and not torch.cuda.is_current_stream_capturing():
             # the allocator may not reuse the states' memory under this stream's work
             for t in self.state.values():
-                t.record_stream(stream)
-            self._streams.add(stream.cuda_stream)
-        rc = self.lib.falcom_adamw_step(self._h, ctypes.byref(a), stream.cuda_stream)
+                t.record_stream(torch.cuda.current_stream(self.device))
+            self._streams.add(stream)
+        rc = self.lib.falcom_adamw_step(self._h, self._args_ref, stream)
         if rc != 0:
             raise RuntimeError(f"falcom_adamw_step failed ({rc})")
         if self._autograd:

@@ -15,13 +15,14 @@ from tests.emu import build as base  # noqa: E402
 from tests.emu import prep  # noqa: E402
 
 BUILD = os.path.join(HERE, "_build_optim")
-INPUTS = [os.path.join(base.CSRC, f) for f in ("mc_optim.c", "mc_optim.cu", "mc_optim.h")] + \
+INPUTS = [os.path.join(base.CSRC, f) for f in ("mc_optim.c", "mc_optim.cu", "mc_optim.h", "mc_util.c", "mc_internal.h")] + \
          [os.path.join(base.INCLUDE, "falcom_b200.h")] + \
          [os.path.join(HERE, f) for f in ("emu.h", "emu_optim.h", "fake_cudart.cpp", "prep.py", "build_optim.py")]
 
 LD_STREAM = ' if (((uintptr_t)p) & (sizeof(*p) - 1)) abort(); return *p; '
 # host bodies of the inline-PTX helpers
 BODIES = {
+    "prefetch": " (void)p; ",
     "pdl_wait": "",
     "pdl_release": "",
     "smem_u32": " return emu_smem_u32(p); ",
@@ -85,8 +86,11 @@ def build() -> str:
         f.write(s)
     inc = ["-I" + HERE, "-I" + base.INCLUDE, "-I" + base.CSRC, "-I" + os.path.join(base.CUDA, "include")]
     common = ["-O1", "-g", "-fPIC", "-fvisibility=hidden", *base.SAN, *inc]
-    host = os.path.join(BUILD, "mc_optim.o")
-    cmds, objs = [["gcc", "-std=gnu11", *common, "-c", os.path.join(base.CSRC, "mc_optim.c"), "-o", host]], [host]
+    cmds, objs = [], []
+    for src in ("mc_optim.c", "mc_util.c"):
+        o = os.path.join(BUILD, src + ".o")
+        cmds.append(["gcc", "-std=gnu11", *common, "-c", os.path.join(base.CSRC, src), "-o", o])
+        objs.append(o)
     for path in (kern, os.path.join(HERE, "fake_cudart.cpp")):
         o = os.path.join(BUILD, os.path.basename(path) + ".o")
         cmds.append(["g++", "-std=c++17", "-ffp-contract=off", *common, "-c", path, "-o", o])

@@ -410,7 +410,7 @@ MC_EXPORT falcom_adamw *falcom_adamw_create(const falcom_adamw_tensor *tensors, 
     for (int c = 0; c < OP_NTYPES * OP_NTYPES; c++) {
         plan->n_units[c] = counts[c];
         if (counts[c]) plan->last = c;
-        plan->grid[c] = mc_op_adamw_grid(counts[c], sms, state_bits);
+        plan->grid[c] = mc_op_adamw_grid(counts[c], sms, state_bits, c / OP_NTYPES, c % OP_NTYPES);
     }
     return plan;
 }
@@ -442,7 +442,10 @@ MC_EXPORT int falcom_adamw_step(falcom_adamw *plan, const falcom_adamw_args *a, 
     L.beta2 = a->beta2;
     L.b1.x = L.b1.y = (float)a->beta1;
     L.b2.x = L.b2.y = (float)a->beta2;
-    L.b2root = (float)sqrt(a->beta2);
+    L.b1c.x = L.b1c.y = (float)(1.0 - a->beta1);
+    L.one.x = L.one.y = 1.0f;
+    L.minus_b2.x = L.minus_b2.y = -L.b2.x;
+    L.minus_b2c.x = L.minus_b2c.y = -(float)(1.0 - a->beta2);
     L.eps.x = L.eps.y = (float)a->eps;
     L.scale = (float)a->grad_scale;
     L.seed_key = mc_op_hash(mc_op_hash((uint32_t)a->seed ^ 0x9E3779B9u) ^ (uint32_t)(a->seed >> 32));

@@ -70,8 +70,8 @@ typedef struct {
     const float *lr_dev;   /* NULL, or the learning rate */
     uint32_t *ticket;      /* 0 between calls */
     double lr, beta1, beta2;
-    float2 b1, b2, eps;    /* twice each, for two-element operations */
-    float b2root, scale;   /* sqrt(beta2) */
+    float2 b1, b1c, b2, eps, minus_b2, minus_b2c, one;   /* twice each, for two-element operations; c: 1 - */
+    float scale;
     uint32_t seed_key;     /* hash of the seed */
     int32_t advance;       /* this launch's last CTA counts the step */
 } op_adamw_launch;
@@ -81,7 +81,7 @@ typedef struct {
 
 uint32_t mc_op_hash(uint32_t x);
 int mc_op_norm_grid(int64_t n_units, int sms);
-int mc_op_adamw_grid(int64_t n_units, int sms, int bits);
+int mc_op_adamw_grid(int64_t n_units, int sms, int bits, int ptype, int gtype);
 /* Both return a CUDA error code (0: queued). */
 int mc_launch_norm(const op_norm_launch *L, int grid, void *stream);
 int mc_launch_adamw(const op_adamw_launch *L, int bits, int ptype, int gtype, int grid, void *stream);

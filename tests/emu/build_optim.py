@@ -48,6 +48,8 @@ BODIES = {
     fprintf(stderr, "emu: a barrier never completed\\n");
     abort();
 """,
+    "add2": " return make_float2(a.x + b.x, a.y + b.y); ",
+    "rsqrt_fast": " return 1.0f / sqrtf(x); ",
     "mul2": " return make_float2(a.x * b.x, a.y * b.y); ",
     "fma2": " return make_float2(fmaf(a.x, b.x, c.x), fmaf(a.y, b.y, c.y)); ",
     "sqrt_fast": " return sqrtf(x); ",

@@ -118,10 +118,15 @@ static uint8_t *upload(const char *who, int device, const uint8_t *host, size_t 
     return d;
 }
 
+/* A collector may drop a plan while some stream is being captured: in the
+ * relaxed mode freeing does not end the capture. */
 static void release(uint8_t *table, int device) {
     const int prev = enter(device);
     if (prev == -2) return;
+    enum cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    const int relaxed = cudaThreadExchangeStreamCaptureMode(&mode) == cudaSuccess;
     cudaFree(table);   /* waits for the device's work first */
+    if (relaxed) cudaThreadExchangeStreamCaptureMode(&mode);
     leave(prev, device);
 }
 

@@ -8,12 +8,13 @@ instance with the weighted aggregate fused into the decode
 (``falcom_set_aggregate``), and one sum all-reduce of the flat aggregate over
 NCCL finishes the global update.
 
-Everything here but PeerAggregate is plain host logic (which clients a rank
+Everything here but PeerAggregate and ServerAdamW is plain host logic (which clients a rank
 owns, their weights, the aggregate layout and the collective); it runs the
 same under the ``gloo`` backend on CPU tensors.  PeerAggregate maps the
 aggregate buffers between the ranks' GPUs for the two NVLink peer-memory
 sums (the reduce-scatter fused into the decoder, or the one-shot in-place
-all-reduce kernel).
+all-reduce kernel); ServerAdamW takes an optimiser step on the global model
+with the finished aggregate.
 """
 from __future__ import annotations
 
@@ -324,6 +325,62 @@ class PeerAggregate:
         for p in self.local.values():
             self.rt.cudaFree(p)
         self.local = {}
+
+
+class ServerAdamW:
+    """The server's optimiser step: AdamW on the global model with the round's
+    aggregate as the gradient, after the aggregate is complete on every rank
+    (allreduce_aggregate, ChunkedAllreduce.wait or PeerAggregate.finish).
+
+    `weights` and `aggregate` are flat float32 tensors on the GPU in the
+    layout's order and offsets.  The aggregate of weight differences is the
+    negative of a gradient, hence grad_scale = -1; pass 1 for clients that
+    send gradients.  Tensors with more than one dimension decay
+    (`decays(name, shape)` says otherwise), `names` restricts the step to
+    some of the tensors, state_bits = 8 holds the moments in a byte each, and
+    max_norm clips the whole aggregate's norm first; an aggregate that is not
+    finite is then skipped.
+
+    Every rank steps its own copy of the weights: the step's bits depend on
+    the aggregate's alone, so copies that were equal stay equal.  Plans hold
+    addresses, so `weights` and `aggregate` must stay where they are."""
+
+    def __init__(self, layout: AggregateLayout, weights, aggregate, lr: float = 1e-3, betas=(0.9, 0.999),
+                 eps: float = 1e-8, weight_decay: float = 0.0, state_bits: int = 32, max_norm: float = None,
+                 grad_scale: float = -1.0, decays=None, names: Sequence[str] = None, seed: int = 0,
+                 lib_path: str = None):
+        from . import optim
+        for what, t in (("weights", weights), ("aggregate", aggregate)):
+            if t.dim() != 1 or t.numel() < layout.total or not t.is_contiguous():
+                raise ValueError(f"{what} must be flat and contiguous, at least {layout.total} elements, "
+                                 f"got {tuple(t.shape)}")
+        wanted = set(layout.names if names is None else names)
+        if wanted - set(layout.names):
+            raise ValueError(f"not in the layout: {sorted(wanted - set(layout.names))}")
+        decays = decays or (lambda name, shape: len(shape) > 1)
+        items = [(n, s, o) for n, s, o in zip(layout.names, layout.shapes, layout.offsets) if n in wanted]
+        spans = [(o, o + int(np.prod(s))) for _, s, o in items]
+        self.names = [n for n, _, _ in items]
+        self.max_norm, self.grad_scale = max_norm, float(grad_scale)
+        grads = [aggregate[a:b] for a, b in spans]
+        self.norm = optim.GradNorm(grads, lib_path=lib_path) if max_norm is not None else None
+        self.opt = optim.AdamW([weights[a:b] for a, b in spans], grads, lr=lr, betas=betas, eps=eps,
+                               weight_decay=[weight_decay if decays(n, s) else 0.0 for n, s, _ in items],
+                               state_bits=state_bits, seed=seed, lib_path=lib_path)
+
+    def step(self, lr=None):
+        """One step, queued on the current stream.  Returns GradNorm's [norm,
+        coefficient] on the device, or None without max_norm."""
+        clip = None
+        if self.norm is not None:
+            clip = self.norm(max_norm=self.max_norm, grad_scale=self.grad_scale)
+        self.opt.step(lr=lr, grad_scale=self.grad_scale, clip=clip)
+        return clip
+
+    def close(self) -> None:
+        if self.norm is not None:
+            self.norm.close()
+        self.opt.close()
 
 
 class _DeviceFloats:

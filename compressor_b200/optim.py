@@ -68,6 +68,9 @@ def _check_list(tensors: Sequence[torch.Tensor], what: str) -> List[torch.Tensor
             raise ValueError(f"{what} {i} is {t.dtype}: float32, bfloat16 or float16 is wanted")
         if not t.is_cuda:
             raise ValueError(f"{what} {i} is on {t.device}: a CUDA device is wanted")
+        if t.layout != torch.strided or t.is_neg():
+            raise ValueError(f"{what} {i} does not hold its values as they are ({t.layout}, negation pending: "
+                             f"{t.layout == torch.strided and t.is_neg()})")
         device = t.device if device is None else device
         if t.device != device:
             raise ValueError(f"{what} {i} is on {t.device}, the first on {device}")
@@ -294,6 +297,11 @@ class AdamW:
         for p, o in zip(self.params, self.offsets):
             out.append(tuple(flat[k][o:o + p.numel()].clone().as_strided(p.shape, p.stride()) for k in "mv"))
         return out
+
+    def errors(self) -> int:
+        """Nonzero once a step gave up waiting for its own memory copies (8-bit
+        states; never seen).  Synchronises with the device's default stream."""
+        return self.lib.falcom_adamw_errors(self._h) if self._h else 0
 
     def close(self) -> None:
         if self._h:

@@ -361,10 +361,11 @@ void falcom_norm_destroy(falcom_norm *plan);
  *   p' = (1 - lr * weight_decay) p
  *        - lr / (1 - beta1^t) * m' / (sqrt(v') / sqrt(1 - beta2^t) + eps)
  * in float32 from the element types' values (the coefficients of t, lr and
- * the betas are formed in 64 bits and rounded once; the root and the quotient
- * are within two units in the last place, and a v' under 2^-126 counts as 0
- * in the root), p' rounded to the parameter's type at the end.  A server
- * whose aggregate is the sum of weight *differences* passes grad_scale = -1.
+ * the betas are formed in 64 bits and rounded once; root and quotient are
+ * within two units in the last place, and a v' under 2^-100 may count as
+ * less than it is, down to 0, in the root), p' rounded to the parameter's
+ * type at the end.  A server whose aggregate is the sum of weight
+ * *differences* passes grad_scale = -1.
  *
  * state_bits = 32: m and v are float32[n].
  * state_bits = 8: m and v are one byte per element.  Every FALCOM_ADAMW_BLOCK
@@ -377,9 +378,11 @@ void falcom_norm_destroy(falcom_norm *plan);
  * nearest would hold sqrt(v) still: it moves by 0.05 % a step for beta2 =
  * 0.999, the codes are 6 to 12 % apart).  The random bits are a hash of
  * (seed, t, position), the position being 256 * (blocks of the plan's
- * earlier tensors) + the element's index: the same call on the same state
- * gives the same bits on every GPU.  A v > 0 never gets code 0, so no
- * denominator vanishes under a first moment that did not.  All-zero state
+ * earlier tensors) + the element's index.  g', m', v', the root, scales and
+ * codes are rounded operation by operation as written, nothing fused (the
+ * code is that of |x| * (448 / max), exactly rounded quotient), so any
+ * implementation of these formulas gets the same codes.  A v > 0 never gets
+ * code 0, so no denominator vanishes under a first moment that did not.  All-zero state
  * (codes and scales 0) is the start.  Of a block in which a new value of m
  * (of sqrt(v)) is infinite, NaN or 2^100 and more, m's (v's) scale becomes
  * NaN and its codes 0; one whose values are all below 2^-100 gets zeros.
@@ -393,7 +396,7 @@ void falcom_norm_destroy(falcom_norm *plan);
  * memory used instead of `lr`.
  *
  * falcom_adamw_create returns NULL (message on stderr) for state_bits other
- * than 32 and 8, NULL or misaligned addresses (param, grad: element size; m,
+ * than 32 and 8, more than 2^39 elements in a tensor, NULL or misaligned addresses (param, grad: element size; m,
  * v: 4 bytes with 32 bits; scales: 4; step: 8), unknown types, a negative or
  * non-finite weight decay, memory that is not device memory of one device,
  * arrays that are written and overlap any other array, or when allocation

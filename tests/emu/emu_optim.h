@@ -7,6 +7,9 @@ extern "C" inline __attribute__((used)) cudaError_t cudaDeviceGetAttribute(int *
     return cudaSuccess;
 }
 
+extern "C" inline __attribute__((used)) cudaError_t cudaThreadExchangeStreamCaptureMode(cudaStreamCaptureMode *) {
+    return cudaSuccess;
+}
 inline float emu_e4m3(unsigned code) {
     const int e = code >> 3 & 15, f = code & 7;
     float v = e ? ldexpf(1.0f + f / 8.0f, e - 7) : ldexpf(f / 8.0f, -6);

@@ -332,6 +332,12 @@ static int check_tensors(const char *who, const falcom_adamw_tensor *t, size_t n
     return 1;
 }
 
+static int64_t adamw_units(const falcom_adamw_tensor *t, int bits) {
+    const size_t unit = (size_t)OP_ADAMW_UNIT * (bits == 32 ? 1 : OP_ADAMW8_ROUNDS(g_type_size[t->param_type],
+                                                                                   g_type_size[t->grad_type]));
+    return (int64_t)((t->n + unit - 1) / unit);
+}
+
 MC_EXPORT falcom_adamw *falcom_adamw_create(const falcom_adamw_tensor *tensors, size_t n, int state_bits,
                                             int64_t *step) {
     static const char *who = "falcom_adamw_create";
@@ -351,7 +357,7 @@ MC_EXPORT falcom_adamw *falcom_adamw_create(const falcom_adamw_tensor *tensors, 
 
     int64_t counts[OP_NTYPES * OP_NTYPES] = {0}, total = 0;
     for (size_t i = 0; i < n; i++) {
-        const int64_t k = (int64_t)((tensors[i].n + OP_ADAMW_UNIT - 1) / OP_ADAMW_UNIT);
+        const int64_t k = adamw_units(&tensors[i], state_bits);
         counts[tensors[i].param_type * OP_NTYPES + tensors[i].grad_type] += k;
         total += k;
     }
@@ -393,8 +399,8 @@ MC_EXPORT falcom_adamw *falcom_adamw_create(const falcom_adamw_tensor *tensors, 
         else t[i].how = OP_ALIGNED;
         blocks += (int64_t)((a->n + OP_BLOCK - 1) / OP_BLOCK);
         const int c = a->param_type * OP_NTYPES + a->grad_type;
-        const size_t k = (a->n + OP_ADAMW_UNIT - 1) / OP_ADAMW_UNIT;
-        for (size_t j = 0; j < k; j++) {
+        const int64_t k = adamw_units(a, state_bits);
+        for (int64_t j = 0; j < k; j++) {
             fill[c]->tensor = (uint32_t)i;
             fill[c]->index = (uint32_t)j;
             fill[c]++;

@@ -78,6 +78,9 @@ typedef struct {
 
 #define OP_NORM_BYTES 32768   /* of a unit */
 #define OP_ADAMW_UNIT (OP_WARPS * OP_BLOCK)
+/* With 8-bit states a warp has so many blocks of a unit, by the sizes of
+ * parameter and gradient types. */
+#define OP_ADAMW8_ROUNDS(psize, gsize) ((psize) + (gsize) > 4 ? 1 : 2)
 
 uint32_t mc_op_hash(uint32_t x);
 int mc_op_norm_grid(int64_t n_units, int sms);

@@ -69,6 +69,13 @@ def test_adamw_shapes(emu, bits, name):
                  grad_scale=-1.0)
 
 
+@pytest.mark.parametrize("pk,gk", [("bf16", "bf16"), ("f16", "bf16")])
+@pytest.mark.parametrize("name", ["units", "shifted"])
+def test_adamw8_narrow_units(emu, name, pk, gk):
+    """Units of 16 blocks, whole, cut short and off their alignment."""
+    oc.run_adamw(emu, oc.case_tensors(emu, name, 8, pk, gk), 8, steps=2)
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_adamw_mixed_types(emu, bits):
     rng = np.random.default_rng(2)

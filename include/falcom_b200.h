@@ -382,10 +382,11 @@ void falcom_norm_destroy(falcom_norm *plan);
  * codes are rounded operation by operation as written, nothing fused (the
  * code is that of |x| * (448 / max), exactly rounded quotient), so any
  * implementation of these formulas gets the same codes.  A v > 0 never gets
- * code 0, so no denominator vanishes under a first moment that did not.  All-zero state
- * (codes and scales 0) is the start.  Of a block in which a new value of m
- * (of sqrt(v)) is infinite, NaN or 2^100 and more, m's (v's) scale becomes
- * NaN and its codes 0; one whose values are all below 2^-100 gets zeros.
+ * code 0, so no denominator vanishes under a first moment that did not.
+ * All-zero state (codes and scales 0) is the start.  Of a block in which a
+ * new value of m (of sqrt(v)) is infinite, NaN or 2^100 and more, m's (v's)
+ * scale becomes NaN and its codes 0, and an infinite v' makes its p' NaN; a
+ * block whose values are all below 2^-100 gets zeros.
  *
  * `step` is an int64 counter in device memory (0 at the start): a step reads
  * it, takes step number t = *step + 1 and writes it back, so a captured step
@@ -396,11 +397,11 @@ void falcom_norm_destroy(falcom_norm *plan);
  * memory used instead of `lr`.
  *
  * falcom_adamw_create returns NULL (message on stderr) for state_bits other
- * than 32 and 8, more than 2^39 elements in a tensor, NULL or misaligned addresses (param, grad: element size; m,
- * v: 4 bytes with 32 bits; scales: 4; step: 8), unknown types, a negative or
- * non-finite weight decay, memory that is not device memory of one device,
- * arrays that are written and overlap any other array, or when allocation
- * fails.  The steps of one plan must be ordered (one stream, or events).
+ * than 32 and 8, more than 2^39 elements in a tensor, NULL or misaligned
+ * addresses (param, grad: element size; m, v: 4 bytes with 32 bits; scales:
+ * 4; step: 8), unknown types, a negative or non-finite weight decay, memory
+ * that is not device memory of one device, arrays that are written and
+ * overlap any other array, or when allocation fails.  The steps of one plan must be ordered (one stream, or events).
  * falcom_adamw_step returns 0; ERROR_INVALID_PARAM for lr < 0 or not finite,
  * betas outside [0, 1), eps not positive as a float32, a non-finite
  * grad_scale, or a clip or lr_device that is not device memory of the plan's

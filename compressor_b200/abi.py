@@ -526,7 +526,8 @@ def bind_extensions(lib: ctypes.CDLL) -> None:
     lib.falcom_state_load.argtypes = [c_vp, ctypes.c_char_p]
     lib.falcom_state_load.restype = ctypes.c_int
     bind_replay(lib)
-    bind_optim(lib)
+    if hasattr(lib, "falcom_adamw_create"):   # builds of the codec alone lack the optimiser entry points
+        bind_optim(lib)
 
 
 TYPE_F32, TYPE_BF16, TYPE_F16 = range(3)

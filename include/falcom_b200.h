@@ -406,7 +406,9 @@ void falcom_norm_destroy(falcom_norm *plan);
  * betas outside [0, 1), eps not positive as a float32, a non-finite
  * grad_scale, or a clip or lr_device that is not device memory of the plan's
  * device; ERROR_COMPRESSION when a launch fails or an error is pending, as
- * above.  One launch per pair of parameter and gradient type in the list. */
+ * above.  One launch per pair of parameter and gradient type in the list, in
+ * a fixed order; should one fail, the pairs before it have been stepped and
+ * the counter has not. */
 #define FALCOM_ADAMW_BLOCK 256
 typedef struct falcom_adamw_tensor {
     void *param;

@@ -60,12 +60,20 @@ static int check_range(mc_ptrcache *pc, const char *who, const char *what, size_
     return 1;
 }
 
-/* One small value in device memory of `device`. */
-static int check_scalar(const char *who, const char *what, const void *p, size_t bytes, size_t align, int device) {
-    mc_ptrcache pc;
-    pc.n = MC_PTRCACHE;   /* for two looks the ranges are not worth asking for */
-    memset(pc.r, 0, sizeof(pc.r));
-    return check_range(&pc, who, what, 0, p, bytes, align, &device);
+/* An argument of a run or step: a few values in device memory of `device`,
+ * by its first byte (the driver's allocations are larger). */
+static int check_scalar(const char *who, const char *what, const void *p, size_t align, int device) {
+    struct cudaPointerAttributes at;
+    if (p && ((uintptr_t)p & (align - 1)) == 0) {
+        if (cudaPointerGetAttributes(&at, p) == cudaSuccess) {
+            if ((at.type == cudaMemoryTypeDevice || at.type == cudaMemoryTypeManaged) && at.device == device) return 1;
+        } else {
+            (void)cudaGetLastError();
+        }
+    }
+    fprintf(stderr, "[ERROR] %s: %s is NULL, not %zu-byte aligned or not device memory of device %d\n", who, what,
+            align, device);
+    return 0;
 }
 
 /* Makes `device` current; returns the device to restore, or -2 on failure. */
@@ -231,8 +239,8 @@ MC_EXPORT int falcom_norm_run(falcom_norm *plan, double scale, double max_norm, 
         fprintf(stderr, "[ERROR] %s: invalid arguments\n", who);
         return ERROR_INVALID_PARAM;
     }
-    if (!check_scalar(who, "out", out, 2 * sizeof(float), 4, plan->device) ||
-        !check_scalar(who, "work", work, falcom_norm_work_bytes(plan), 8, plan->device))
+    if (!check_scalar(who, "out", out, 4, plan->device) ||
+        !check_scalar(who, "work", work, 8, plan->device))
         return ERROR_INVALID_PARAM;
     if (error_pending(who)) return ERROR_COMPRESSION;
     const int prev = enter(plan->device);
@@ -434,8 +442,8 @@ MC_EXPORT int falcom_adamw_step(falcom_adamw *plan, const falcom_adamw_args *a, 
         fprintf(stderr, "[ERROR] %s: invalid arguments\n", who);
         return ERROR_INVALID_PARAM;
     }
-    if ((a->clip && !check_scalar(who, "clip", a->clip, 2 * sizeof(float), 4, plan->device)) ||
-        (a->lr_device && !check_scalar(who, "lr_device", a->lr_device, sizeof(float), 4, plan->device)))
+    if ((a->clip && !check_scalar(who, "clip", a->clip, 4, plan->device)) ||
+        (a->lr_device && !check_scalar(who, "lr_device", a->lr_device, 4, plan->device)))
         return ERROR_INVALID_PARAM;
     if (error_pending(who)) return ERROR_COMPRESSION;
     const int prev = enter(plan->device);

@@ -37,6 +37,14 @@ _libs: Dict[str, ctypes.CDLL] = {}
 _current_stream = torch._C._cuda_getCurrentRawStream
 
 
+def _capturing(index: int) -> bool:
+    """Whether the current stream of that device is being captured."""
+    if torch.cuda.current_device() == index:
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(index):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _library(path: Optional[str]) -> ctypes.CDLL:
     path = path or _build.OUT
     if path not in _libs:
@@ -127,7 +135,7 @@ class GradNorm:
         if not math.isfinite(grad_scale):
             raise ValueError(f"grad_scale must be finite, got {grad_scale}")
         stream = _current_stream(self.device.index)
-        if torch.cuda.is_current_stream_capturing():
+        if _capturing(self.device.index):
             if self._spare:
                 self._captured.append(self._spare.pop())
                 work = self._captured[-1]
@@ -262,7 +270,7 @@ class AdamW:
         a.lr_device = _scalar_input(lr, 1, self.device, "lr") if on_device else None
         a.clip = _scalar_input(clip, 2, self.device, "clip") if clip is not None else None
         stream = _current_stream(self.device.index)
-        if stream not in self._streams and not torch.cuda.is_current_stream_capturing():
+        if stream not in self._streams and not _capturing(self.device.index):
             # the allocator may not reuse the states' memory under this stream's work
             for t in self.state.values():
                 t.record_stream(torch.cuda.current_stream(self.device))

@@ -186,3 +186,30 @@ def test_refuses_what_does_not_hold_its_values(optim):
     empty = optim.AdamW([], [])
     empty.step()
     assert int(empty.state["step"]) == 1
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_two_plans_at_once(optim, bits):
+    """Two optimisers with their norms on two streams at once leave what they leave one after the other."""
+    def make():
+        gen = torch.Generator("cuda").manual_seed(8)
+        sets = []
+        for n in (700_001, 1_300_000):
+            p = torch.randn(n, device="cuda", generator=gen)
+            g = torch.randn(n, device="cuda", generator=gen)
+            sets.append((p, optim.AdamW([p], [g], state_bits=bits), optim.GradNorm([g])))
+        return sets
+
+    apart, together = make(), make()
+    for _, opt, norm in apart:
+        for _ in range(30):
+            opt.step(clip=norm(max_norm=0.5))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(30):
+        for s, (_, opt, norm) in zip(streams, together):
+            with torch.cuda.stream(s):
+                opt.step(clip=norm(max_norm=0.5))
+    torch.cuda.synchronize()
+    for (p, o, _), (q, r, _) in zip(apart, together):
+        assert torch.equal(p, q) and all(torch.equal(o.state[k].view(torch.uint8), r.state[k].view(torch.uint8)) for k in o.state)

@@ -121,6 +121,7 @@ class GradNorm:
         if not self._h:
             raise RuntimeError("falcom_norm_create failed")
         self._work_words = -(-self.lib.falcom_norm_work_bytes(self._h) // 8)
+        self._pair = torch.empty(2, dtype=torch.float32, device=self.device)   # a result's shape
         self._work: Dict[int, torch.Tensor] = {}      # by stream
         self._captured: List[torch.Tensor] = []       # in use by graphs from then on
         # one each for the first captured calls, so that their graphs need not clear theirs
@@ -145,7 +146,7 @@ class GradNorm:
             work = self._work.get(stream)
             if work is None:
                 work = self._work[stream] = torch.zeros(self._work_words, dtype=torch.int64, device=self.device)
-        out = torch.empty(2, dtype=torch.float32, device=self.device)
+        out = torch.empty_like(self._pair)
         rc = self.lib.falcom_norm_run(self._h, grad_scale, max_norm, out.data_ptr(), work.data_ptr(), stream)
         if rc != 0:
             raise RuntimeError(f"falcom_norm_run failed ({rc})")

@@ -53,8 +53,3 @@ inline void emu_mbar_arrive(uint32_t bar) {
 inline bool emu_mbar_done(uint32_t bar, uint32_t parity) {
     return (__atomic_load_n((uint64_t *)emu_smem_ptr(bar), __ATOMIC_SEQ_CST) & 1) != parity;
 }
-inline double __longlong_as_double(long long v) {
-    double d;
-    memcpy(&d, &v, 8);
-    return d;
-}

@@ -40,8 +40,14 @@ def codes_of(x, chance, least):
     return code.astype(np.uint8), np.where(live, top * F(1 / 448.0), F(0))
 
 
-def check_maxima(backend, pk, gk, shift=0, state_shift=0):
-    """One step over every pair of maxima, without gradients."""
+# gradients of an element whose states are zero: roots so small that a
+# 2^-100th of either is no float32 number
+VANISHING = [2.0 ** -50, 2.0 ** -55, 2.0 ** -62]
+
+
+def check_maxima(backend, pk, gk, shift=0, state_shift=0, gradient=0.0):
+    """One step over every pair of maxima.  `gradient`: of one element, whose
+    states are zero, in the blocks whose roots reach 1."""
     pairs = [(a, b) for a in M_TOPS for b in V_TOPS]
     blocks = len(pairs) + 1
     n = blocks * BLOCK - 100                       # the last block is short
@@ -55,6 +61,7 @@ def check_maxima(backend, pk, gk, shift=0, state_shift=0):
     ms = (tops[:, 0] / 128).astype(F)              # 256 * scale / 2 is the maximum
     vs = (tops[:, 1] / 128).astype(F)
     g = np.zeros((blocks, BLOCK))
+    g[:len(pairs), 28] = gradient * (tops[:len(pairs), 1] >= 1.0)
     gs = oc.round_to(g.reshape(-1)[:n], gk)
     ps = oc.round_to(np.zeros(n), pk)
     dp, dg = oc.Placed(backend, ps, oc.SIZE[pk] * shift), oc.Placed(backend, gs, oc.SIZE[gk] * shift)

@@ -39,8 +39,9 @@ BODIES = {
 """,
     "copy_async4": " if ((char *)dst < (char *)emu_cta->lo || (char *)(dst + 1) > (char *)emu_cta->hi) abort(); *dst = *src; ",
     "arrive_after_copies": " emu_mbar_arrive(bar); ",
-    "mbar_try_wait": " return emu_mbar_done(bar, parity); ",
-    "mbar_wait_long": """
+    "mbar_try_wait": " return emu_late_waits == 0 && emu_mbar_done(bar, parity); ",
+    "mbar_wait_some": """
+    if (emu_wait_is_late()) return false;
     for (int i = 0; i < 50000000; i++) {
         if (emu_mbar_done(bar, parity)) return true;
         std::this_thread::yield();

@@ -39,6 +39,17 @@ inline T __shfl_sync(unsigned, T v, int src) {   // emu_shfl knows lane ^ arg: f
 }
 inline int __all_sync(unsigned, int p) { return __ballot_sync(0xffffffffu, p) == 0xffffffffu; }
 
+// Test hook: so many lanes find that their wait has run out, whatever the
+// barrier says.
+inline std::atomic<int> emu_late_waits{0};
+extern "C" __attribute__((used, visibility("default"))) inline void emu_optim_late_waits(int n) { emu_late_waits = n; }
+inline bool emu_wait_is_late() {
+    int n = emu_late_waits;
+    while (n > 0 && !emu_late_waits.compare_exchange_weak(n, n - 1)) {
+    }
+    return n > 0;
+}
+
 // An mbarrier: arrivals expected, arrivals missing in this phase, phase.
 inline void emu_mbar_init(uint32_t bar, uint64_t count) {
     __atomic_store_n((uint64_t *)emu_smem_ptr(bar), count << 40 | count << 8, __ATOMIC_SEQ_CST);

@@ -487,7 +487,9 @@ MC_EXPORT int falcom_adamw_errors(falcom_adamw *plan) {
     const int prev = enter(plan->device);
     if (prev == -2) return ERROR_COMPRESSION;
     uint32_t word = 0;
-    const cudaError_t e = cudaMemcpy(&word, plan->table + 4, 4, cudaMemcpyDeviceToHost);
+    /* steps may be in flight on streams that the copy does not wait for */
+    cudaError_t e = cudaDeviceSynchronize();
+    if (e == cudaSuccess) e = cudaMemcpy(&word, plan->table + 4, 4, cudaMemcpyDeviceToHost);
     leave(prev, plan->device);
     if (e != cudaSuccess) return ERROR_COMPRESSION;
     return word != 0;

@@ -309,7 +309,8 @@ class AdamW:
 
     def errors(self) -> int:
         """Nonzero once a step gave up waiting for its own memory copies (8-bit
-        states; never seen).  Synchronises with the device's default stream."""
+        states; never seen): what it left is then not to be used.  Waits for
+        all work of the device."""
         return self.lib.falcom_adamw_errors(self._h) if self._h else 0
 
     def close(self) -> None:

@@ -430,8 +430,9 @@ typedef struct falcom_adamw falcom_adamw;
 falcom_adamw *falcom_adamw_create(const falcom_adamw_tensor *tensors, size_t n, int state_bits, int64_t *step);
 int falcom_adamw_step(falcom_adamw *plan, const falcom_adamw_args *args, void *stream);
 /* 1 when a step of the plan gave up waiting for its own memory copies (about
- * four seconds; its result is then not to be used), else 0.  Waits for the
- * legacy default stream's work. */
+ * four seconds; its result is then not to be used), else 0; negative when
+ * the device cannot be asked.  Waits for all work queued on the plan's
+ * device, so it does not belong inside a stream capture. */
 int falcom_adamw_errors(falcom_adamw *plan);
 void falcom_adamw_destroy(falcom_adamw *plan);
 

@@ -19,6 +19,7 @@ with the finished aggregate.
 from __future__ import annotations
 
 import ctypes
+import math
 from dataclasses import dataclass
 from typing import List, Sequence
 
@@ -327,6 +328,9 @@ class PeerAggregate:
         self.local = {}
 
 
+_STATISTICS = ("running_mean", "running_var", "num_batches_tracked")
+
+
 class ServerAdamW:
     """The server's optimiser step: AdamW on the global model with the round's
     aggregate as the gradient, after the aggregate is complete on every rank
@@ -341,6 +345,13 @@ class ServerAdamW:
     max_norm clips the whole aggregate's norm first; an aggregate that is not
     finite is then skipped.
 
+    Running statistics are no parameters: a step of about lr, whatever their
+    size, would take a small variance below zero.  Tensors named
+    running_mean, running_var or num_batches_tracked (`averaged(name, shape)`
+    says otherwise) get -grad_scale times the aggregate added, the clients'
+    average, and have no part in the norm; one that is not finite skips the
+    step too, where max_norm is given.
+
     Every rank steps its own copy of the weights: the step's bits depend on
     the aggregate's alone, so copies that were equal stay equal.  Plans hold
     addresses, so `weights` and `aggregate` must stay where they are."""
@@ -348,7 +359,8 @@ class ServerAdamW:
     def __init__(self, layout: AggregateLayout, weights, aggregate, lr: float = 1e-3, betas=(0.9, 0.999),
                  eps: float = 1e-8, weight_decay: float = 0.0, state_bits: int = 32, max_norm: float = None,
                  grad_scale: float = -1.0, decays=None, names: Sequence[str] = None, seed: int = 0,
-                 lib_path: str = None):
+                 lib_path: str = None, averaged=None):
+        import torch
         from . import optim
         for what, t in (("weights", weights), ("aggregate", aggregate)):
             if t.dim() != 1 or t.numel() < layout.total or not t.is_contiguous():
@@ -358,9 +370,17 @@ class ServerAdamW:
         if wanted - set(layout.names):
             raise ValueError(f"not in the layout: {sorted(wanted - set(layout.names))}")
         decays = decays or (lambda name, shape: len(shape) > 1)
+        averaged = averaged or (lambda name, shape: name.split(".")[-1] in _STATISTICS)
         items = [(n, s, o) for n, s, o in zip(layout.names, layout.shapes, layout.offsets) if n in wanted]
+        apart = [(n, s, o) for n, s, o in items if averaged(n, s)]
+        self.averaged = [n for n, _, _ in apart]
+        items = [i for i in items if i[0] not in set(self.averaged)]
         spans = [(o, o + int(np.prod(s))) for _, s, o in items]
         self.names = [n for n, _, _ in items]
+        self.weights, self.aggregate = weights, aggregate
+        # the averaged elements' places
+        self._places = torch.cat([torch.arange(o, o + int(np.prod(s))) for _, s, o in apart]).to(weights.device) \
+            if apart else None
         self.max_norm, self.grad_scale = max_norm, float(grad_scale)
         grads = [aggregate[a:b] for a, b in spans]
         self.norm = optim.GradNorm(grads, lib_path=lib_path) if max_norm is not None else None
@@ -374,7 +394,24 @@ class ServerAdamW:
         clip = None
         if self.norm is not None:
             clip = self.norm(max_norm=self.max_norm, grad_scale=self.grad_scale)
+        if self._places is not None:
+            clip = self._average(clip)
         self.opt.step(lr=lr, grad_scale=self.grad_scale, clip=clip)
+        return clip
+
+    def _average(self, clip):
+        """Adds the aggregate to the averaged tensors unless the step is to be
+        skipped; returns `clip`, its coefficient NaN if one of them is why."""
+        import torch
+        with torch.no_grad():
+            change = self.aggregate.index_select(0, self._places)
+            old = self.weights.index_select(0, self._places)
+            new = torch.add(old, change, alpha=-self.grad_scale)
+            if clip is not None:
+                skip = clip[1].isnan() | ~change.isfinite().all()
+                new = torch.where(skip, old, new)
+                clip = torch.stack([clip[0], torch.where(skip, math.nan, clip[1])])
+            self.weights.index_copy_(0, self._places, new)
         return clip
 
     def close(self) -> None:

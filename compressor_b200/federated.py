@@ -414,6 +414,11 @@ class ServerAdamW:
             self.weights.index_copy_(0, self._places, new)
         return clip
 
+    def errors(self) -> int:
+        """Nonzero once a step went wrong on the device (optim.AdamW.errors):
+        the weights are then not to be used.  Waits for all work of the device."""
+        return self.opt.errors()
+
     def close(self) -> None:
         if self.norm is not None:
             self.norm.close()

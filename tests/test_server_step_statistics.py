@@ -102,3 +102,10 @@ def test_the_models_statistics_are_found(seen, model, count):
     s = fed.ServerAdamW(layout, torch.zeros(layout.total), torch.zeros(layout.total))
     assert len(s.averaged) == count and not any("running" in n for n in s.names)
     assert len(s.names) + count == len(names)
+
+
+def test_errors_of_the_step_are_reported(seen):
+    w, a = _flat()
+    s = fed.ServerAdamW(LAYOUT, w, a)
+    s.opt.errors = lambda: 1
+    assert s.errors() == 1

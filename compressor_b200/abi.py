@@ -572,6 +572,8 @@ def bind_optim(lib: ctypes.CDLL) -> None:
     lib.falcom_norm_work_bytes.restype = ctypes.c_size_t
     lib.falcom_norm_run.argtypes = [c_vp, ctypes.c_double, ctypes.c_double, c_vp, c_vp, c_vp]
     lib.falcom_norm_run.restype = ctypes.c_int
+    lib.falcom_norm_graphs.argtypes = [c_vp]
+    lib.falcom_norm_graphs.restype = ctypes.c_int
     lib.falcom_norm_destroy.argtypes = [c_vp]
     lib.falcom_norm_destroy.restype = None
     lib.falcom_adamw_create.argtypes = [P(AdamWTensorC), ctypes.c_size_t, ctypes.c_int, c_vp]
@@ -580,6 +582,8 @@ def bind_optim(lib: ctypes.CDLL) -> None:
     lib.falcom_adamw_step.restype = ctypes.c_int
     lib.falcom_adamw_errors.argtypes = [c_vp]
     lib.falcom_adamw_errors.restype = ctypes.c_int
+    lib.falcom_adamw_graphs.argtypes = [c_vp]
+    lib.falcom_adamw_graphs.restype = ctypes.c_int
     lib.falcom_adamw_destroy.argtypes = [c_vp]
     lib.falcom_adamw_destroy.restype = None
 

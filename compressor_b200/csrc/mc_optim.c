@@ -6,6 +6,7 @@
 #include <cuda_runtime_api.h>
 #include <float.h>
 #include <math.h>
+#include <pthread.h>
 #include <stdio.h>
 #include <stdlib.h>
 #include <string.h>
@@ -15,19 +16,25 @@
 
 static const size_t g_type_size[OP_NTYPES] = {4, 2, 2};
 
-struct falcom_norm {
+/* What both kinds of plans start with. */
+typedef struct op_plan {
+    uint8_t *table;          /* device memory */
     int device;
+    int graphs;              /* captured calls whose graphs still exist (atomic) */
+    struct op_plan *next;    /* in the list of destroyed plans that graphs still use */
+} op_plan;
+
+struct falcom_norm {
+    op_plan base;     /* table: op_norm_tensor[n], then op_unit[n_units] */
     int grid;
     int64_t n_units;
-    uint8_t *table;   /* op_norm_tensor[n], then op_unit[n_units] */
     size_t units_at;
 };
 
 struct falcom_adamw {
-    int device;
+    op_plan base;     /* table: ticket, error word, op_adamw_tensor[n], op_unit[] of every type pair */
     int bits;
     int64_t *step;
-    uint8_t *table;   /* ticket, error word, op_adamw_tensor[n], op_unit[] of every type pair */
     size_t tensors_at, units_at;
     int64_t n_units[OP_NTYPES * OP_NTYPES];   /* by param_type * OP_NTYPES + grad_type */
     int grid[OP_NTYPES * OP_NTYPES];
@@ -128,14 +135,69 @@ static uint8_t *upload(const char *who, int device, const uint8_t *host, size_t 
 
 /* A collector may drop a plan while some stream is being captured: in the
  * relaxed mode freeing does not end the capture. */
-static void release(uint8_t *table, int device) {
-    const int prev = enter(device);
-    if (prev == -2) return;
-    enum cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-    const int relaxed = cudaThreadExchangeStreamCaptureMode(&mode) == cudaSuccess;
-    cudaFree(table);   /* waits for the device's work first */
-    if (relaxed) cudaThreadExchangeStreamCaptureMode(&mode);
-    leave(prev, device);
+static void release(op_plan *plan) {
+    const int prev = enter(plan->device);
+    if (prev != -2) {
+        enum cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        const int relaxed = cudaThreadExchangeStreamCaptureMode(&mode) == cudaSuccess;
+        cudaFree(plan->table);   /* waits for the device's work first */
+        if (relaxed) cudaThreadExchangeStreamCaptureMode(&mode);
+        leave(prev, plan->device);
+    }
+    free(plan);
+}
+
+/* A captured call's graph reads the plan's table whenever it runs, so a plan
+ * is freed after the graphs that captured it.  The graph (and whatever is
+ * instantiated or cloned from it) holds an object whose end drops the count;
+ * that happens on a thread of the driver's, where nothing can be freed. */
+static int graphs_of(const op_plan *plan) { return __atomic_load_n(&plan->graphs, __ATOMIC_ACQUIRE); }
+
+static void graph_gone(void *plan) { __atomic_fetch_sub(&((op_plan *)plan)->graphs, 1, __ATOMIC_RELEASE); }
+
+static int hold_for_graph(op_plan *plan, cudaStream_t stream) {
+    enum cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    cudaGraph_t graph = NULL;
+    cudaError_t e = cudaStreamGetCaptureInfo(stream, &status, NULL, &graph, NULL, NULL);
+    if (e == cudaSuccess && status != cudaStreamCaptureStatusActive) return cudaSuccess;
+    cudaUserObject_t object = NULL;
+    __atomic_fetch_add(&plan->graphs, 1, __ATOMIC_RELAXED);
+    if (e == cudaSuccess) e = cudaUserObjectCreate(&object, plan, graph_gone, 1, cudaUserObjectNoDestructorSync);
+    if (e != cudaSuccess) graph_gone(plan);
+    else if ((e = cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove)) != cudaSuccess)
+        cudaUserObjectRelease(object, 1);   /* and so graph_gone */
+    if (e != cudaSuccess) (void)cudaGetLastError();
+    return e;
+}
+
+static op_plan *g_left;   /* destroyed, used by graphs */
+static pthread_mutex_t g_left_mu = PTHREAD_MUTEX_INITIALIZER;
+
+/* Frees the destroyed plans that no graph uses any longer, and `plan` when
+ * none does (NULL: nothing new). */
+static void retire(op_plan *plan) {
+    op_plan *free_now = NULL;
+    pthread_mutex_lock(&g_left_mu);
+    if (plan) {
+        plan->next = g_left;
+        g_left = plan;
+    }
+    for (op_plan **at = &g_left; *at;) {
+        op_plan *p = *at;
+        if (graphs_of(p) > 0) {
+            at = &p->next;
+            continue;
+        }
+        *at = p->next;
+        p->next = free_now;
+        free_now = p;
+    }
+    pthread_mutex_unlock(&g_left_mu);
+    while (free_now) {
+        op_plan *p = free_now;
+        free_now = p->next;
+        release(p);
+    }
 }
 
 static int current_device(const char *who) {
@@ -168,6 +230,7 @@ MC_EXPORT falcom_norm *falcom_norm_create(const void *const *tensors, const size
         fprintf(stderr, "[ERROR] %s: invalid arguments\n", who);
         return NULL;
     }
+    retire(NULL);
     int device = -1;
     int64_t n_units = 0;
     mc_ptrcache pc;
@@ -215,12 +278,12 @@ MC_EXPORT falcom_norm *falcom_norm_create(const void *const *tensors, const size
         }
     }
     int sms = 0;
-    plan->device = device;
+    plan->base.device = device;
     plan->n_units = n_units;
     plan->units_at = units_at;
-    plan->table = upload(who, device, host, bytes, &sms);
+    plan->base.table = upload(who, device, host, bytes, &sms);
     free(host);
-    if (!plan->table) {
+    if (!plan->base.table) {
         free(plan);
         return NULL;
     }
@@ -239,31 +302,32 @@ MC_EXPORT int falcom_norm_run(falcom_norm *plan, double scale, double max_norm, 
         fprintf(stderr, "[ERROR] %s: invalid arguments\n", who);
         return ERROR_INVALID_PARAM;
     }
-    if (!check_scalar(who, "out", out, 4, plan->device) ||
-        !check_scalar(who, "work", work, 8, plan->device))
+    if (!check_scalar(who, "out", out, 4, plan->base.device) ||
+        !check_scalar(who, "work", work, 8, plan->base.device))
         return ERROR_INVALID_PARAM;
     if (error_pending(who)) return ERROR_COMPRESSION;
-    const int prev = enter(plan->device);
+    const int prev = enter(plan->base.device);
     if (prev == -2) return ERROR_COMPRESSION;
+    int e = hold_for_graph(&plan->base, (cudaStream_t)stream);
     op_norm_launch L;
     memset(&L, 0, sizeof(L));
-    L.tensors = (const op_norm_tensor *)plan->table;
-    L.units = (const op_unit *)(plan->table + plan->units_at);
+    L.tensors = (const op_norm_tensor *)plan->base.table;
+    L.units = (const op_unit *)(plan->base.table + plan->units_at);
     L.n_units = plan->n_units;
     L.scale = scale;
     L.max_norm = max_norm;
     L.out = out;
     L.ticket = (uint32_t *)work;
     L.partial = (double *)((uint8_t *)work + 16);
-    const int e = mc_launch_norm(&L, plan->grid, stream);
-    leave(prev, plan->device);
+    if (e == 0) e = mc_launch_norm(&L, plan->grid, stream);
+    leave(prev, plan->base.device);
     return e == 0 ? ERROR_NONE : launch_failed(who, e);
 }
 
+MC_EXPORT int falcom_norm_graphs(const falcom_norm *plan) { return plan ? graphs_of(&plan->base) : 0; }
+
 MC_EXPORT void falcom_norm_destroy(falcom_norm *plan) {
-    if (!plan) return;
-    release(plan->table, plan->device);
-    free(plan);
+    if (plan) retire(&plan->base);
 }
 
 /* ------------------------------------------------------------------ AdamW */
@@ -353,6 +417,7 @@ MC_EXPORT falcom_adamw *falcom_adamw_create(const falcom_adamw_tensor *tensors, 
         fprintf(stderr, "[ERROR] %s: invalid arguments (state_bits must be 32 or 8)\n", who);
         return NULL;
     }
+    retire(NULL);
     int device = -1;
     span *spans = (span *)malloc((6 * n + 1) * sizeof(*spans));
     if (!spans) {
@@ -415,14 +480,14 @@ MC_EXPORT falcom_adamw *falcom_adamw_create(const falcom_adamw_tensor *tensors, 
         }
     }
     int sms = 0;
-    plan->device = device;
+    plan->base.device = device;
     plan->bits = state_bits;
     plan->step = step;
     plan->tensors_at = tensors_at;
     plan->units_at = units_at;
-    plan->table = upload(who, device, host, bytes, &sms);
+    plan->base.table = upload(who, device, host, bytes, &sms);
     free(host);
-    if (!plan->table) {
+    if (!plan->base.table) {
         free(plan);
         return NULL;
     }
@@ -442,20 +507,21 @@ MC_EXPORT int falcom_adamw_step(falcom_adamw *plan, const falcom_adamw_args *a, 
         fprintf(stderr, "[ERROR] %s: invalid arguments\n", who);
         return ERROR_INVALID_PARAM;
     }
-    if ((a->clip && !check_scalar(who, "clip", a->clip, 4, plan->device)) ||
-        (a->lr_device && !check_scalar(who, "lr_device", a->lr_device, 4, plan->device)))
+    if ((a->clip && !check_scalar(who, "clip", a->clip, 4, plan->base.device)) ||
+        (a->lr_device && !check_scalar(who, "lr_device", a->lr_device, 4, plan->base.device)))
         return ERROR_INVALID_PARAM;
     if (error_pending(who)) return ERROR_COMPRESSION;
-    const int prev = enter(plan->device);
+    const int prev = enter(plan->base.device);
     if (prev == -2) return ERROR_COMPRESSION;
+    int e = hold_for_graph(&plan->base, (cudaStream_t)stream);
     op_adamw_launch L;
     memset(&L, 0, sizeof(L));
-    L.tensors = (const op_adamw_tensor *)(plan->table + plan->tensors_at);
-    L.units = (const op_unit *)(plan->table + plan->units_at);
+    L.tensors = (const op_adamw_tensor *)(plan->base.table + plan->tensors_at);
+    L.units = (const op_unit *)(plan->base.table + plan->units_at);
     L.step = plan->step;
     L.clip = a->clip;
     L.lr_dev = a->lr_device;
-    L.ticket = (uint32_t *)plan->table;
+    L.ticket = (uint32_t *)plan->base.table;
     L.lr = a->lr;
     L.beta1 = a->beta1;
     L.beta2 = a->beta2;
@@ -468,7 +534,6 @@ MC_EXPORT int falcom_adamw_step(falcom_adamw *plan, const falcom_adamw_args *a, 
     L.eps.x = L.eps.y = (float)a->eps;
     L.scale = (float)a->grad_scale;
     L.seed_key = mc_op_hash(mc_op_hash((uint32_t)a->seed ^ 0x9E3779B9u) ^ (uint32_t)(a->seed >> 32));
-    int e = 0;
     for (int c = 0; c < OP_NTYPES * OP_NTYPES && e == 0; c++) {
         /* a plan without elements still counts its steps */
         if (plan->n_units[c] > 0 || c == plan->last) {
@@ -478,25 +543,25 @@ MC_EXPORT int falcom_adamw_step(falcom_adamw *plan, const falcom_adamw_args *a, 
         }
         L.units += plan->n_units[c];
     }
-    leave(prev, plan->device);
+    leave(prev, plan->base.device);
     return e == 0 ? ERROR_NONE : launch_failed(who, e);
 }
 
 MC_EXPORT int falcom_adamw_errors(falcom_adamw *plan) {
     if (!plan) return ERROR_INVALID_PARAM;
-    const int prev = enter(plan->device);
+    const int prev = enter(plan->base.device);
     if (prev == -2) return ERROR_COMPRESSION;
     uint32_t word = 0;
     /* steps may be in flight on streams that the copy does not wait for */
     cudaError_t e = cudaDeviceSynchronize();
-    if (e == cudaSuccess) e = cudaMemcpy(&word, plan->table + 4, 4, cudaMemcpyDeviceToHost);
-    leave(prev, plan->device);
+    if (e == cudaSuccess) e = cudaMemcpy(&word, plan->base.table + 4, 4, cudaMemcpyDeviceToHost);
+    leave(prev, plan->base.device);
     if (e != cudaSuccess) return ERROR_COMPRESSION;
     return word != 0;
 }
 
+MC_EXPORT int falcom_adamw_graphs(const falcom_adamw *plan) { return plan ? graphs_of(&plan->base) : 0; }
+
 MC_EXPORT void falcom_adamw_destroy(falcom_adamw *plan) {
-    if (!plan) return;
-    release(plan->table, plan->device);
-    free(plan);
+    if (plan) retire(&plan->base);
 }

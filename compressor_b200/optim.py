@@ -18,12 +18,14 @@ once, so gradients are written in place from then on (zero_grad with
 set_to_none=False).  Calls queue work on the device's current stream and may
 be captured in a CUDA graph; the hyperparameters are captured by value, the
 step number, a clip coefficient and a learning rate given as a device tensor
-are read when the graph runs.
+are read when the graph runs.  Closing or dropping an object leaves what
+graphs captured of it in place until they are gone.
 """
 from __future__ import annotations
 
 import ctypes
 import math
+import threading
 from typing import Dict, List, Optional, Sequence, Union
 
 import torch
@@ -99,6 +101,25 @@ def _scalar_input(t: torch.Tensor, numel: int, device: torch.device, what: str) 
     return t.data_ptr()
 
 
+# (graphs, destroy, handle, memory) of dropped objects whose captured calls'
+# graphs may still run
+_kept: List[tuple] = []
+_kept_lock = threading.RLock()   # a collector may come back here on the same thread
+
+
+def _retire(graphs, destroy, handle: int, memory: tuple) -> None:
+    """Destroys a plan, and lets go of the memory that its calls use, once no
+    graph that captured them is left; looks after earlier ones too."""
+    global _kept
+    with _kept_lock:
+        waiting, _kept = _kept + [(graphs, destroy, handle, memory)], []
+        for item in waiting:
+            if item[0](item[2]) > 0:
+                _kept.append(item)
+            else:
+                item[1](item[2])
+
+
 class GradNorm:
     """L2 norm over a list of tensors, and the coefficient that clips it.
 
@@ -153,9 +174,10 @@ class GradNorm:
         return out
 
     def close(self) -> None:
-        if self._h:
-            self.lib.falcom_norm_destroy(self._h)
-            self._h = None
+        h, self._h = self._h, None
+        if h:
+            _retire(self.lib.falcom_norm_graphs, self.lib.falcom_norm_destroy, h,
+                    (self.tensors, self._work, self._captured))
 
     def __del__(self):
         try:
@@ -314,9 +336,10 @@ class AdamW:
         return self.lib.falcom_adamw_errors(self._h) if self._h else 0
 
     def close(self) -> None:
-        if self._h:
-            self.lib.falcom_adamw_destroy(self._h)
-            self._h = None
+        h, self._h = self._h, None
+        if h:
+            _retire(self.lib.falcom_adamw_graphs, self.lib.falcom_adamw_destroy, h,
+                    (self.params, self.grads, self.state))
 
     def __del__(self):
         try:

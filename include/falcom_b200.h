@@ -324,7 +324,10 @@ int falcom_state_load(MomentumCompressor *mc, const char *path);
  * allocate and synchronise, so they do not belong inside a stream capture;
  * run and step only queue kernels on `stream` (cudaStream_t of the plan's
  * device, NULL = its legacy default stream), whatever device is current, and
- * may be captured.  Element types: */
+ * may be captured.  A graph that captured calls of a plan uses its tables:
+ * destroy then only ends the plan, and a later create or destroy frees the
+ * tables once no such graph exists.  falcom_*_graphs counts the captured
+ * calls whose graphs exist.  Element types: */
 enum { FALCOM_TYPE_F32 = 0, FALCOM_TYPE_BF16 = 1, FALCOM_TYPE_F16 = 2 };
 
 /* Gradient norm with clipping coefficient.
@@ -351,6 +354,7 @@ typedef struct falcom_norm falcom_norm;
 falcom_norm *falcom_norm_create(const void *const *tensors, const size_t *numels, const int *dtypes, size_t n);
 size_t falcom_norm_work_bytes(const falcom_norm *plan);
 int falcom_norm_run(falcom_norm *plan, double scale, double max_norm, float *out, void *work, void *stream);
+int falcom_norm_graphs(const falcom_norm *plan);
 void falcom_norm_destroy(falcom_norm *plan);
 
 /* AdamW (decoupled weight decay).  With t the number of the step taken, lr
@@ -434,6 +438,7 @@ int falcom_adamw_step(falcom_adamw *plan, const falcom_adamw_args *args, void *s
  * the device cannot be asked.  Waits for all work queued on the plan's
  * device, so it does not belong inside a stream capture. */
 int falcom_adamw_errors(falcom_adamw *plan);
+int falcom_adamw_graphs(const falcom_adamw *plan);
 void falcom_adamw_destroy(falcom_adamw *plan);
 
 #ifdef __cplusplus

@@ -10,6 +10,39 @@ extern "C" inline __attribute__((used)) cudaError_t cudaDeviceGetAttribute(int *
 extern "C" inline __attribute__((used)) cudaError_t cudaThreadExchangeStreamCaptureMode(cudaStreamCaptureMode *) {
     return cudaSuccess;
 }
+
+// Stream capture: between the two calls of emu_optim_capture every stream is
+// being captured into one graph (kernels run all the same), which lives until
+// emu_optim_graph_gone.
+#include <utility>
+#include <vector>
+inline bool emu_capturing = false;
+inline std::vector<std::pair<cudaHostFn_t, void *>> emu_objects;
+extern "C" __attribute__((used, visibility("default"))) inline void emu_optim_capture(int on) { emu_capturing = on != 0; }
+extern "C" __attribute__((used, visibility("default"))) inline void emu_optim_graph_gone() {
+    for (auto &o : emu_objects) o.first(o.second);
+    emu_objects.clear();
+}
+extern "C" inline __attribute__((used)) cudaError_t cudaStreamGetCaptureInfo(cudaStream_t, cudaStreamCaptureStatus *st,
+                                                                             unsigned long long *, cudaGraph_t *g,
+                                                                             const cudaGraphNode_t **, size_t *) {
+    *st = emu_capturing ? cudaStreamCaptureStatusActive : cudaStreamCaptureStatusNone;
+    if (g) *g = (cudaGraph_t)&emu_capturing;
+    return cudaSuccess;
+}
+extern "C" inline __attribute__((used)) cudaError_t cudaUserObjectCreate(cudaUserObject_t *o, void *p, cudaHostFn_t f,
+                                                                         unsigned, unsigned) {
+    emu_objects.emplace_back(f, p);
+    *o = (cudaUserObject_t)&emu_objects;
+    return cudaSuccess;
+}
+extern "C" inline __attribute__((used)) cudaError_t cudaGraphRetainUserObject(cudaGraph_t, cudaUserObject_t, unsigned,
+                                                                              unsigned) {
+    return cudaSuccess;
+}
+extern "C" inline __attribute__((used)) cudaError_t cudaUserObjectRelease(cudaUserObject_t, unsigned) {
+    return cudaSuccess;
+}
 inline float emu_e4m3(unsigned code) {
     const int e = code >> 3 & 15, f = code & 7;
     float v = e ? ldexpf(1.0f + f / 8.0f, e - 7) : ldexpf(f / 8.0f, -6);

@@ -235,6 +235,10 @@ extern "C" __attribute__((visibility("default"))) void *emu_device_alloc(size_t 
     return cudaMalloc(&p, n) == cudaSuccess ? p : nullptr;
 }
 extern "C" __attribute__((visibility("default"))) void emu_device_free(void *p) { cudaFree(p); }
+extern "C" __attribute__((visibility("default"))) size_t emu_device_count(void) {
+    std::lock_guard<std::mutex> lk(g_mu);
+    return g_dev.size();
+}
 extern "C" __attribute__((visibility("default"))) void *emu_host_alloc(size_t n) {
     void *p = nullptr;
     return cudaHostAlloc(&p, n, 0) == cudaSuccess ? p : nullptr;

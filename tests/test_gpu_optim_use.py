@@ -1,5 +1,8 @@
 """GPU tests of what surrounds the optimiser operators' steps: error reports,
 plans and the graphs and tensors that they are used with."""
+import gc
+import time
+
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -25,3 +28,53 @@ def test_errors_waits_for_steps_on_other_streams(optim):
     assert not side.query()
     assert opt.errors() == 0
     assert side.query() and int(opt.state["step"]) == 2
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("how", ["drop", "close"])
+def test_graphs_outlive_their_objects(optim, bits, how):
+    """Captured calls replay as ever after the objects are gone and their
+    memory would have been used anew; with the last graph the rest goes."""
+    def make():
+        gen = torch.Generator("cuda").manual_seed(3)
+        p = [torch.randn(n, device="cuda", generator=gen) for n in (70_001, 300)]
+        g = [torch.randn(n, device="cuda", generator=gen) for n in (70_001, 300)]
+        return p, optim.AdamW(p, g, state_bits=bits), optim.GradNorm(g)
+
+    p, opt, norm = make()
+    q, ref, rnorm = make()
+    for o, n in ((opt, norm), (ref, rnorm)):
+        o.step(clip=n(max_norm=0.5))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        opt.step(clip=norm(max_norm=0.5))          # a stream that has seen eager steps is captured too
+    ref.step(clip=rnorm(max_norm=0.5))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        opt.step(clip=norm(max_norm=0.5))
+    lib, handles = opt.lib, (norm._h, opt._h)
+    assert lib.falcom_norm_graphs(handles[0]) == 1 and lib.falcom_adamw_graphs(handles[1]) == 1
+    if how == "close":
+        opt.close()
+        norm.close()
+    del opt, norm
+    gc.collect()
+    torch.cuda.empty_cache()
+    junk = [torch.full((k,), 7, dtype=torch.uint8, device="cuda") for k in (512, 3000, 70_144, 300_000, 1 << 20) for _ in range(8)]
+    for _ in range(3):
+        graph.replay()
+        ref.step(clip=rnorm(max_norm=0.5))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(p, q)) and all(bool((j == 7).all()) for j in junk)
+    assert len(optim._kept) == 2
+    del graph
+    gc.collect()
+    torch.cuda.synchronize()
+    for _ in range(100):                           # a graph's end reaches the count on a thread of the driver's
+        if lib.falcom_norm_graphs(handles[0]) + lib.falcom_adamw_graphs(handles[1]) == 0:
+            break
+        time.sleep(0.05)
+    rnorm.close()
+    assert not optim._kept

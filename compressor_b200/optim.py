@@ -15,7 +15,8 @@ them (federated.ServerAdamW), a client on its local gradients:
 
 Parameters and gradients are fixed lists of tensors: the addresses are read
 once, so gradients are written in place from then on (zero_grad with
-set_to_none=False).  Calls queue work on the device's current stream and may
+set_to_none=False; a step refuses parameters whose .grad was one of its
+gradients and is so no longer).  Calls queue work on the device's current stream and may
 be captured in a CUDA graph; the hyperparameters are captured by value, the
 step number, a clip coefficient and a learning rate given as a device tensor
 are read when the graph runs.  Closing or dropping an object leaves what
@@ -101,6 +102,23 @@ def _scalar_input(t: torch.Tensor, numel: int, device: torch.device, what: str) 
     return t.data_ptr()
 
 
+def _ties(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor]) -> List[tuple]:
+    """(index, parameter, its address, its gradient's) of the parameters that
+    autograd writes the given gradients of."""
+    return [(i, p, p.data_ptr(), g.data_ptr()) for i, (p, g) in enumerate(zip(params, grads))
+            if p.requires_grad and p.numel() and p.grad is not None and p.grad.data_ptr() == g.data_ptr()]
+
+
+def _check_ties(ties: List[tuple]) -> None:
+    for i, p, p_at, g_at in ties:
+        g = p.grad
+        if g is None or g.data_ptr() != g_at:
+            raise RuntimeError(f"the gradient of parameter {i} is no longer the tensor that this plan reads: keep it "
+                               "with zero_grad(set_to_none=False), or make a new plan")
+        if p.data_ptr() != p_at:
+            raise RuntimeError(f"parameter {i} has moved since this plan was made: make a new one")
+
+
 # (graphs, destroy, handle, memory) of dropped objects whose captured calls'
 # graphs may still run
 _kept: List[tuple] = []
@@ -131,6 +149,7 @@ class GradNorm:
     def __init__(self, tensors: Sequence[torch.Tensor], lib_path: Optional[str] = None):
         self._h = None
         self.tensors = _check_list(tensors, "tensor")
+        self._held = [t.detach() for t in self.tensors]   # the memory stays, whatever becomes of a tensor's data
         self.device = _device_of(self.tensors)
         self.lib = _library(lib_path)
         n = len(self.tensors)
@@ -177,7 +196,7 @@ class GradNorm:
         h, self._h = self._h, None
         if h:
             _retire(self.lib.falcom_norm_graphs, self.lib.falcom_norm_destroy, h,
-                    (self.tensors, self._work, self._captured))
+                    (self._held, self._work, self._captured))
 
     def __del__(self):
         try:
@@ -230,6 +249,8 @@ class AdamW:
         self.state_bits = state_bits
         self.lib = _library(lib_path)
         self._autograd = [p for p in self.params if p.requires_grad]
+        self._tied = _ties(self.params, self.grads)
+        self._held = [t.detach() for t in self.params + self.grads]   # the memory stays, whatever becomes of a tensor's data
 
         self.offsets, total = [], 0
         for p in self.params:
@@ -282,6 +303,8 @@ class AdamW:
         self.lr, a number or a float32 tensor of one element on the device."""
         if not self._h:
             raise RuntimeError("AdamW is closed")
+        if self._tied:
+            _check_ties(self._tied)
         a = self._args
         on_device = isinstance(lr, torch.Tensor)
         rate = self.lr if lr is None or on_device else float(lr)
@@ -339,7 +362,7 @@ class AdamW:
         h, self._h = self._h, None
         if h:
             _retire(self.lib.falcom_adamw_graphs, self.lib.falcom_adamw_destroy, h,
-                    (self.params, self.grads, self.state))
+                    (self._held, self.state))
 
     def __del__(self):
         try:

@@ -78,3 +78,34 @@ def test_graphs_outlive_their_objects(optim, bits, how):
         time.sleep(0.05)
     rnorm.close()
     assert not optim._kept
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_replaced_gradients_stop_the_step(optim, bits):
+    """A training loop that drops its gradients fails loudly and changes nothing."""
+    net = torch.nn.Linear(33, 65).cuda()
+    for p in net.parameters():
+        p.grad = torch.zeros_like(p)
+    opt = optim.AdamW(list(net.parameters()), [p.grad for p in net.parameters()], state_bits=bits)
+    x = torch.randn(16, 33, device="cuda")
+    net.zero_grad(set_to_none=False)
+    net(x).square().sum().backward()
+    opt.step()
+    before = [p.detach().clone() for p in net.parameters()]
+    net.zero_grad()
+    net(x).square().sum().backward()
+    with pytest.raises(RuntimeError, match="set_to_none=False"):
+        opt.step()
+    assert all(torch.equal(a, b) for a, b in zip(before, net.parameters())) and int(opt.state["step"]) == 1
+
+
+def test_replaced_memory_is_held(optim):
+    """What a plan's addresses lead to is not given to others while it exists."""
+    p, g = torch.zeros(100_000, device="cuda"), torch.ones(100_000, device="cuda")
+    opt, norm = optim.AdamW([p], [g], weight_decay=0.0), optim.GradNorm([g])
+    places = {p.data_ptr(), g.data_ptr()}
+    p.data, g.data = torch.zeros(7, device="cuda"), torch.zeros(7, device="cuda")
+    others = [torch.empty(100_000, device="cuda") for _ in range(16)]
+    assert not places & {t.data_ptr() for t in others}
+    norm()
+    opt.step()

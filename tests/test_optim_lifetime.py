@@ -99,9 +99,9 @@ def test_classes_leave_graphs_their_memory(kind, how):
     def make(h):
         o = object.__new__(getattr(optim, kind))
         o._h, o.lib = h, lib
-        o.tensors = o.params = o.grads = [torch.zeros(1)]
+        o._held = [torch.zeros(1)]
         o._work, o._captured, o.state = {}, [torch.zeros(1)], {"m": torch.zeros(1)}
-        return o, [weakref.ref(t) for t in (o.tensors[0], o._captured[0] if kind == "GradNorm" else o.state["m"])]
+        return o, [weakref.ref(t) for t in (o._held[0], o._captured[0] if kind == "GradNorm" else o.state["m"])]
 
     def drop(o):
         if how == "close":

@@ -67,19 +67,25 @@ static int check_range(mc_ptrcache *pc, const char *who, const char *what, size_
     return 1;
 }
 
-/* An argument of a run or step: a few values in device memory of `device`,
- * by its first byte (the driver's allocations are larger). */
-static int check_scalar(const char *who, const char *what, const void *p, size_t align, int device) {
+static int device_byte(const void *p, int device) {
     struct cudaPointerAttributes at;
-    if (p && ((uintptr_t)p & (align - 1)) == 0) {
-        if (cudaPointerGetAttributes(&at, p) == cudaSuccess) {
-            if ((at.type == cudaMemoryTypeDevice || at.type == cudaMemoryTypeManaged) && at.device == device) return 1;
-        } else {
-            (void)cudaGetLastError();
-        }
+    if (cudaPointerGetAttributes(&at, p) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return 0;
     }
-    fprintf(stderr, "[ERROR] %s: %s is NULL, not %zu-byte aligned or not device memory of device %d\n", who, what,
-            align, device);
+    return (at.type == cudaMemoryTypeDevice || at.type == cudaMemoryTypeManaged) && at.device == device;
+}
+
+/* An argument of a run or step: `bytes` of device memory of `device`.  Its
+ * last byte is asked about where another allocation could start before it:
+ * they start at multiples of 256 bytes. */
+static int check_argument(const char *who, const char *what, const void *p, size_t bytes, size_t align, int device) {
+    const uintptr_t first = (uintptr_t)p, last = first + bytes - 1;
+    if (p && (first & (align - 1)) == 0 && device_byte(p, device) &&
+        (first / 256 == last / 256 || device_byte((const void *)last, device)))
+        return 1;
+    fprintf(stderr, "[ERROR] %s: %s is NULL, not %zu-byte aligned or not %zu bytes of device memory of device %d\n",
+            who, what, align, bytes, device);
     return 0;
 }
 
@@ -302,8 +308,8 @@ MC_EXPORT int falcom_norm_run(falcom_norm *plan, double scale, double max_norm, 
         fprintf(stderr, "[ERROR] %s: invalid arguments\n", who);
         return ERROR_INVALID_PARAM;
     }
-    if (!check_scalar(who, "out", out, 4, plan->base.device) ||
-        !check_scalar(who, "work", work, 8, plan->base.device))
+    if (!check_argument(who, "out", out, 2 * sizeof(float), 4, plan->base.device) ||
+        !check_argument(who, "work", work, falcom_norm_work_bytes(plan), 8, plan->base.device))
         return ERROR_INVALID_PARAM;
     if (error_pending(who)) return ERROR_COMPRESSION;
     const int prev = enter(plan->base.device);
@@ -507,8 +513,8 @@ MC_EXPORT int falcom_adamw_step(falcom_adamw *plan, const falcom_adamw_args *a, 
         fprintf(stderr, "[ERROR] %s: invalid arguments\n", who);
         return ERROR_INVALID_PARAM;
     }
-    if ((a->clip && !check_scalar(who, "clip", a->clip, 4, plan->base.device)) ||
-        (a->lr_device && !check_scalar(who, "lr_device", a->lr_device, 4, plan->base.device)))
+    if ((a->clip && !check_argument(who, "clip", a->clip, 2 * sizeof(float), 4, plan->base.device)) ||
+        (a->lr_device && !check_argument(who, "lr_device", a->lr_device, sizeof(float), 4, plan->base.device)))
         return ERROR_INVALID_PARAM;
     if (error_pending(who)) return ERROR_COMPRESSION;
     const int prev = enter(plan->base.device);

@@ -36,8 +36,9 @@ from . import build as _build
 
 _TYPES = {torch.float32: abi.TYPE_F32, torch.bfloat16: abi.TYPE_BF16, torch.float16: abi.TYPE_F16}
 _libs: Dict[str, ctypes.CDLL] = {}
-# (device index) -> cudaStream_t; the public route through a Stream object takes 2 us
-_current_stream = torch._C._cuda_getCurrentRawStream
+# (device index) -> cudaStream_t; the public route through a Stream object takes 2 us.  A torch without CUDA has none
+# and no tensor that would get as far.
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _capturing(index: int) -> bool:

@@ -359,12 +359,11 @@ static int spans_disjoint(span *s, size_t n) {
     return 1;
 }
 
-static int add_span(span *s, size_t *k, const void *p, size_t bytes, int written) {
+static void add_span(span *s, size_t *k, const void *p, size_t bytes, int written) {
     s[*k].lo = (uintptr_t)p;
     s[*k].hi = (uintptr_t)p + bytes;
     s[*k].written = written;
     (*k)++;
-    return 1;
 }
 
 static int check_tensors(const char *who, const falcom_adamw_tensor *t, size_t n, int bits, int64_t *step,

@@ -49,22 +49,12 @@ inline float emu_e4m3(unsigned code) {
     if ((code & 0x7F) == 0x7F) v = NAN;
     return code & 0x80 ? -v : v;
 }
-// towards zero, by way of a 64-bit value (products and sums of the scale's
-// computation fit it)
-inline float __fmaf_rz(float a, float b, float c) {
-    const double x = fma((double)a, (double)b, (double)c);
-    float r = (float)x;
-    if (fabs((double)r) > fabs(x)) r = nextafterf(r, 0.0f);
-    return r;
-}
-
 inline unsigned __byte_perm(unsigned a, unsigned b, unsigned sel) {
     const unsigned long long ab = (unsigned long long)b << 32 | a;
     unsigned r = 0;
     for (int i = 0; i < 4; i++) r |= (unsigned)(ab >> 8 * (sel >> 4 * i & 7) & 0xFF) << 8 * i;
     return r;
 }
-inline float __saturatef(float x) { return x > 0.0f ? (x < 1.0f ? x : 1.0f) : 0.0f; }
 
 template <class T>
 inline T __shfl_sync(unsigned, T v, int src) {   // emu_shfl knows lane ^ arg: from src's own side

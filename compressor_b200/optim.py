@@ -107,7 +107,8 @@ def _ties(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor]) -> List
     """(index, parameter, its address, its gradient's) of the parameters that
     autograd writes the given gradients of."""
     return [(i, p, p.data_ptr(), g.data_ptr()) for i, (p, g) in enumerate(zip(params, grads))
-            if p.requires_grad and p.numel() and p.grad is not None and p.grad.data_ptr() == g.data_ptr()]
+            if p.requires_grad and (p.is_leaf or p.retains_grad) and p.numel() and p.grad is not None
+            and p.grad.data_ptr() == g.data_ptr()]
 
 
 def _check_ties(ties: List[tuple]) -> None:

@@ -58,3 +58,16 @@ def test_gradients_of_ones_own_are_not_tied():
     empty = torch.zeros(0, requires_grad=True)
     empty.grad = torch.zeros(0)
     assert optim._ties([empty], [empty.grad]) == []
+
+
+def test_slices_of_a_leaf_are_not_asked_for_gradients(recwarn):
+    """torch warns where .grad of a tensor is read that autograd never fills."""
+    from compressor_b200 import optim
+    flat = torch.zeros(10, requires_grad=True)
+    flat.grad = torch.zeros(10)
+    assert optim._ties([flat[:4], flat[4:]], [flat.grad[:4], flat.grad[4:]]) == []
+    assert not recwarn.list
+    kept = flat * 2
+    kept.retain_grad()
+    kept.sum().backward()
+    assert len(optim._ties([kept], [kept.grad])) == 1 and not recwarn.list

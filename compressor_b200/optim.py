@@ -259,16 +259,17 @@ class AdamW:
             self.offsets.append(total)
             total += -(-p.numel() // abi.ADAMW_BLOCK) * abi.ADAMW_BLOCK
         kind = torch.float32 if state_bits == 32 else torch.uint8
-        self.state: Dict[str, torch.Tensor] = {k: torch.zeros(total, dtype=kind, device=self.device) for k in "mv"}
+        state: Dict[str, torch.Tensor] = {k: torch.zeros(total, dtype=kind, device=self.device) for k in "mv"}
         if state_bits == 8:
-            self.state = {k: t.view(torch.float8_e4m3fn) for k, t in self.state.items()}
+            state = {k: t.view(torch.float8_e4m3fn) for k, t in state.items()}
             for k in ("m_scale", "v_scale"):
-                self.state[k] = torch.zeros(total // abi.ADAMW_BLOCK, dtype=torch.float32, device=self.device)
-        self.state["step"] = torch.zeros(1, dtype=torch.int64, device=self.device)
+                state[k] = torch.zeros(total // abi.ADAMW_BLOCK, dtype=torch.float32, device=self.device)
+        state["step"] = torch.zeros(1, dtype=torch.int64, device=self.device)
+        self._state = state
 
         table = (abi.AdamWTensorC * n)()
         size = 4 if state_bits == 32 else 1
-        base = {k: t.data_ptr() for k, t in self.state.items()}
+        base = {k: t.data_ptr() for k, t in state.items()}
         for c, p, g, o, w in zip(table, self.params, self.grads, self.offsets, decay):
             c.param, c.grad, c.n = p.data_ptr(), g.data_ptr(), p.numel()
             c.m, c.v = base["m"] + size * o, base["v"] + size * o
@@ -286,6 +287,13 @@ class AdamW:
         self._args_ref = ctypes.byref(self._args)
         self._given = None
         self._streams = set()
+
+    @property
+    def state(self) -> Dict[str, torch.Tensor]:
+        """The states, to read, to save and to change in place; others' values
+        come in with load_state (the plan goes on with these tensors whatever
+        becomes of the dict)."""
+        return dict(self._state)
 
     def _check_hyper(self, lr: float, grad_scale: float) -> None:
         if not (math.isfinite(lr) and lr >= 0):
@@ -320,7 +328,7 @@ class AdamW:
         stream = _current_stream(self.device.index)
         if stream not in self._streams and not _capturing(self.device.index):
             # the allocator may not reuse the states' memory under this stream's work
-            for t in self.state.values():
+            for t in self._state.values():
                 t.record_stream(torch.cuda.current_stream(self.device))
             self._streams.add(stream)
         rc = self.lib.falcom_adamw_step(self._h, self._args_ref, stream)
@@ -332,21 +340,21 @@ class AdamW:
 
     def load_state(self, state: Dict[str, torch.Tensor]) -> None:
         """Copies a `state` of the same layout into this one's (in place)."""
-        if set(state) != set(self.state):
-            raise ValueError(f"state has {sorted(state)}, wanted {sorted(self.state)}")
-        for k, t in self.state.items():
+        if set(state) != set(self._state):
+            raise ValueError(f"state has {sorted(state)}, wanted {sorted(self._state)}")
+        for k, t in self._state.items():
             if state[k].shape != t.shape or state[k].dtype != t.dtype:
                 raise ValueError(f"state {k} is {state[k].dtype} {tuple(state[k].shape)}, wanted {t.dtype} "
                                  f"{tuple(t.shape)}")
-        for k, t in self.state.items():
+        for k, t in self._state.items():
             t.copy_(state[k])
 
     def moments(self) -> List[tuple]:
         """Both moments of every parameter, as new float32 tensors (m, v) in
         the parameter's shape and memory order."""
-        flat = {"m": self.state["m"], "v": self.state["v"]}
+        flat = {"m": self._state["m"], "v": self._state["v"]}
         if self.state_bits == 8:
-            flat = {k: (t.float().view(-1, abi.ADAMW_BLOCK) * self.state[k + "_scale"][:, None]).view(-1)
+            flat = {k: (t.float().view(-1, abi.ADAMW_BLOCK) * self._state[k + "_scale"][:, None]).view(-1)
                     for k, t in flat.items()}
             flat["v"] = flat["v"].square()
         out = []
@@ -364,7 +372,7 @@ class AdamW:
         h, self._h = self._h, None
         if h:
             _retire(self.lib.falcom_adamw_graphs, self.lib.falcom_adamw_destroy, h,
-                    (self._held, self.state))
+                    (self._held, self._state))
 
     def __del__(self):
         try:

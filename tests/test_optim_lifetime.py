@@ -100,8 +100,8 @@ def test_classes_leave_graphs_their_memory(kind, how):
         o = object.__new__(getattr(optim, kind))
         o._h, o.lib = h, lib
         o._held = [torch.zeros(1)]
-        o._work, o._captured, o.state = {}, [torch.zeros(1)], {"m": torch.zeros(1)}
-        return o, [weakref.ref(t) for t in (o._held[0], o._captured[0] if kind == "GradNorm" else o.state["m"])]
+        o._work, o._captured, o._state = {}, [torch.zeros(1)], {"m": torch.zeros(1)}
+        return o, [weakref.ref(t) for t in (o._held[0], o._captured[0] if kind == "GradNorm" else o._state["m"])]
 
     def drop(o):
         if how == "close":

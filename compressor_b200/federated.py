@@ -342,8 +342,8 @@ class ServerAdamW:
     send gradients.  Tensors with more than one dimension decay
     (`decays(name, shape)` says otherwise), `names` restricts the step to
     some of the tensors, state_bits = 8 holds the moments in a byte each, and
-    max_norm clips the whole aggregate's norm first; an aggregate that is not
-    finite is then skipped.
+    max_norm first clips the norm over all tensors that are stepped; a round
+    whose norm is not finite is then skipped.
 
     Running statistics are no parameters: a step of about lr, whatever their
     size, would take a small variance below zero.  Tensors named
@@ -352,9 +352,14 @@ class ServerAdamW:
     average, and have no part in the norm; one that is not finite skips the
     step too, where max_norm is given.
 
-    Every rank steps its own copy of the weights: the step's bits depend on
-    the aggregate's alone, so copies that were equal stay equal.  Plans hold
-    addresses, so `weights` and `aggregate` must stay where they are."""
+    Every rank steps its own copy of the weights.  The step's bits depend on
+    the aggregate's, and with max_norm also on the order of the norm's sum:
+    copies that were equal stay equal where every rank's aggregate lies at
+    the same offset from a 16-byte boundary (a tensor of its own always does)
+    and the GPUs have the same number of SMs.  Elsewhere two coefficients may
+    be neighbouring float32 values, and one rank's weights have to be
+    broadcast after each step.  Plans hold addresses, so `weights` and
+    `aggregate` must stay where they are."""
 
     def __init__(self, layout: AggregateLayout, weights, aggregate, lr: float = 1e-3, betas=(0.9, 0.999),
                  eps: float = 1e-8, weight_decay: float = 0.0, state_bits: int = 32, max_norm: float = None,

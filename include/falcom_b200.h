@@ -334,8 +334,11 @@ enum { FALCOM_TYPE_F32 = 0, FALCOM_TYPE_BF16 = 1, FALCOM_TYPE_F16 = 2 };
  *   norm        = |scale| * sqrt(sum of squares over every tensor)
  *   coefficient = max_norm / norm when norm > max_norm, else 1;
  *                 NaN when the norm is infinite or NaN
- * Squares and sums are taken in 64 bits, in an order that depends only on
- * the list, so repeated runs give the same bits.
+ * (A finite norm above float32's range is written as infinity, and its
+ * coefficient stands.)  Squares and sums are taken in 64 bits, in an order
+ * that depends on the list's lengths and types, on the arrays' offsets from
+ * 16-byte boundaries and on the device's number of SMs: where these are
+ * equal the bits are, elsewhere results may be neighbouring float32 values.
  *
  * falcom_norm_create: tensors[i] has numels[i] elements of dtypes[i].
  * Returns NULL (message on stderr) for a NULL or misaligned address, memory

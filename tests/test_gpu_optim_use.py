@@ -109,3 +109,20 @@ def test_replaced_memory_is_held(optim):
     assert not places & {t.data_ptr() for t in others}
     norm()
     opt.step()
+
+
+def test_norms_at_other_offsets_differ_in_the_last_place(optim):
+    """The sum's order follows the arrays' offsets from 16 bytes: the same
+    offsets give the same bits wherever the arrays lie, others at most
+    neighbouring results."""
+    src = torch.randn(1_000_003, device="cuda", generator=torch.Generator("cuda").manual_seed(6))
+    first = None
+    for k in (0, 0, 1, 1, 2, 3, 3):
+        buf = torch.empty(src.numel() + 8, device="cuda")
+        g = buf[k:k + src.numel()].copy_(src)
+        got = optim.GradNorm([g])(max_norm=1.0)
+        again = optim.GradNorm([g.clone() if k == 0 else g])(max_norm=1.0)
+        assert torch.equal(got, again)
+        first = got if first is None else first
+        # 64-bit sums in another order, each result rounded to float32 once
+        assert bool(((got - first).abs() <= 2.0 ** -23 * first).all())

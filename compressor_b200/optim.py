@@ -4,8 +4,9 @@ coefficient (GradNorm) and AdamW with 32-bit or 8-bit states (AdamW).
 The reference has no optimiser of its own: its server averages the decoded
 updates and its clients train with their framework's.  These classes are the
 torch side of falcom_norm_* and falcom_adamw_* (include/falcom_b200.h, which
-defines every formula): one kernel launch for the whole list, results on the
-device, nothing read back.  A server steps on the round's aggregate with
+defines every formula): one kernel launch for the whole list (a step: for
+each pair of parameter and gradient type in it), results on the device,
+nothing read back.  A server steps on the round's aggregate with
 them (federated.ServerAdamW), a client on its local gradients:
 
     norm = GradNorm(grads)
@@ -16,8 +17,10 @@ them (federated.ServerAdamW), a client on its local gradients:
 Parameters and gradients are fixed lists of tensors: the addresses are read
 once, so gradients are written in place from then on (zero_grad with
 set_to_none=False; a step refuses parameters whose .grad was one of its
-gradients and is so no longer).  Calls queue work on the device's current stream and may
-be captured in a CUDA graph; the hyperparameters are captured by value, the
+gradients and is so no longer).  Making an object waits for the device; it is
+meant once per list.  Calls queue work on the device's current stream (the
+steps of one AdamW have to be ordered: one stream, or events) and may be
+captured in a CUDA graph; the hyperparameters are captured by value, the
 step number, a clip coefficient and a learning rate given as a device tensor
 are read when the graph runs.  Closing or dropping an object leaves what
 graphs captured of it in place until they are gone.
@@ -145,8 +148,10 @@ class GradNorm:
 
     norm(max_norm, grad_scale) returns a new float32 tensor [norm,
     coefficient]: norm = |grad_scale| * sqrt(sum of squares), coefficient =
-    min(1, max_norm / norm), NaN when the norm is not finite.  Calls on
-    different streams, and captured ones, do not share scratch memory."""
+    min(1, max_norm / norm), NaN when the norm is not finite (in 64 bits: a
+    norm above float32's range comes out as infinity beside its coefficient).
+    Calls on different streams, and captured ones, do not share scratch
+    memory."""
 
     def __init__(self, tensors: Sequence[torch.Tensor], lib_path: Optional[str] = None):
         self._h = None

@@ -318,16 +318,19 @@ int falcom_state_load(MomentumCompressor *mc, const char *path);
  *
  * Common rules.  Tensors are contiguous device memory of one device, each
  * aligned to its element size, of any length (0 too); 16-byte alignment of
- * a tensor's arrays, of its states above all, gives the fast loads.  A plan copies the lists
- * and keeps the addresses: the memory must stay allocated while the plan, or
- * a CUDA graph that captured its calls, is used.  create and destroy
- * allocate and synchronise, so they do not belong inside a stream capture;
- * run and step only queue kernels on `stream` (cudaStream_t of the plan's
- * device, NULL = its legacy default stream), whatever device is current, and
- * may be captured.  A graph that captured calls of a plan uses its tables:
- * destroy then only ends the plan, and a later create or destroy frees the
- * tables once no such graph exists.  falcom_*_graphs counts the captured
- * calls whose graphs exist.  Element types: */
+ * a tensor's arrays, of its states above all, gives the fast loads.  A plan
+ * copies the lists and keeps the addresses: the memory must stay allocated
+ * while the plan, or a CUDA graph that captured its calls, is used.  create
+ * copies tables of 8 bytes per 2048 to 16384 elements to the device and waits
+ * for all of the device's streams, destroy frees them and waits likewise:
+ * once per list of addresses, and neither belongs inside a stream capture
+ * (destroy does not end one).  run and step only queue kernels on `stream`
+ * (cudaStream_t of the plan's device, NULL = its legacy default stream),
+ * whatever device is current, and may be captured.  A graph that captured
+ * calls of a plan uses its tables: destroy then only ends the plan, and a
+ * later create or destroy frees the tables once no such graph exists.
+ * falcom_*_graphs counts the captured calls whose graphs exist.  Element
+ * types: */
 enum { FALCOM_TYPE_F32 = 0, FALCOM_TYPE_BF16 = 1, FALCOM_TYPE_F16 = 2 };
 
 /* Gradient norm with clipping coefficient.
@@ -386,9 +389,10 @@ void falcom_norm_destroy(falcom_norm *plan);
  * 0.999, the codes are 6 to 12 % apart).  The random bits are a hash of
  * (seed, t, position), the position being 256 * (blocks of the plan's
  * earlier tensors) + the element's index.  g', m', v', the root, scales and
- * codes are rounded operation by operation as written, nothing fused (the
- * code is that of |x| * (448 / max), exactly rounded quotient), so any
- * implementation of these formulas gets the same codes.  A v > 0 never gets
+ * codes are rounded operation by operation as written, nothing fused, so any
+ * implementation of these formulas gets the same codes: a code is that of
+ * |x| * (448 / max), the quotient rounded to float32, the product too and
+ * below 2^-6 to a multiple of 2^-29, once.  A v > 0 never gets
  * code 0, so no denominator vanishes under a first moment that did not.
  * All-zero state (codes and scales 0) is the start.  Of a block in which a
  * new value of m (of sqrt(v)) is infinite, NaN or 2^100 and more, m's (v's)
@@ -408,14 +412,15 @@ void falcom_norm_destroy(falcom_norm *plan);
  * addresses (param, grad: element size; m, v: 4 bytes with 32 bits; scales:
  * 4; step: 8), unknown types, a negative or non-finite weight decay, memory
  * that is not device memory of one device, arrays that are written and
- * overlap any other array, or when allocation fails.  The steps of one plan must be ordered (one stream, or events).
+ * overlap any other array, or when allocation fails.  The steps of one plan
+ * must be ordered (one stream, or events).
  * falcom_adamw_step returns 0; ERROR_INVALID_PARAM for lr < 0 or not finite,
- * betas outside [0, 1), eps not positive as a float32, a non-finite
- * grad_scale, or a clip or lr_device that is not device memory of the plan's
- * device; ERROR_COMPRESSION when a launch fails or an error is pending, as
- * above.  One launch per pair of parameter and gradient type in the list, in
- * a fixed order; should one fail, the pairs before it have been stepped and
- * the counter has not. */
+ * betas outside [0, 1), eps that is infinite or below the smallest normal
+ * number as a float32, a non-finite grad_scale, or a clip or lr_device that
+ * does not lie in device memory of the plan's device; ERROR_COMPRESSION when
+ * a launch fails or an error is pending, as above.  One launch per pair of
+ * parameter and gradient type in the list, in a fixed order; should one fail,
+ * the pairs before it have been stepped and the counter has not. */
 #define FALCOM_ADAMW_BLOCK 256
 typedef struct falcom_adamw_tensor {
     void *param;

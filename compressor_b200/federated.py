@@ -399,25 +399,28 @@ class ServerAdamW:
         clip = None
         if self.norm is not None:
             clip = self.norm(max_norm=self.max_norm, grad_scale=self.grad_scale)
-        if self._places is not None:
-            clip = self._average(clip)
-        self.opt.step(lr=lr, grad_scale=self.grad_scale, clip=clip)
-        return clip
-
-    def _average(self, clip):
-        """Adds the aggregate to the averaged tensors unless the step is to be
-        skipped; returns `clip`, its coefficient NaN if one of them is why."""
+        if self._places is None:
+            self.opt.step(lr=lr, grad_scale=self.grad_scale, clip=clip)
+            return clip
         import torch
         with torch.no_grad():
-            change = self.aggregate.index_select(0, self._places)
-            old = self.weights.index_select(0, self._places)
-            new = torch.add(old, change, alpha=-self.grad_scale)
-            if clip is not None:
-                skip = clip[1].isnan() | ~change.isfinite().all()
-                new = torch.where(skip, old, new)
-                clip = torch.stack([clip[0], torch.where(skip, math.nan, clip[1])])
-            self.weights.index_copy_(0, self._places, new)
+            statistics, clip = self._averages(clip)
+            self.opt.step(lr=lr, grad_scale=self.grad_scale, clip=clip)
+            self.weights.index_copy_(0, self._places, statistics)   # a step that is refused leaves them
         return clip
+
+    def _averages(self, clip):
+        """The averaged tensors' values after the step, the old ones if it is
+        skipped, and `clip`, its coefficient NaN if one of them is why."""
+        import torch
+        change = self.aggregate.index_select(0, self._places)
+        old = self.weights.index_select(0, self._places)
+        new = torch.add(old, change, alpha=-self.grad_scale)
+        if clip is not None:
+            skip = clip[1].isnan() | ~change.isfinite().all()
+            new = torch.where(skip, old, new)
+            clip = torch.stack([clip[0], torch.where(skip, math.nan, clip[1])])
+        return new, clip
 
     def errors(self) -> int:
         """Nonzero once a step went wrong on the device (optim.AdamW.errors):

@@ -109,3 +109,17 @@ def test_errors_of_the_step_are_reported(seen):
     s = fed.ServerAdamW(LAYOUT, w, a)
     s.opt.errors = lambda: 1
     assert s.errors() == 1
+
+
+def test_a_refused_step_leaves_the_statistics(seen):
+    w, a = _flat()
+    before = w.clone()
+    s = fed.ServerAdamW(LAYOUT, w, a, max_norm=1.0)
+
+    def refuse(**kw):
+        raise ValueError("lr")
+
+    s.opt.step = refuse
+    with pytest.raises(ValueError):
+        s.step(lr=-1.0)
+    assert torch.equal(w, before)

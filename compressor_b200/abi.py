@@ -528,6 +528,8 @@ def bind_extensions(lib: ctypes.CDLL) -> None:
     bind_replay(lib)
     if hasattr(lib, "falcom_adamw_create"):   # builds of the codec alone lack the optimiser entry points
         bind_optim(lib)
+    if hasattr(lib, "falcom_mx4_product"):
+        bind_mx4(lib)
 
 
 TYPE_F32, TYPE_BF16, TYPE_F16 = range(3)
@@ -586,6 +588,52 @@ def bind_optim(lib: ctypes.CDLL) -> None:
     lib.falcom_adamw_graphs.restype = ctypes.c_int
     lib.falcom_adamw_destroy.argtypes = [c_vp]
     lib.falcom_adamw_destroy.restype = None
+
+
+MX4_BLOCK = 32
+
+
+class RandomC(ctypes.Structure):
+    _fields_ = [
+        ("seed", ctypes.c_uint64),
+        ("counter", ctypes.c_void_p),
+    ]
+
+
+class DropoutArgsC(ctypes.Structure):
+    _fields_ = [
+        ("p", ctypes.c_double),
+        ("random", RandomC),
+    ]
+
+
+class Mx4MatrixC(ctypes.Structure):
+    _fields_ = [
+        ("codes", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+        ("rows", ctypes.c_size_t),
+        ("cols", ctypes.c_size_t),
+    ]
+
+
+def bind_mx4(lib: ctypes.CDLL) -> None:
+    """4-bit entry points (falcom_mx4_*) and falcom_dropout; no instance needed."""
+    P = ctypes.POINTER
+    c_vp, size, c_int = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int
+    lib.falcom_mx4_encode.argtypes = [c_vp, c_int, size, c_vp, P(RandomC), c_vp, c_vp, c_vp]
+    lib.falcom_mx4_decode.argtypes = [c_vp, c_vp, size, ctypes.c_float, c_int, c_vp, c_int, c_vp]
+    for fn in (lib.falcom_mx4_codes_bytes, lib.falcom_mx4_scales_bytes):
+        fn.argtypes = [size, size]
+        fn.restype = size
+    lib.falcom_mx4_quantize.argtypes = [c_vp, c_int, size, size, size, P(RandomC), P(DropoutArgsC), P(Mx4MatrixC),
+                                        P(Mx4MatrixC), c_vp]
+    lib.falcom_mx4_dequantize.argtypes = [P(Mx4MatrixC), c_vp, c_int, size, c_vp]
+    lib.falcom_mx4_product.argtypes = [P(Mx4MatrixC), P(Mx4MatrixC), c_vp, c_int, size, P(DropoutArgsC), c_vp]
+    lib.falcom_mx4_errors.argtypes = []
+    lib.falcom_dropout.argtypes = [c_vp, c_vp, c_vp, c_int, size, size, P(DropoutArgsC), c_vp]
+    for fn in (lib.falcom_mx4_encode, lib.falcom_mx4_decode, lib.falcom_mx4_quantize, lib.falcom_mx4_dequantize,
+               lib.falcom_mx4_product, lib.falcom_mx4_errors, lib.falcom_dropout):
+        fn.restype = c_int
 
 
 def bind_replay(lib: ctypes.CDLL) -> None:

@@ -1,0 +1,103 @@
+/*
+ * mc_mx4.h -- what the host side (mc_mx4.c) hands to the kernels of the 4-bit
+ * operators and of dropout (mc_mx4.cu, mc_mx4_product.cu).
+ */
+#ifndef MC_MX4_H
+#define MC_MX4_H
+
+#include <cuda_runtime_api.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "falcom_b200.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+#define MX_BLOCK FALCOM_MX4_BLOCK   /* elements of a scale */
+#define MX_PANEL 256                /* columns of a matrix whose codes lie together: 128 bytes a row */
+#define MX_GROUP 128                /* rows whose scales lie together */
+#define MX_TYPES 3
+
+/* Random bits of one purpose; counter NULL counts as 0. */
+typedef struct {
+    uint32_t key;              /* hash of purpose and seed */
+    int32_t on;
+    const int64_t *counter;    /* device memory */
+} mx_random;
+
+typedef struct {
+    mx_random random;
+    uint32_t threshold;        /* an element is dropped when its 16 bits are below */
+    float factor;              /* of the others */
+} mx_drop;
+
+typedef struct {
+    uint8_t *codes;            /* [panels][rows up to 8][128], 16-byte pieces exchanged within a row */
+    uint8_t *scales;           /* [panels][groups][2][32][4][4] */
+    int64_t rows, cols;
+} mx_matrix;
+
+typedef struct {
+    const void *x;
+    int64_t n;
+    float *base;               /* or NULL */
+    uint8_t *codes, *scales;
+    mx_random random;
+} mx_encode_launch;
+
+typedef struct {
+    const uint8_t *codes, *scales;
+    int64_t n;
+    void *out;
+    float weight;
+    int32_t accumulate;
+} mx_decode_launch;
+
+typedef struct {
+    const void *x;
+    int64_t rows, cols, ld;
+    mx_matrix along_rows, along_cols;   /* codes NULL: not wanted */
+    mx_random random;
+    mx_drop drop;
+    int32_t vectors;           /* every row starts on a 16-byte boundary */
+    uint32_t tiles;            /* of 128 columns */
+} mx_quantize_launch;
+
+typedef struct {
+    mx_matrix m;
+    void *out;
+    int64_t ld;
+} mx_dequantize_launch;
+
+typedef struct {
+    mx_matrix a, b;
+    void *out;                 /* [a.rows][ld] */
+    int64_t ld;
+    mx_drop drop;
+} mx_product_launch;
+
+typedef struct {
+    const void *x, *residual;
+    void *y;
+    int64_t rows, cols;
+    mx_drop drop;
+    int32_t vectors;           /* rows are whole 16-byte vectors of aligned memory */
+} mx_dropout_launch;
+
+/* All return a CUDA error code (0: queued). */
+int mc_launch_mx_encode(const mx_encode_launch *L, int type, int sms, void *stream);
+int mc_launch_mx_decode(const mx_decode_launch *L, int type, int sms, void *stream);
+int mc_launch_mx_quantize(const mx_quantize_launch *L, int type, void *stream);
+int mc_launch_mx_dequantize(const mx_dequantize_launch *L, int type, void *stream);
+int mc_launch_mx_product(const mx_product_launch *L, int type, int sms, void *stream);
+int mc_launch_mx_dropout(const mx_dropout_launch *L, int type, int sms, void *stream);
+int mc_mx_errors(uint32_t *word);
+uint32_t mc_mx_hash(uint32_t x);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif

@@ -1,0 +1,330 @@
+// mc_mx4_product.cu -- out[t][n] = sum over k of a[t][k] * b[n][k], both
+// factors in microscaled 4-bit form, on the tensor cores (tcgen05.mma,
+// kind::mxf4 with a scale per 32 elements), sums in float32.
+//
+// The matrices lie in memory as the tensor cores want them in shared memory:
+// panels of 256 columns, in a panel 128 bytes a row with the 128-byte swizzle
+// already applied, and the scales in pieces of 128 rows by 4.  So a tile of
+// any rows is one contiguous run, and a bulk copy brings it in.
+//
+// b's rows are the instruction's M (128 lanes of the accumulator), a's rows
+// its N: neighbouring lanes are neighbouring elements of a row of `out`, and
+// few rows of a (tokens) cost a narrow instruction instead of an empty one.
+
+#include "mc_mx4_device.h"
+
+namespace {
+
+// ------------------------------------------------------------ instructions
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bulk_g2s(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+                 "selp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    return done != 0;
+}
+// Every wait is bounded: false when it ran out (some seconds).
+__device__ __noinline__ bool mbar_wait_long(uint32_t bar, uint32_t parity, uint32_t seconds) {
+    uint64_t t0, t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+    for (uint32_t i = 0; i < 1u << 26; i++) {
+        if (mbar_try_wait(bar, parity)) return true;
+        asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+        if (t - t0 > seconds * 1000000000ull) return false;
+    }
+    return false;
+}
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint32_t seconds) {
+    return mbar_try_wait(bar, parity) || mbar_wait_long(bar, parity, seconds);
+}
+
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+template <int COLUMNS>
+__device__ __forceinline__ void tmem_alloc(uint32_t dst) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "n"(COLUMNS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+template <int COLUMNS>
+__device__ __forceinline__ void tmem_free(uint32_t at) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "n"(COLUMNS));
+}
+__device__ __forceinline__ void tc_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// 512 bytes of scales (128 rows, 4 each) to 4 columns, for all four quarters of the lanes
+__device__ __forceinline__ void tc_copy_scales(uint32_t tmem, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+__device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
+                                       uint32_t add) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(add) : "memory");
+}
+__device__ __forceinline__ void tc_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// 16 columns of a warp's 32 lanes
+__device__ __forceinline__ void tc_ld16(uint32_t at, uint32_t *r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(at));
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ld_cluster(uint32_t at, uint32_t rank) {
+    float v;
+    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}"
+                 : "=f"(v) : "r"(at), "r"(rank) : "memory");
+    return v;
+}
+
+// Shared memory matrix, rows of 128 bytes with the 128-byte swizzle, 8 rows
+// 1024 bytes further on.
+__device__ __forceinline__ uint64_t desc_codes(uint32_t at) {
+    return (uint64_t)(at >> 4 & 0x3FFF) | 1ull << 16 | 64ull << 32 | 1ull << 46 | 2ull << 61;
+}
+// 16 bytes a row, 8 rows 128 bytes further on, no swizzle.
+__device__ __forceinline__ uint64_t desc_scales(uint32_t at) {
+    return (uint64_t)(at >> 4 & 0x3FFF) | 1ull << 16 | 8ull << 32 | 1ull << 46;
+}
+
+__device__ uint32_t g_mx_error;   // a wait ran out
+
+// --------------------------------------------------------------- constants
+// BN: rows of a in a tile.
+template <int BN>
+struct mx_cfg {
+    static constexpr int GROUPS = BN > 128 ? 2 : 1;                  // of a's rows with scales
+    static constexpr int B_BYTES = 128 * 128, A_BYTES = BN * 128;    // codes of a panel
+    static constexpr int STAGE = B_BYTES + A_BYTES + 1024 + GROUPS * 1024;
+    static constexpr int ROOM = BN == 256 ? 225 * 1024 : BN == 128 ? 112 * 1024 : 100 * 1024;
+    static constexpr int STAGES = ROOM / STAGE < 8 ? ROOM / STAGE : 8;
+    static constexpr int SMEM = STAGES * STAGE + 1024;
+    static constexpr int SCALES = 8 + 8 * GROUPS;                    // columns of a panel's scales
+    static constexpr int NEED = BN + 2 * SCALES;
+    static constexpr int COLUMNS = NEED <= 64 ? 64 : NEED <= 128 ? 128 : NEED <= 256 ? 256 : 512;
+    // E2M1 both, E8M0 scales, M = 128
+    static constexpr uint32_t IDESC = 1u << 7 | 1u << 10 | (uint32_t)(BN / 8) << 17 | 1u << 23 | 1u << 27;
+};
+
+#define MX_THREADS 192   // warps 0 to 3: results; 4: copies; 5: instructions
+
+template <typename T, bool DROP>
+__device__ __forceinline__ void put(const mx_product_launch &L, mx_key key, int64_t wide, int64_t t, int64_t n, float v) {
+    if (DROP) {
+        const uint64_t pair = (uint64_t)(t * wide + n) / 2;
+        const uint32_t w = mx_word(mx_key_at(key, pair), (uint32_t)pair);
+        v = ((n & 1) ? w >> 16 : w & 0xFFFFu) < L.drop.threshold ? 0.0f : v * L.drop.factor;
+    }
+    mx_from((T *)L.out + t * L.ld + n, v);
+}
+
+// One tile of 128 x BN a CTA.  The CTAs of a cluster have the same tile and a
+// share of the panels each; their sums meet in the order of the ranks.
+template <typename T, int BN, bool DROP>
+__global__ void __launch_bounds__(MX_THREADS) k_mx_product(const __grid_constant__ mx_product_launch L, int tiles_n, int split) {
+    typedef mx_cfg<BN> C;
+    extern __shared__ uint8_t s_raw[];
+    __shared__ __align__(8) uint64_t s_full[C::STAGES], s_empty[C::STAGES], s_done;
+    __shared__ uint32_t s_tmem, s_failed;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t smem = (smem_u32(s_raw) + 1023) & ~1023u;
+    const int rank = blockIdx.x % split, tile = blockIdx.x / split;
+    const int64_t n0 = (int64_t)(tile % tiles_n) * 128, t0 = (int64_t)(tile / tiles_n) * BN;
+    const int64_t cols = L.a.cols;
+    const int panels = (int)((cols + MX_PANEL - 1) / MX_PANEL);
+    const int p0 = (int)((int64_t)panels * rank / split), p1 = (int)((int64_t)panels * (rank + 1) / split);
+
+    if (warp == 5) tmem_alloc<C::COLUMNS>(smem_u32(&s_tmem));
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::STAGES; i++) {
+            mbar_init(smem_u32(&s_full[i]), 1);
+            mbar_init(smem_u32(&s_empty[i]), 1);
+        }
+        mbar_init(smem_u32(&s_done), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        s_failed = 0;
+    }
+    tc_before_sync();
+    __syncthreads();
+    tc_after_sync();
+    const uint32_t tmem = s_tmem;
+
+    if (warp == 4 && elect_one()) {
+        const int64_t rows_b = mx_rows8(L.b.rows), rows_a = mx_rows8(L.a.rows);
+        const int64_t groups_b = (L.b.rows + 127) / 128, groups_a = (L.a.rows + 127) / 128;
+        const uint32_t nb = (uint32_t)min((int64_t)128, rows_b - n0) * 128, na = (uint32_t)min((int64_t)BN, rows_a - t0) * 128;
+        const uint32_t ga = (uint32_t)min((int64_t)C::GROUPS, groups_a - t0 / 128) * 1024;
+        int issued = p0;
+        for (int p = p0; p < p1; p++) {
+            const int i = p - p0, s = i % C::STAGES;
+            if (i >= C::STAGES && !mbar_wait(smem_u32(&s_empty[s]), (i / C::STAGES - 1) & 1, 4)) {
+                s_failed = 1;
+                break;
+            }
+            const uint32_t at = smem + s * C::STAGE, bar = smem_u32(&s_full[s]);
+            mbar_expect_tx(bar, nb + na + 1024 + ga);
+            bulk_g2s(at, L.b.codes + ((int64_t)p * rows_b + n0) * 128, nb, bar);
+            bulk_g2s(at + C::B_BYTES, L.a.codes + ((int64_t)p * rows_a + t0) * 128, na, bar);
+            bulk_g2s(at + C::B_BYTES + C::A_BYTES, L.b.scales + ((int64_t)p * groups_b + n0 / 128) * 1024, 1024, bar);
+            bulk_g2s(at + C::B_BYTES + C::A_BYTES + 1024, L.a.scales + ((int64_t)p * groups_a + t0 / 128) * 1024, ga, bar);
+            issued = p + 1;
+        }
+        if (s_failed)   // no copy may outlive the CTA
+            for (int i = max(0, issued - p0 - C::STAGES); i < issued - p0; i++)
+                mbar_wait(smem_u32(&s_full[i % C::STAGES]), (i / C::STAGES) & 1, 2);
+    }
+    if (warp == 5 && elect_one()) {
+        for (int p = p0; p < p1; p++) {
+            const int i = p - p0, s = i % C::STAGES;
+            bool ok = mbar_wait(smem_u32(&s_full[s]), (i / C::STAGES) & 1, 4);
+            // the columns of scales are free once the panel before the last one is done with
+            if (ok && i >= 2) ok = mbar_wait(smem_u32(&s_empty[(i - 2) % C::STAGES]), ((i - 2) / C::STAGES) & 1, 4);
+            if (!ok) {
+                s_failed = 1;
+                break;
+            }
+            tc_after_sync();
+            const uint32_t at = smem + s * C::STAGE, sb = at + C::B_BYTES + C::A_BYTES, sa = sb + 1024;
+            const uint32_t cols_b = tmem + BN + (i & 1) * C::SCALES, cols_a = cols_b + 8;
+            const int steps = (int)min((int64_t)4, (cols - (int64_t)p * MX_PANEL + 63) / 64);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                tc_copy_scales(cols_b + h * 4, desc_scales(sb + h * 512));
+#pragma unroll
+                for (int g = 0; g < C::GROUPS; g++)
+                    tc_copy_scales(cols_a + (h * C::GROUPS + g) * 4, desc_scales(sa + g * 1024 + h * 512));
+            }
+            const uint64_t db = desc_codes(at), da = desc_codes(at + C::B_BYTES);
+            for (int j = 0; j < steps; j++) {
+                const uint32_t id = (j & 1) * 2, h = j >> 1;
+                tc_mma(tmem, db + 2 * j, da + 2 * j, C::IDESC | id << 4 | id << 29, cols_b + h * 4,
+                       cols_a + h * C::GROUPS * 4, i > 0 || j > 0);
+            }
+            tc_commit(smem_u32(&s_empty[s]));
+        }
+        tc_commit(smem_u32(&s_done));
+    }
+    __syncwarp();
+
+    bool fine = true;
+    if (warp < 4) fine = mbar_wait(smem_u32(&s_done), 0, 16);
+    if (!fine) s_failed = 1;
+    tc_after_sync();
+    const int64_t n = n0 + 32 * warp + lane;
+    const int valid = (int)min((int64_t)BN, L.a.rows - t0);
+    mx_key key = {};
+    if (DROP) key = mx_key_of(L.drop.random);
+    const int64_t wide = mx_wide(L.b.rows);
+    const uint32_t mine = tmem + ((uint32_t)(32 * warp) << 16);
+    if (split == 1) {
+        if (warp < 4) {
+            for (int c = 0; c < BN; c += 16) {
+                if (c >= valid) break;
+                uint32_t r[16];
+                __syncwarp();
+                tc_ld16(mine + c, r);
+                tc_wait_ld();
+                if (n < L.b.rows && fine)
+#pragma unroll
+                    for (int j = 0; j < 16; j++)
+                        if (c + j < valid) put<T, DROP>(L, key, wide, t0 + c + j, n, panels ? __uint_as_float(r[j]) : 0.0f);
+            }
+        }
+    } else {
+        // [BN][128] float32 over the stages, which are all used up
+        if (warp < 4)
+            for (int c = 0; c < BN && c < valid; c += 16) {
+                uint32_t r[16];
+                tc_ld16(mine + c, r);
+                tc_wait_ld();
+#pragma unroll
+                for (int j = 0; j < 16; j++)
+                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(smem + ((c + j) * 128 + 32 * warp + lane) * 4), "r"(r[j]) : "memory");
+            }
+        cluster_sync();
+        if (warp < 4 && n < L.b.rows) {
+            const int from = valid * rank / split, to = valid * (rank + 1) / split;
+            for (int c = from; c < to; c++) {
+                float v = 0.0f;
+                for (int q = 0; q < split; q++) v += ld_cluster(smem + (c * 128 + 32 * warp + lane) * 4, q);
+                put<T, DROP>(L, key, wide, t0 + c, n, v);
+            }
+        }
+        __syncwarp();
+        cluster_sync();
+    }
+    tc_before_sync();
+    __syncthreads();
+    if (threadIdx.x == 0 && s_failed) atomicExch(&g_mx_error, 1u);
+    if (warp == 5) tmem_free<C::COLUMNS>(tmem);
+}
+
+template <typename T, int BN, bool DROP>
+static int product_as(const mx_product_launch &L, int sms, cudaStream_t s) {
+    typedef mx_cfg<BN> C;
+    auto kern = k_mx_product<T, BN, DROP>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (e != cudaSuccess) return e;
+    const int64_t tiles_n = (L.b.rows + 127) / 128, tiles_t = (L.a.rows + BN - 1) / BN, tiles = tiles_n * tiles_t;
+    const int64_t panels = (L.a.cols + MX_PANEL - 1) / MX_PANEL;
+    int split = 1;
+    while (split < 8 && tiles * split * 2 <= sms && split * 2 <= panels) split *= 2;
+    if (tiles * split > 0x7FFFFFFF) return cudaErrorInvalidValue;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(tiles * split));
+    cfg.blockDim = dim3(MX_THREADS);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)split;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, kern, L, (int)tiles_n, split);
+    const cudaError_t late = cudaGetLastError();
+    return e != cudaSuccess ? e : late;
+}
+
+template <typename T, bool DROP>
+static int product_for(const mx_product_launch &L, int sms, cudaStream_t s) {
+    const int64_t t = L.a.rows;
+    if (t <= 16) return product_as<T, 16, DROP>(L, sms, s);
+    if (t <= 32) return product_as<T, 32, DROP>(L, sms, s);
+    if (t <= 64) return product_as<T, 64, DROP>(L, sms, s);
+    if (t <= 128) return product_as<T, 128, DROP>(L, sms, s);
+    return product_as<T, 256, DROP>(L, sms, s);
+}
+
+template <typename T>
+static int product(const mx_product_launch &L, int sms, cudaStream_t s) {
+    return L.drop.random.on ? product_for<T, true>(L, sms, s) : product_for<T, false>(L, sms, s);
+}
+
+}  // namespace
+
+extern "C" int mc_launch_mx_product(const mx_product_launch *L, int type, int sms, void *stream) {
+    if (type == FALCOM_TYPE_F32) return product<float>(*L, sms, (cudaStream_t)stream);
+    if (type == FALCOM_TYPE_BF16) return product<__nv_bfloat16>(*L, sms, (cudaStream_t)stream);
+    return product<__half>(*L, sms, (cudaStream_t)stream);
+}
+
+extern "C" int mc_mx_errors(uint32_t *word) { return cudaMemcpyFromSymbol(word, g_mx_error, sizeof(*word)); }

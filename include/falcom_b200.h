@@ -449,6 +449,117 @@ int falcom_adamw_errors(falcom_adamw *plan);
 int falcom_adamw_graphs(const falcom_adamw *plan);
 void falcom_adamw_destroy(falcom_adamw *plan);
 
+/* Microscaled 4-bit floating point, and dropout.  No counterpart in the
+ * reference interface.
+ *
+ * What comes next to the codec on the way down and on a client: a server
+ * sends its new model in 4 bits (encode), clients bring theirs forward
+ * (decode), and compute with 4-bit factors on the tensor cores (quantize,
+ * product); dropout needs no stored mask.
+ *
+ * The format.  FALCOM_MX4_BLOCK consecutive elements share one scale byte s,
+ * which stands for 2^(s - 127): the smallest such power (2^-127 at least)
+ * with which no magnitude of the block is above 6 times the scale.  An
+ * element is 4 bits, sign above a magnitude code 0..7 for 0, 0.5, 1, 1.5, 2,
+ * 3, 4, 6 (times the scale).  No value is clipped.  A block with an infinity
+ * or NaN gets the scale byte 255, codes 0, and reads back as NaN throughout.
+ * Elements are taken as float32 values of their type.  Rounding is to the
+ * nearest value, ties to the even code; or, when a falcom_random is given, up
+ * or down at random: up when the distance from the value below, as a part of
+ * the distance between the two, is at least 1 - (u + 1/2) / 65536, u being
+ * the element's 16 random bits.
+ *
+ * Random bits are a hash and need no state.  With mix the 32-bit avalanche
+ *   x ^= x >> 16; x *= 0x85EBCA6B; x ^= x >> 13; x *= 0xC2B2AE35; x ^= x >> 16
+ * and purpose 0x9E3779B9 for rounding, 0x7F4A7C15 for dropout:
+ *   a = mix(mix(mix(mix(seed_low ^ purpose) ^ seed_high) ^ counter_low) ^ counter_high)
+ *   b = mix(a ^ 0x85EBCA77)
+ * Elements at positions 2 j and 2 j + 1 have the low and the high 16 bits of
+ *   x = j_low ^ a ^ mix(j_high), then mix's lines, with x ^= b after its first
+ *   product.
+ * The position of element (r, c) of a matrix of `cols` columns is
+ * r * (cols rounded up to 32) + c, that of element i of a vector is i.
+ * `counter` points to a number in device memory that is read when the work
+ * runs, so that a captured graph has other bits each time if the caller
+ * counts it up; NULL counts as 0.
+ *
+ * Common rules.  All data is device memory of one device; calls queue work
+ * on `stream` (cudaStream_t of that device, NULL = its legacy default
+ * stream), whatever device is current, need no workspace, may be captured,
+ * and may run at the same time on several streams as long as their outputs
+ * are apart.  Results are the same bits every time.  Element types are those
+ * above, each array aligned to its element size; codes and scales 16 bytes.
+ * An output may not overlap anything else, but for dropout's y, which may be
+ * x or the residual itself.  Return values: 0; ERROR_INVALID_PARAM for bad
+ * arguments; ERROR_COMPRESSION when a launch fails or a CUDA error from
+ * earlier work is pending (nothing is launched then). */
+#define FALCOM_MX4_BLOCK 32
+typedef struct falcom_random {
+    uint64_t seed;
+    const int64_t *counter;   /* device memory, or NULL */
+} falcom_random;
+typedef struct falcom_dropout_args {
+    double p;                 /* 0 <= p < 1; an element is dropped with round(65536 p) / 65536 */
+    falcom_random random;
+} falcom_dropout_args;
+
+/* A vector of n elements: codes[(n + 1) / 2], the even element in the low
+ * half (the last high half 0), scales[(n + 31) / 32].
+ * falcom_mx4_encode, base NULL: x into codes and scales.  With base
+ * (float32[n], what the receivers hold): the differences x - base, rounded to
+ * float32, and base += what they read back as, so that what was rounded away
+ * is part of the next difference.
+ * falcom_mx4_decode: v = weight * value (float32, rounded once);
+ * out = v, or out = out + v with accumulate (each rounded to float32, then
+ * to out's type). */
+int falcom_mx4_encode(const void *x, int dtype, size_t n, float *base, const falcom_random *random, void *codes,
+                      void *scales, void *stream);
+int falcom_mx4_decode(const void *codes, const void *scales, size_t n, float weight, int accumulate, void *out,
+                      int dtype, void *stream);
+
+/* A matrix for products, rounded along its rows.  Panels of 256 columns (the
+ * last one filled up with zeros); of a panel first all rows' codes, 128 bytes
+ * each, for rows up to a multiple of 8, the 16-byte piece of the row's block k
+ * (0..7) at k ^ (row & 7); scales in pieces of 512 bytes, [panel][row / 128]
+ * [half panel][row & 31][row / 32 & 3][block & 3].  falcom_mx4_codes_bytes and
+ * falcom_mx4_scales_bytes give the sizes; 0 for an empty matrix or one of
+ * more than 2^31 rows or columns.
+ * falcom_mx4_quantize rounds x (rows x cols, rows `ld` elements apart) along
+ * its rows into along_rows (rows x cols), along its columns into along_cols
+ * (the transposed matrix, cols x rows), or both from one read; NULL leaves one
+ * out.  With drop the elements go through dropout first (dropped ones are 0,
+ * others times 1 / (1 - p), in float32).  Random bits and dropout go by the
+ * element's place in x, along columns too.
+ * falcom_mx4_dequantize writes the values, rows `ld` elements apart. */
+typedef struct falcom_mx4_matrix {
+    void *codes, *scales;
+    size_t rows, cols;
+} falcom_mx4_matrix;
+size_t falcom_mx4_codes_bytes(size_t rows, size_t cols);
+size_t falcom_mx4_scales_bytes(size_t rows, size_t cols);
+int falcom_mx4_quantize(const void *x, int dtype, size_t rows, size_t cols, size_t ld, const falcom_random *random,
+                        const falcom_dropout_args *drop, const falcom_mx4_matrix *along_rows,
+                        const falcom_mx4_matrix *along_cols, void *stream);
+int falcom_mx4_dequantize(const falcom_mx4_matrix *m, void *out, int dtype, size_t ld, void *stream);
+
+/* out[i][j] = sum over k of a[i][k] * b[j][k], out's rows `ld` elements
+ * apart, summed in float32 on the tensor cores, rounded to dtype at the end;
+ * with drop, out is then put through dropout (before the last rounding).
+ * A sum over no columns is 0. */
+int falcom_mx4_product(const falcom_mx4_matrix *a, const falcom_mx4_matrix *b, void *out, int dtype, size_t ld,
+                       const falcom_dropout_args *drop, void *stream);
+/* 1 when a product on the current device gave up waiting for its own copies
+ * (some seconds; its result is then not to be used), else 0; negative when
+ * the device cannot be asked.  Waits for the device, so it does not belong
+ * inside a stream capture. */
+int falcom_mx4_errors(void);
+
+/* y = residual + (kept ? x / (1 - p) : 0) in float32 (x times the rounded
+ * factor), rounded to dtype; residual NULL counts as 0.  The same call without
+ * a residual on the gradient of y gives that of x. */
+int falcom_dropout(const void *x, const void *residual, void *y, int dtype, size_t rows, size_t cols,
+                   const falcom_dropout_args *drop, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

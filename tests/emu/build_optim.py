@@ -15,7 +15,7 @@ from tests.emu import build as base  # noqa: E402
 from tests.emu import prep  # noqa: E402
 
 BUILD = os.path.join(HERE, "_build_optim")
-INPUTS = [os.path.join(base.CSRC, f) for f in ("mc_optim.c", "mc_optim.cu", "mc_optim.h", "mc_util.c", "mc_internal.h")] + \
+INPUTS = [os.path.join(base.CSRC, f) for f in ("mc_optim.c", "mc_optim.cu", "mc_optim.h", "mc_call.h", "mc_util.c", "mc_internal.h")] + \
          [os.path.join(base.INCLUDE, "falcom_b200.h")] + \
          [os.path.join(HERE, f) for f in ("emu.h", "emu_optim.h", "fake_cudart.cpp", "prep.py", "build_optim.py")]
 

@@ -277,6 +277,275 @@ __global__ void __launch_bounds__(MX_THREADS) k_mx_product(const __grid_constant
     if (warp == 5) tmem_free<C::COLUMNS>(tmem);
 }
 
+// ------------------------------------------------------------------- wide
+// Many tiles of 128 x 256: one CTA an SM takes tile after tile, and a tile's
+// results leave while the next one is summed.  Here a's rows are the lanes and
+// b's the columns of the sum, so that a lane has neighbouring elements of a
+// row of `out` in its registers, rounds two at a time and stores 16 bytes at a
+// time.  Two sums of 256 columns and the scales are more than the 512 columns
+// there are, so the two overlap by 64: those are read first, and the next
+// tile's first instruction waits for that alone.
+struct mx_wide_cfg {
+    static constexpr int BN = 256;
+    static constexpr int A_BYTES = 128 * 128, B_BYTES = BN * 128;
+    static constexpr int STAGE = A_BYTES + B_BYTES + 1024 + 2048, STAGES = 4;
+    static constexpr int PITCH = 128 + 16, OUT = 32 * PITCH;         // a warp's part of the results: 32 rows, 128 bytes each
+    static constexpr int SMEM = STAGES * STAGE + 4 * OUT + 1024;
+    static constexpr int SECOND = 192, OVERLAP = 64, SCALES_AT = 448, SCALES = 24;
+    static constexpr uint32_t IDESC = 1u << 7 | 1u << 10 | (uint32_t)(BN / 8) << 17 | 1u << 23 | 1u << 27;
+};
+#define MX_WIDE_THREADS 192   // warps 0 to 3: results; 4: copies; 5: instructions
+
+__device__ __forceinline__ void st_shared16(uint32_t at, uint4 v) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared16(uint32_t at) {
+    uint4 r;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at) : "memory");
+    return r;
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// 16 bytes of results.
+__device__ __forceinline__ uint4 pack16(const float *v, float) {
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
+    return *(const uint32_t *)&p;
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
+    const __half2 p = __floats2half2_rn(a, b);
+    return *(const uint32_t *)&p;
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack16(const float *v, T t) {
+    return make_uint4(pack2(v[0], v[1], t), pack2(v[2], v[3], t), pack2(v[4], v[5], t), pack2(v[6], v[7], t));
+}
+
+// The 16 bytes that end `off` bytes (0, 2, ..., 14) into `now`, after `last`.
+__device__ __forceinline__ uint4 shifted(uint4 last, uint4 now, uint32_t off) {
+    uint32_t w[8] = {last.x, last.y, last.z, last.w, now.x, now.y, now.z, now.w};
+    // from byte 16 - off on
+    const uint32_t from = 16 - off;
+    const bool c = from & 8, b = from & 4;
+#pragma unroll
+    for (int i = 0; i < 6; i++) w[i] = c ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i < 5; i++) w[i] = b ? w[i + 1] : w[i];
+    const uint32_t sel = from & 2 ? 0x5432u : 0x3210u;
+    return make_uint4(__byte_perm(w[0], w[1], sel), __byte_perm(w[1], w[2], sel), __byte_perm(w[2], w[3], sel),
+                      __byte_perm(w[3], w[4], sel));
+}
+
+// A warp's 32 rows of up to 128 bytes, from shared memory to `out` (of its
+// first row): 8 lanes a row, 16 bytes each, at any alignment.
+template <typename T>
+__device__ __forceinline__ void rows_out(uint32_t buf, uint8_t *out, int64_t ld_bytes, int rows, int bytes, int lane, bool even) {
+    constexpr int SIZE = sizeof(T), PITCH = mx_wide_cfg::PITCH;
+    const int h = lane & 7;
+    if (even && bytes == 128) {   // every row on a 16-byte boundary
+        uint8_t *g = out + (lane >> 3) * ld_bytes + 16 * h;
+        uint32_t at = buf + (lane >> 3) * PITCH + 16 * h;
+#pragma unroll
+        for (int r = 0; r < 32; r += 4, g += 4 * ld_bytes, at += 4 * PITCH)
+            if (r + (lane >> 3) < rows) *(uint4 *)g = ld_shared16(at);
+        return;
+    }
+    for (int r = lane >> 3; r < rows; r += 4) {
+        uint8_t *g = out + r * ld_bytes;
+        const uint32_t at = buf + r * PITCH;
+        const int off = (int)((uintptr_t)g & 15), end = off + bytes;
+        uint8_t *line = g - off;   // piece i of it: the image's bytes 16 i - off on
+        const uint4 now = ld_shared16(at + 16 * h);
+        if (off == 0) {
+            if (16 * h + 16 <= bytes) *(uint4 *)(line + 16 * h) = now;
+        } else if (h > 0 && 16 * h + 16 <= end) {
+            *(uint4 *)(line + 16 * h) = shifted(ld_shared16(at + 16 * h - 16), now, off);
+        }
+        // elements before the first and after the last whole piece, 16 / SIZE at most in each
+        const int head = off ? min(16, end) - off : 0, from = max(head, (end & ~15) - off);
+        for (int b = h * SIZE; b < head + bytes - from; b += 8 * SIZE) {
+            const int i = b < head ? b : from + b - head;
+            if (SIZE == 4) {
+                uint32_t v;
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at + i) : "memory");
+                *(uint32_t *)(g + i) = v;
+            } else {
+                uint16_t v;
+                asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(at + i) : "memory");
+                *(uint16_t *)(g + i) = v;
+            }
+        }
+    }
+}
+
+template <typename T, bool DROP>
+__global__ void __launch_bounds__(MX_WIDE_THREADS, 1) k_mx_product_wide(const __grid_constant__ mx_product_launch L, int tiles_n, int tiles) {
+    typedef mx_wide_cfg C;
+    constexpr int CHUNK = 128 / sizeof(T), CHUNKS = C::BN / CHUNK, FIRST = C::OVERLAP / CHUNK, E = 16 / sizeof(T);
+    extern __shared__ uint8_t s_raw[];
+    __shared__ __align__(8) uint64_t s_full[C::STAGES], s_empty[C::STAGES], s_done, s_free;
+    __shared__ uint32_t s_tmem;
+    __shared__ volatile uint32_t s_failed;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t smem = (smem_u32(s_raw) + 1023) & ~1023u;
+    const int64_t cols = L.a.cols;
+    const int panels = (int)((cols + MX_PANEL - 1) / MX_PANEL);
+
+    if (warp == 5) tmem_alloc<512>(smem_u32(&s_tmem));
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::STAGES; i++) {
+            mbar_init(smem_u32(&s_full[i]), 1);
+            mbar_init(smem_u32(&s_empty[i]), 1);
+        }
+        mbar_init(smem_u32(&s_done), 1);
+        mbar_init(smem_u32(&s_free), 4);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        s_failed = 0;
+    }
+    tc_before_sync();
+    __syncthreads();
+    tc_after_sync();
+    const uint32_t tmem = s_tmem;
+
+    if (warp == 4 && elect_one()) {
+        const int64_t rows_b = mx_rows8(L.b.rows), rows_a = mx_rows8(L.a.rows);
+        const int64_t groups_b = (L.b.rows + 127) / 128, groups_a = (L.a.rows + 127) / 128;
+        int i = 0;   // panels so far
+        bool ok = true;
+        for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+            const int64_t n0 = (int64_t)(tile % tiles_n) * C::BN, t0 = (int64_t)(tile / tiles_n) * 128;
+            const uint32_t na = (uint32_t)min((int64_t)128, rows_a - t0) * 128, nb = (uint32_t)min((int64_t)C::BN, rows_b - n0) * 128;
+            const uint32_t gb = (uint32_t)min((int64_t)2, groups_b - n0 / 128) * 1024;
+            for (int p = 0; p < panels; p++, i++) {
+                const int s = i % C::STAGES;
+                if (i >= C::STAGES && !mbar_wait(smem_u32(&s_empty[s]), (i / C::STAGES - 1) & 1, 4)) {
+                    s_failed = 1;
+                    ok = false;
+                    break;
+                }
+                const uint32_t at = smem + s * C::STAGE, bar = smem_u32(&s_full[s]);
+                mbar_expect_tx(bar, na + nb + 1024 + gb);
+                bulk_g2s(at, L.a.codes + ((int64_t)p * rows_a + t0) * 128, na, bar);
+                bulk_g2s(at + C::A_BYTES, L.b.codes + ((int64_t)p * rows_b + n0) * 128, nb, bar);
+                bulk_g2s(at + C::A_BYTES + C::B_BYTES, L.a.scales + ((int64_t)p * groups_a + t0 / 128) * 1024, 1024, bar);
+                bulk_g2s(at + C::A_BYTES + C::B_BYTES + 1024, L.b.scales + ((int64_t)p * groups_b + n0 / 128) * 1024, gb, bar);
+            }
+        }
+        // no copy may outlive the CTA, whoever gave up
+        for (int k = max(0, i - C::STAGES); k < i; k++) mbar_wait(smem_u32(&s_full[k % C::STAGES]), (k / C::STAGES) & 1, 2);
+    }
+    if (warp == 5 && elect_one()) {
+        int i = 0, count = 0;
+        bool ok = true;
+        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, count++) {
+            const uint32_t sum = tmem + (count & 1) * C::SECOND;
+            if (count > 0) ok = mbar_wait(smem_u32(&s_free), (count - 1) & 1, 4);
+            tc_after_sync();
+            for (int p = 0; p < panels && ok; p++, i++) {
+                const int s = i % C::STAGES;
+                ok = mbar_wait(smem_u32(&s_full[s]), (i / C::STAGES) & 1, 4);
+                // the columns of scales are free once the panel before the last one is done with
+                if (ok && i >= 2) ok = mbar_wait(smem_u32(&s_empty[(i - 2) % C::STAGES]), ((i - 2) / C::STAGES) & 1, 4);
+                if (!ok) break;
+                tc_after_sync();
+                const uint32_t at = smem + s * C::STAGE, sa = at + C::A_BYTES + C::B_BYTES, sb = sa + 1024;
+                const uint32_t cols_a = tmem + C::SCALES_AT + (i & 1) * C::SCALES, cols_b = cols_a + 8;
+                const int steps = (int)min((int64_t)4, (cols - (int64_t)p * MX_PANEL + 63) / 64);
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    tc_copy_scales(cols_a + h * 4, desc_scales(sa + h * 512));
+#pragma unroll
+                    for (int g = 0; g < 2; g++) tc_copy_scales(cols_b + (h * 2 + g) * 4, desc_scales(sb + g * 1024 + h * 512));
+                }
+                const uint64_t da = desc_codes(at), db = desc_codes(at + C::A_BYTES);
+                for (int j = 0; j < steps; j++) {
+                    const uint32_t id = (j & 1) * 2, h = j >> 1;
+                    tc_mma(sum, da + 2 * j, db + 2 * j, C::IDESC | id << 4 | id << 29, cols_a + h * 4, cols_b + h * 8, p > 0 || j > 0);
+                }
+                tc_commit(smem_u32(&s_empty[s]));
+            }
+            if (!ok) {
+                s_failed = 1;
+                break;
+            }
+            tc_commit(smem_u32(&s_done));
+        }
+        if (!ok) {   // what was issued ends before the memory goes
+            tc_commit(smem_u32(&s_done));
+            mbar_wait(smem_u32(&s_done), count & 1, 2);
+        }
+    }
+    __syncwarp();
+    if (warp < 4) {
+        const uint32_t buf = smem + C::STAGES * C::STAGE + warp * C::OUT;
+        const int64_t ld_bytes = L.ld * (int64_t)sizeof(T), wide = mx_wide(L.b.rows);
+        const bool even = (((uintptr_t)L.out | (uintptr_t)ld_bytes) & 15) == 0;
+        mx_key key = {};
+        if (DROP) key = mx_key_of(L.drop.random);
+        int count = 0;
+        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, count++) {
+            const int64_t n0 = (int64_t)(tile % tiles_n) * C::BN, t0 = (int64_t)(tile / tiles_n) * 128 + 32 * warp;
+            const int rows = (int)max((int64_t)0, min((int64_t)32, L.a.rows - t0)), columns = (int)min((int64_t)C::BN, L.b.rows - n0);
+            uint8_t *out = (uint8_t *)L.out + t0 * ld_bytes + n0 * (int64_t)sizeof(T);
+            if (!s_failed && !mbar_wait(smem_u32(&s_done), count & 1, 20)) s_failed = 1;
+            tc_after_sync();
+            const uint32_t mine = tmem + (count & 1) * C::SECOND + ((uint32_t)(32 * warp) << 16);
+            for (int k = 0; k < CHUNKS; k++) {
+                const int c = ((count & 1 ? 0 : CHUNKS - FIRST) + k) % CHUNKS * CHUNK;
+                const bool some = c < columns && rows > 0;
+                float v[CHUNK];
+                if (some) {
+#pragma unroll
+                    for (int j = 0; j < CHUNK; j += 16) tc_ld16(mine + c + j, (uint32_t *)v + j);
+                    tc_wait_ld();
+                }
+                if (k == FIRST - 1) {   // the overlap is read
+                    tc_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&s_free));
+                }
+                if (!some) continue;
+                if (DROP) {
+                    const uint64_t pair = (uint64_t)((t0 + lane) * wide + n0 + c) / 2;
+                    const mx_key q = mx_key_at(key, pair);   // (a chunk's pairs have the same high bits: they are aligned)
+#pragma unroll
+                    for (int j = 0; j < CHUNK; j += 2) {
+                        const uint32_t w = mx_word(q, (uint32_t)pair + j / 2);
+                        v[j] = (w & 0xFFFFu) < L.drop.threshold ? 0.0f : v[j] * L.drop.factor;
+                        v[j + 1] = (w >> 16) < L.drop.threshold ? 0.0f : v[j + 1] * L.drop.factor;
+                    }
+                }
+                __syncwarp();   // the last part has left the buffer
+#pragma unroll
+                for (int j = 0; j < CHUNK; j += E) st_shared16(buf + lane * C::PITCH + j * sizeof(T), pack16(v + j, T()));
+                __syncwarp();
+                if (!s_failed)
+                    rows_out<T>(buf, out + c * (int64_t)sizeof(T), ld_bytes, rows, min(CHUNK, columns - c) * (int)sizeof(T), lane, even);
+            }
+        }
+    }
+    tc_before_sync();
+    __syncthreads();
+    if (threadIdx.x == 0 && s_failed) atomicExch(&g_mx_error, 1u);
+    if (warp == 5) tmem_free<512>(tmem);
+}
+
+template <typename T, bool DROP>
+static int product_wide(const mx_product_launch &L, int sms, cudaStream_t s) {
+    typedef mx_wide_cfg C;
+    auto kern = k_mx_product_wide<T, DROP>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (e != cudaSuccess) return e;
+    const int64_t tiles_n = (L.b.rows + C::BN - 1) / C::BN, tiles = tiles_n * ((L.a.rows + 127) / 128);
+    if (tiles > 0x3FFFFFFF) return cudaErrorInvalidValue;
+    kern<<<(unsigned)(tiles < sms ? tiles : sms), MX_WIDE_THREADS, C::SMEM, s>>>(L, (int)tiles_n, (int)tiles);
+    return cudaGetLastError();
+}
+
 template <typename T, int BN, bool DROP>
 static int product_as(const mx_product_launch &L, int sms, cudaStream_t s) {
     typedef mx_cfg<BN> C;
@@ -311,7 +580,10 @@ static int product_for(const mx_product_launch &L, int sms, cudaStream_t s) {
     if (t <= 32) return product_as<T, 32, DROP>(L, sms, s);
     if (t <= 64) return product_as<T, 64, DROP>(L, sms, s);
     if (t <= 128) return product_as<T, 128, DROP>(L, sms, s);
-    return product_as<T, 256, DROP>(L, sms, s);
+    const int64_t tiles = (L.b.rows + 255) / 256 * ((t + 127) / 128);
+    // fewer tiles than SMs: their panels are shared out
+    if (tiles * 2 <= sms || L.a.cols == 0 || L.b.rows <= 128) return product_as<T, 256, DROP>(L, sms, s);
+    return product_wide<T, DROP>(L, sms, s);
 }
 
 template <typename T>

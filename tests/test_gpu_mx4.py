@@ -59,6 +59,21 @@ def test_product(mx4, t, n, k, dtype):
     assert torch.equal(y, mx4.product(a, b, dtype=dtype)) and mx4.errors() == 0
 
 
+# enough tiles for every SM to take several, rows of `out` at all offsets from 16 bytes, sums of one and of many panels
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("t,n,k", [(2048, 4096, 64), (1500, 5001, 300), (4099, 2051, 1025), (300, 20010, 256), (257, 19000, 2048)])
+def test_product_of_many_tiles(mx4, t, n, k, dtype):
+    a, b = mx4.quantize(wild(t, k, torch.float32, 1).cuda()), mx4.quantize(wild(n, k, torch.float32, 2).cuda())
+    room = torch.full((t * n + 64,), 7.0, dtype=dtype, device="cuda")
+    y = mx4.product(a, b, out=room[13:13 + t * n].view(t, n))
+    u, v = a.dequantize().double(), b.dequantize().double()
+    want = u @ v.t()
+    finite = want.abs() < torch.finfo(dtype).max / 2
+    assert ((y.double() - want).abs() <= ref.sum_bound(u, v, dtype))[finite].all()
+    assert (room[:13] == 7).all() and (room[13 + t * n:] == 7).all() and mx4.errors() == 0
+    assert torch.equal(y, mx4.product(a, b, dtype=dtype))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("p", [0.0, 0.25])
 @pytest.mark.parametrize("t,k,n", [(1, 32, 8), (77, 513, 10), (130, 96, 257)])

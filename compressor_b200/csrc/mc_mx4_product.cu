@@ -11,6 +11,8 @@
 // its N: neighbouring lanes are neighbouring elements of a row of `out`, and
 // few rows of a (tokens) cost a narrow instruction instead of an empty one.
 
+#include <cuda.h>
+
 #include "mc_mx4_device.h"
 
 namespace {
@@ -33,9 +35,12 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
                  "selp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
     return done != 0;
 }
-// Every wait is bounded: false when it ran out (some seconds).
+// Every wait is bounded: false when it ran out (some seconds).  The clock is
+// looked at late and rarely.
 __device__ __noinline__ bool mbar_wait_long(uint32_t bar, uint32_t parity, uint32_t seconds) {
     uint64_t t0, t;
+    for (int i = 0; i < 256; i++)
+        if (mbar_try_wait(bar, parity)) return true;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
     for (uint32_t i = 0; i < 1u << 26; i++) {
         if (mbar_try_wait(bar, parity)) return true;
@@ -46,6 +51,17 @@ __device__ __noinline__ bool mbar_wait_long(uint32_t bar, uint32_t parity, uint3
 }
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint32_t seconds) {
     return mbar_try_wait(bar, parity) || mbar_wait_long(bar, parity, seconds);
+}
+
+// The same for a barrier at which threads of another CTA of the cluster arrive.
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+                 "selp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    return done != 0;
+}
+__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, uint32_t seconds) {
+    return mbar_try_wait_cluster(bar, parity) || (mbar_wait_long(bar, parity, seconds) && mbar_try_wait_cluster(bar, parity));
 }
 
 __device__ __forceinline__ bool elect_one() {
@@ -278,23 +294,65 @@ __global__ void __launch_bounds__(MX_THREADS) k_mx_product(const __grid_constant
 }
 
 // ------------------------------------------------------------------- wide
-// Many tiles of 128 x 256: one CTA an SM takes tile after tile, and a tile's
-// results leave while the next one is summed.  Here a's rows are the lanes and
-// b's the columns of the sum, so that a lane has neighbouring elements of a
-// row of `out` in its registers, rounds two at a time and stores 16 bytes at a
-// time.  Two sums of 256 columns and the scales are more than the 512 columns
-// there are, so the two overlap by 64: those are read first, and the next
-// tile's first instruction waits for that alone.
+// Many tiles of 256 x 256, each by a pair of CTAs on neighbouring SMs
+// (cta_group::2): each has half of a's rows and half of b's in shared memory,
+// and the sums of its half of a's rows, so a panel costs an SM 35 KB of copies
+// instead of 51.  A pair takes tile after tile, and a tile's results leave
+// while the next one is summed.  Here a's rows are the lanes and b's the
+// columns of the sum, so that a lane has neighbouring elements of a row of
+// `out` in its registers, rounds two at a time and stores 16 bytes at a time.
+// Two sums of 256 columns and the scales of 5 panels are more than the 512
+// columns there are, so the sums overlap by 128: those are read first, and the
+// next tile's first instruction waits for that alone.
 struct mx_wide_cfg {
-    static constexpr int BN = 256;
-    static constexpr int A_BYTES = 128 * 128, B_BYTES = BN * 128;
-    static constexpr int STAGE = A_BYTES + B_BYTES + 1024 + 2048, STAGES = 4;
+    static constexpr int BN = 256, THREADS = 320;                    // warps 0 to 7: results; 8: copies; 9: instructions
+    static constexpr int A_BYTES = 128 * 128, B_BYTES = BN / 2 * 128;
+    static constexpr int STAGE = A_BYTES + B_BYTES + 1024 + 2048, STAGES = 5;
     static constexpr int PITCH = 128 + 16, OUT = 32 * PITCH;         // a warp's part of the results: 32 rows, 128 bytes each
-    static constexpr int SMEM = STAGES * STAGE + 4 * OUT + 1024;
-    static constexpr int SECOND = 192, OVERLAP = 64, SCALES_AT = 448, SCALES = 24;
-    static constexpr uint32_t IDESC = 1u << 7 | 1u << 10 | (uint32_t)(BN / 8) << 17 | 1u << 23 | 1u << 27;
+    static constexpr int SMEM = STAGES * STAGE + 8 * OUT + 1024;
+    static constexpr int SECOND = 128, SCALES_AT = 384, SCALES = 24; // columns: a stage's scales have their own
+    static constexpr uint32_t IDESC = 1u << 7 | 1u << 10 | (uint32_t)(BN / 8) << 17 | 1u << 23 | 2u << 27;
+    static_assert(SMEM <= 227 * 1024 && SCALES_AT + STAGES * SCALES <= 512 && SECOND + BN <= SCALES_AT, "");
 };
-#define MX_WIDE_THREADS 192   // warps 0 to 3: results; 4: copies; 5: instructions
+
+// The forms for a pair.
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t dst) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "n"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+}
+__device__ __forceinline__ void tmem_free_pair(uint32_t at) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(at), "n"(512));
+}
+__device__ __forceinline__ void tc_copy_scales_pair(uint32_t tmem, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+__device__ __forceinline__ void tc_mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
+                                            uint32_t add) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+                 "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(add) : "memory");
+}
+// Arrives at the barrier of both CTAs.
+__device__ __forceinline__ void tc_commit_pair(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+// Arrives at the first CTA's barrier.  Relaxed: the arriving thread has read
+// sums (tcgen05.wait::ld) that may be written over now and hands on nothing
+// that it wrote; a release at cluster scope would wait for its stores of
+// results (over 1000 clocks).
+__device__ __forceinline__ void mbar_arrive_first(uint32_t bar) {
+    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, 0;\n\t"
+                 "mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [a];\n\t}" ::"r"(bar) : "memory");
+}
+// A box of rows from `row` on to this CTA's shared memory, which the first
+// CTA's barrier is told.
+__device__ __forceinline__ void load_rows_pair(uint32_t dst, const CUtensorMap *map, int32_t row, uint32_t bar) {
+    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %3, 0;\n\t"
+                 "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+                 "[%0], [%1, {%2, %4}], [a];\n\t}"
+                 ::"r"(dst), "l"(map), "r"(0), "r"(bar), "r"(row) : "memory");
+}
 
 __device__ __forceinline__ void st_shared16(uint32_t at, uint4 v) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
@@ -304,10 +362,6 @@ __device__ __forceinline__ uint4 ld_shared16(uint32_t at) {
     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at) : "memory");
     return r;
 }
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-
 // 16 bytes of results.
 __device__ __forceinline__ uint4 pack16(const float *v, float) {
     return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
@@ -325,177 +379,233 @@ __device__ __forceinline__ uint4 pack16(const float *v, T t) {
     return make_uint4(pack2(v[0], v[1], t), pack2(v[2], v[3], t), pack2(v[4], v[5], t), pack2(v[6], v[7], t));
 }
 
-// The 16 bytes that end `off` bytes (0, 2, ..., 14) into `now`, after `last`.
-__device__ __forceinline__ uint4 shifted(uint4 last, uint4 now, uint32_t off) {
-    uint32_t w[8] = {last.x, last.y, last.z, last.w, now.x, now.y, now.z, now.w};
-    // from byte 16 - off on
-    const uint32_t from = 16 - off;
-    const bool c = from & 8, b = from & 4;
+// The 16 bytes that begin `from` (0, 2, ..., 16) bytes into a and then b.
+__device__ __forceinline__ uint4 joined(uint4 a, uint4 b, uint32_t from) {
+    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    const bool two = from & 8, one = from & 4;
 #pragma unroll
-    for (int i = 0; i < 6; i++) w[i] = c ? w[i + 2] : w[i];
+    for (int i = 0; i < 6; i++) w[i] = two ? w[i + 2] : w[i];
 #pragma unroll
-    for (int i = 0; i < 5; i++) w[i] = b ? w[i + 1] : w[i];
+    for (int i = 0; i < 5; i++) w[i] = one ? w[i + 1] : w[i];
     const uint32_t sel = from & 2 ? 0x5432u : 0x3210u;
     return make_uint4(__byte_perm(w[0], w[1], sel), __byte_perm(w[1], w[2], sel), __byte_perm(w[2], w[3], sel),
                       __byte_perm(w[3], w[4], sel));
 }
 
-// A warp's 32 rows of up to 128 bytes, from shared memory to `out` (of its
-// first row): 8 lanes a row, 16 bytes each, at any alignment.
+// A warp's 32 rows of up to 128 bytes (`count` elements) from shared memory to
+// `out` (of its first row).  8 lanes have a row, 16 bytes each.  A row that
+// does not begin on a 16-byte boundary leaves in the 7 whole pieces that lie
+// in it, put together from two, and 16 / SIZE elements at its two ends, one a
+// lane.
 template <typename T>
-__device__ __forceinline__ void rows_out(uint32_t buf, uint8_t *out, int64_t ld_bytes, int rows, int bytes, int lane, bool even) {
+__device__ __forceinline__ void rows_out(uint32_t buf, uint8_t *out, int64_t ld_bytes, int rows, int count, int lane, bool even) {
     constexpr int SIZE = sizeof(T), PITCH = mx_wide_cfg::PITCH;
     const int h = lane & 7;
-    if (even && bytes == 128) {   // every row on a 16-byte boundary
-        uint8_t *g = out + (lane >> 3) * ld_bytes + 16 * h;
-        uint32_t at = buf + (lane >> 3) * PITCH + 16 * h;
+    uint8_t *g = out + (lane >> 3) * ld_bytes;
+    uint32_t at = buf + (lane >> 3) * PITCH;
+    // (all loads of a batch before its stores: one after the other they would wait for each other)
+    if (even && count * SIZE == 128) {
+        uint4 v[8];
 #pragma unroll
-        for (int r = 0; r < 32; r += 4, g += 4 * ld_bytes, at += 4 * PITCH)
-            if (r + (lane >> 3) < rows) *(uint4 *)g = ld_shared16(at);
-        return;
-    }
-    for (int r = lane >> 3; r < rows; r += 4) {
-        uint8_t *g = out + r * ld_bytes;
-        const uint32_t at = buf + r * PITCH;
-        const int off = (int)((uintptr_t)g & 15), end = off + bytes;
-        uint8_t *line = g - off;   // piece i of it: the image's bytes 16 i - off on
-        const uint4 now = ld_shared16(at + 16 * h);
-        if (off == 0) {
-            if (16 * h + 16 <= bytes) *(uint4 *)(line + 16 * h) = now;
-        } else if (h > 0 && 16 * h + 16 <= end) {
-            *(uint4 *)(line + 16 * h) = shifted(ld_shared16(at + 16 * h - 16), now, off);
-        }
-        // elements before the first and after the last whole piece, 16 / SIZE at most in each
-        const int head = off ? min(16, end) - off : 0, from = max(head, (end & ~15) - off);
-        for (int b = h * SIZE; b < head + bytes - from; b += 8 * SIZE) {
-            const int i = b < head ? b : from + b - head;
-            if (SIZE == 4) {
-                uint32_t v;
-                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at + i) : "memory");
-                *(uint32_t *)(g + i) = v;
-            } else {
-                uint16_t v;
-                asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(at + i) : "memory");
-                *(uint16_t *)(g + i) = v;
+        for (int i = 0; i < 8; i++) v[i] = ld_shared16(at + 4 * i * PITCH + 16 * h);
+#pragma unroll
+        for (int i = 0; i < 8; i++, g += 4 * ld_bytes)
+            if (4 * i + (lane >> 3) < rows) *(uint4 *)(g + 16 * h) = v[i];
+    } else if (count * SIZE == 128) {
+        constexpr int BATCH = 4;
+#pragma unroll 1
+        for (int r = lane >> 3; r < rows + (lane >> 3); r += 4 * BATCH, at += 4 * BATCH * PITCH) {
+            uint4 now[BATCH], last[BATCH];
+            uint32_t end[BATCH], off[BATCH];
+#pragma unroll
+            for (int i = 0; i < BATCH; i++) {
+                const uint32_t row = at + 4 * i * PITCH;
+                off[i] = ((uint32_t)(uintptr_t)g + 4 * i * (uint32_t)ld_bytes) & 15;
+                now[i] = ld_shared16(row + 16 * h);
+                last[i] = ld_shared16(row + 16 * h - (h ? 16 : 0));
+                // the elements at the ends: 16 - off bytes of them in front
+                const uint32_t e = row + h * SIZE + (h * SIZE < 16 - off[i] ? 0 : 112);
+                if (SIZE == 4) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(end[i]) : "r"(e) : "memory");
+                else asm volatile("{\n\t.reg .b16 x;\n\tld.shared.b16 x, [%1];\n\tcvt.u32.u16 %0, x;\n\t}" : "=r"(end[i]) : "r"(e) : "memory");
+            }
+#pragma unroll
+            for (int i = 0; i < BATCH; i++, g += 4 * ld_bytes) {
+                if (r + 4 * i >= rows) continue;
+                const uint4 v = joined(last[i], now[i], 16 - off[i]);
+                if (off[i] == 0) *(uint4 *)(g + 16 * h) = now[i];
+                else if (h > 0) *(uint4 *)(g + 16 * h - off[i]) = v;
+                if (off[i] != 0 && h * SIZE < 16) {
+                    uint8_t *e = g + h * SIZE + (h * SIZE < 16 - off[i] ? 0 : 112);
+                    if (SIZE == 4) *(uint32_t *)e = end[i];
+                    else *(uint16_t *)e = (uint16_t)end[i];
+                }
             }
         }
+    } else {   // the last columns of the matrix
+        for (int r = 0; r < rows; r++)
+            for (int i = lane; i < count; i += 32) {
+                if (SIZE == 4) {
+                    uint32_t v;
+                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(buf + r * PITCH + 4 * i) : "memory");
+                    ((uint32_t *)(out + r * ld_bytes))[i] = v;
+                } else {
+                    uint16_t v;
+                    asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(buf + r * PITCH + 2 * i) : "memory");
+                    ((uint16_t *)(out + r * ld_bytes))[i] = v;
+                }
+            }
     }
 }
 
+// Codes as rows of 128 bytes, scales as rows of 1024, of all panels.
+struct mx_maps {
+    CUtensorMap a_codes, b_codes, a_scales, b_scales;
+};
+
 template <typename T, bool DROP>
-__global__ void __launch_bounds__(MX_WIDE_THREADS, 1) k_mx_product_wide(const __grid_constant__ mx_product_launch L, int tiles_n, int tiles) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mx_wide_cfg::THREADS, 1)
+    k_mx_product_wide(const __grid_constant__ mx_product_launch L, const __grid_constant__ mx_maps M, int tiles_n, int tiles) {
     typedef mx_wide_cfg C;
-    constexpr int CHUNK = 128 / sizeof(T), CHUNKS = C::BN / CHUNK, FIRST = C::OVERLAP / CHUNK, E = 16 / sizeof(T);
+    constexpr int CHUNK = 128 / sizeof(T), PARTS = 64 / CHUNK, E = 16 / sizeof(T), BN = C::BN, COPIES = 8, ISSUE = 9;
     extern __shared__ uint8_t s_raw[];
-    __shared__ __align__(8) uint64_t s_full[C::STAGES], s_empty[C::STAGES], s_done, s_free;
+    // s_full: both CTAs' copies, at the first; s_done, s_free: for even and for odd tiles
+    __shared__ __align__(8) uint64_t s_full[C::STAGES], s_empty[C::STAGES], s_done[2], s_free[2];
     __shared__ uint32_t s_tmem;
     __shared__ volatile uint32_t s_failed;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     const uint32_t smem = (smem_u32(s_raw) + 1023) & ~1023u;
     const int64_t cols = L.a.cols;
-    const int panels = (int)((cols + MX_PANEL - 1) / MX_PANEL);
+    const int panels = (int)((cols + MX_PANEL - 1) / MX_PANEL), last_steps = (int)((cols - 1) % MX_PANEL) / 64 + 1;
 
-    if (warp == 5) tmem_alloc<512>(smem_u32(&s_tmem));
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::STAGES; i++) {
             mbar_init(smem_u32(&s_full[i]), 1);
             mbar_init(smem_u32(&s_empty[i]), 1);
         }
-        mbar_init(smem_u32(&s_done), 1);
-        mbar_init(smem_u32(&s_free), 4);
+        for (int i = 0; i < 2; i++) {
+            mbar_init(smem_u32(&s_done[i]), 1);
+            mbar_init(smem_u32(&s_free[i]), 16);   // the result warps of both
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         s_failed = 0;
     }
+    __syncthreads();
+    cluster_sync();
+    if (warp == ISSUE) tmem_alloc_pair(smem_u32(&s_tmem));
     tc_before_sync();
     __syncthreads();
+    cluster_sync();
     tc_after_sync();
     const uint32_t tmem = s_tmem;
 
-    if (warp == 4 && elect_one()) {
-        const int64_t rows_b = mx_rows8(L.b.rows), rows_a = mx_rows8(L.a.rows);
-        const int64_t groups_b = (L.b.rows + 127) / 128, groups_a = (L.a.rows + 127) / 128;
-        int i = 0;   // panels so far
+    if (warp == COPIES) {
+        // One lane for each of a panel's four copies: codes of a and of b, scales of a and of b.  Boxes are whole: what
+        // lies behind a matrix's last row belongs to rows or columns of the sum that nobody stores.
+        const CUtensorMap *map = lane == 0 ? &M.a_codes : lane == 1 ? &M.b_codes : lane == 2 ? &M.a_scales : &M.b_scales;
+        const int stride = (int)(lane == 0 ? mx_rows8(L.a.rows) : lane == 1 ? mx_rows8(L.b.rows) : ((lane == 2 ? L.a.rows : L.b.rows) + 127) / 128);
+        const uint32_t to = smem + (lane == 0 ? 0 : lane == 1 ? C::A_BYTES : C::A_BYTES + C::B_BYTES + (lane == 2 ? 0 : 1024));
+        int s = 0, used = 0;   // stage; stages used so far, up to all
+        uint32_t parity = 1;   // of the wait for an empty stage
         bool ok = true;
-        for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
-            const int64_t n0 = (int64_t)(tile % tiles_n) * C::BN, t0 = (int64_t)(tile / tiles_n) * 128;
-            const uint32_t na = (uint32_t)min((int64_t)128, rows_a - t0) * 128, nb = (uint32_t)min((int64_t)C::BN, rows_b - n0) * 128;
-            const uint32_t gb = (uint32_t)min((int64_t)2, groups_b - n0 / 128) * 1024;
-            for (int p = 0; p < panels; p++, i++) {
-                const int s = i % C::STAGES;
-                if (i >= C::STAGES && !mbar_wait(smem_u32(&s_empty[s]), (i / C::STAGES - 1) & 1, 4)) {
-                    s_failed = 1;
-                    ok = false;
-                    break;
+        for (int tile = pair; tile < tiles && ok; tile += pairs) {
+            const int n0 = tile % tiles_n * BN, t0 = tile / tiles_n * 256 + 128 * rank;
+            int row = lane == 0 ? t0 : lane == 1 ? n0 + BN / 2 * rank : lane == 2 ? t0 / 128 : n0 / 128;
+            for (int p = 0; p < panels; p++, row += stride) {
+                const uint32_t bar = smem_u32(&s_full[s]);
+                if (lane == 0) {
+                    if (used == C::STAGES) ok = mbar_wait(smem_u32(&s_empty[s]), parity, 4);
+                    if (ok && rank == 0) mbar_expect_tx(bar, 2 * C::STAGE);
                 }
-                const uint32_t at = smem + s * C::STAGE, bar = smem_u32(&s_full[s]);
-                mbar_expect_tx(bar, na + nb + 1024 + gb);
-                bulk_g2s(at, L.a.codes + ((int64_t)p * rows_a + t0) * 128, na, bar);
-                bulk_g2s(at + C::A_BYTES, L.b.codes + ((int64_t)p * rows_b + n0) * 128, nb, bar);
-                bulk_g2s(at + C::A_BYTES + C::B_BYTES, L.a.scales + ((int64_t)p * groups_a + t0 / 128) * 1024, 1024, bar);
-                bulk_g2s(at + C::A_BYTES + C::B_BYTES + 1024, L.b.scales + ((int64_t)p * groups_b + n0 / 128) * 1024, gb, bar);
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+                if (!ok) break;
+                if (lane < 4) load_rows_pair(to + s * C::STAGE, map, row, bar);
+                used = min(used + 1, C::STAGES);
+                if (++s == C::STAGES) {
+                    s = 0;
+                    parity ^= 1;
+                }
             }
         }
-        // no copy may outlive the CTA, whoever gave up
-        for (int k = max(0, i - C::STAGES); k < i; k++) mbar_wait(smem_u32(&s_full[k % C::STAGES]), (k / C::STAGES) & 1, 2);
+        if (lane == 0 && !ok) s_failed = 1;
+        // no copy may outlive the pair, whoever gave up: the last round of each stage
+        if (lane == 0 && rank == 0)
+            for (; used > 0; used--) {
+                if (s-- == 0) {
+                    s = C::STAGES - 1;
+                    parity ^= 1;
+                }
+                mbar_wait(smem_u32(&s_full[s]), parity ^ 1, 2);
+            }
     }
-    if (warp == 5 && elect_one()) {
-        int i = 0, count = 0;
+    if (warp == ISSUE && rank == 0 && elect_one()) {
+        const uint64_t codes = desc_codes(smem), scales = desc_scales(smem + C::A_BYTES + C::B_BYTES);
+        int s = 0, count = 0;
+        uint32_t parity = 0;
         bool ok = true;
-        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, count++) {
+        for (int tile = pair; tile < tiles; tile += pairs, count++) {
             const uint32_t sum = tmem + (count & 1) * C::SECOND;
-            if (count > 0) ok = mbar_wait(smem_u32(&s_free), (count - 1) & 1, 4);
+            // the tile before has left the overlap
+            if (count > 0) ok = mbar_wait_cluster(smem_u32(&s_free[(count - 1) & 1]), (count - 1) >> 1 & 1, 4);
             tc_after_sync();
-            for (int p = 0; p < panels && ok; p++, i++) {
-                const int s = i % C::STAGES;
-                ok = mbar_wait(smem_u32(&s_full[s]), (i / C::STAGES) & 1, 4);
-                // the columns of scales are free once the panel before the last one is done with
-                if (ok && i >= 2) ok = mbar_wait(smem_u32(&s_empty[(i - 2) % C::STAGES]), ((i - 2) / C::STAGES) & 1, 4);
+            for (int p = 0; p < panels && ok; p++) {
+                ok = mbar_wait_cluster(smem_u32(&s_full[s]), parity, 4);
+                // a full stage is one whose last panel is done with, and so are that panel's columns of scales
                 if (!ok) break;
                 tc_after_sync();
-                const uint32_t at = smem + s * C::STAGE, sa = at + C::A_BYTES + C::B_BYTES, sb = sa + 1024;
-                const uint32_t cols_a = tmem + C::SCALES_AT + (i & 1) * C::SCALES, cols_b = cols_a + 8;
-                const int steps = (int)min((int64_t)4, (cols - (int64_t)p * MX_PANEL + 63) / 64);
+                const uint64_t da = codes + s * (C::STAGE >> 4), db = da + (C::A_BYTES >> 4);
+                const uint64_t sa = scales + s * (C::STAGE >> 4), sb = sa + (1024 >> 4);
+                const uint32_t cols_a = tmem + C::SCALES_AT + s * C::SCALES, cols_b = cols_a + 8;
+                const int steps = p + 1 < panels ? 4 : last_steps;
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    tc_copy_scales(cols_a + h * 4, desc_scales(sa + h * 512));
+                    tc_copy_scales_pair(cols_a + h * 4, sa + h * (512 >> 4));
 #pragma unroll
-                    for (int g = 0; g < 2; g++) tc_copy_scales(cols_b + (h * 2 + g) * 4, desc_scales(sb + g * 1024 + h * 512));
+                    for (int g = 0; g < 2; g++) tc_copy_scales_pair(cols_b + (h * 2 + g) * 4, sb + g * (1024 >> 4) + h * (512 >> 4));
+#pragma unroll
+                    for (int j = 2 * h; j < 2 * h + 2; j++) {
+                        const uint32_t id = (j & 1) * 2;
+                        if (j < steps)
+                            tc_mma_pair(sum, da + 2 * j, db + 2 * j, C::IDESC | id << 4 | id << 29, cols_a + h * 4, cols_b + h * 8,
+                                        p > 0 || j > 0);
+                    }
                 }
-                const uint64_t da = desc_codes(at), db = desc_codes(at + C::A_BYTES);
-                for (int j = 0; j < steps; j++) {
-                    const uint32_t id = (j & 1) * 2, h = j >> 1;
-                    tc_mma(sum, da + 2 * j, db + 2 * j, C::IDESC | id << 4 | id << 29, cols_a + h * 4, cols_b + h * 8, p > 0 || j > 0);
+                tc_commit_pair(smem_u32(&s_empty[s]));
+                if (++s == C::STAGES) {
+                    s = 0;
+                    parity ^= 1;
                 }
-                tc_commit(smem_u32(&s_empty[s]));
             }
             if (!ok) {
                 s_failed = 1;
                 break;
             }
-            tc_commit(smem_u32(&s_done));
+            tc_commit_pair(smem_u32(&s_done[count & 1]));
         }
         if (!ok) {   // what was issued ends before the memory goes
-            tc_commit(smem_u32(&s_done));
-            mbar_wait(smem_u32(&s_done), count & 1, 2);
+            tc_commit_pair(smem_u32(&s_done[count & 1]));
+            mbar_wait(smem_u32(&s_done[count & 1]), count >> 1 & 1, 2);
         }
     }
     __syncwarp();
-    if (warp < 4) {
+    if (warp < COPIES) {
+        const int set = warp >> 2, quarter = warp & 3;
         const uint32_t buf = smem + C::STAGES * C::STAGE + warp * C::OUT;
         const int64_t ld_bytes = L.ld * (int64_t)sizeof(T), wide = mx_wide(L.b.rows);
         const bool even = (((uintptr_t)L.out | (uintptr_t)ld_bytes) & 15) == 0;
         mx_key key = {};
         if (DROP) key = mx_key_of(L.drop.random);
         int count = 0;
-        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, count++) {
-            const int64_t n0 = (int64_t)(tile % tiles_n) * C::BN, t0 = (int64_t)(tile / tiles_n) * 128 + 32 * warp;
-            const int rows = (int)max((int64_t)0, min((int64_t)32, L.a.rows - t0)), columns = (int)min((int64_t)C::BN, L.b.rows - n0);
+        for (int tile = pair; tile < tiles; tile += pairs, count++) {
+            const int64_t n0 = (int64_t)(tile % tiles_n) * BN, t0 = (int64_t)(tile / tiles_n) * 256 + 128 * rank + 32 * quarter;
+            const int rows = (int)max((int64_t)0, min((int64_t)32, L.a.rows - t0)), columns = (int)min((int64_t)BN, L.b.rows - n0);
             uint8_t *out = (uint8_t *)L.out + t0 * ld_bytes + n0 * (int64_t)sizeof(T);
-            if (!s_failed && !mbar_wait(smem_u32(&s_done), count & 1, 20)) s_failed = 1;
+            if (!s_failed && !mbar_wait(smem_u32(&s_done[count & 1]), count >> 1 & 1, 20)) s_failed = 1;
             tc_after_sync();
-            const uint32_t mine = tmem + (count & 1) * C::SECOND + ((uint32_t)(32 * warp) << 16);
-            for (int k = 0; k < CHUNKS; k++) {
-                const int c = ((count & 1 ? 0 : CHUNKS - FIRST) + k) % CHUNKS * CHUNK;
+            const uint32_t mine = tmem + (count & 1) * C::SECOND + ((uint32_t)(32 * quarter) << 16);
+            // both sets begin with half of the overlap: columns 128 on of even tiles, the first 128 of odd ones
+            for (int k = 0; k < 2 * PARTS; k++) {
+                const int c = 64 * set + ((k < PARTS) == ((count & 1) == 0) ? 128 : 0) + k % PARTS * CHUNK;
                 const bool some = c < columns && rows > 0;
                 float v[CHUNK];
                 if (some) {
@@ -503,18 +613,18 @@ __global__ void __launch_bounds__(MX_WIDE_THREADS, 1) k_mx_product_wide(const __
                     for (int j = 0; j < CHUNK; j += 16) tc_ld16(mine + c + j, (uint32_t *)v + j);
                     tc_wait_ld();
                 }
-                if (k == FIRST - 1) {   // the overlap is read
+                if (k == PARTS - 1) {   // read, and all of the tile before
                     tc_before_sync();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_u32(&s_free));
+                    if (lane == 0) mbar_arrive_first(smem_u32(&s_free[count & 1]));
                 }
                 if (!some) continue;
                 if (DROP) {
-                    const uint64_t pair = (uint64_t)((t0 + lane) * wide + n0 + c) / 2;
-                    const mx_key q = mx_key_at(key, pair);   // (a chunk's pairs have the same high bits: they are aligned)
+                    const uint64_t pos = (uint64_t)((t0 + lane) * wide + n0 + c) / 2;
+                    const mx_key q = mx_key_at(key, pos);   // (a chunk's pairs have the same high bits: they are aligned)
 #pragma unroll
                     for (int j = 0; j < CHUNK; j += 2) {
-                        const uint32_t w = mx_word(q, (uint32_t)pair + j / 2);
+                        const uint32_t w = mx_word(q, (uint32_t)pos + j / 2);
                         v[j] = (w & 0xFFFFu) < L.drop.threshold ? 0.0f : v[j] * L.drop.factor;
                         v[j + 1] = (w >> 16) < L.drop.threshold ? 0.0f : v[j + 1] * L.drop.factor;
                     }
@@ -523,15 +633,43 @@ __global__ void __launch_bounds__(MX_WIDE_THREADS, 1) k_mx_product_wide(const __
 #pragma unroll
                 for (int j = 0; j < CHUNK; j += E) st_shared16(buf + lane * C::PITCH + j * sizeof(T), pack16(v + j, T()));
                 __syncwarp();
-                if (!s_failed)
-                    rows_out<T>(buf, out + c * (int64_t)sizeof(T), ld_bytes, rows, min(CHUNK, columns - c) * (int)sizeof(T), lane, even);
+                if (!s_failed) rows_out<T>(buf, out + c * (int64_t)sizeof(T), ld_bytes, rows, min(CHUNK, columns - c), lane, even);
             }
         }
     }
     tc_before_sync();
     __syncthreads();
     if (threadIdx.x == 0 && s_failed) atomicExch(&g_mx_error, 1u);
-    if (warp == 5) tmem_free<512>(tmem);
+    cluster_sync();   // nothing of the pair is in use any more
+    tc_after_sync();
+    if (warp == ISSUE) tmem_free_pair(tmem);
+    __syncwarp();
+    cluster_sync();
+}
+
+typedef CUresult (*mx_encode_fn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                 const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// `words` 32-bit words a row, `box` rows a copy.
+static bool map_rows(mx_encode_fn encode, CUtensorMap *map, const uint8_t *base, int64_t rows, int words, int box) {
+    const cuuint64_t size[2] = {(cuuint64_t)words, (cuuint64_t)rows}, stride[1] = {(cuuint64_t)words * 4};
+    const cuuint32_t part[2] = {(cuuint32_t)words, (cuuint32_t)box}, step[2] = {1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, (void *)base, size, stride, part, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+static mx_encode_fn encoder() {
+    static mx_encode_fn fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) {
+            (void)cudaGetLastError();
+            return (mx_encode_fn) nullptr;
+        }
+        return (mx_encode_fn)p;
+    }();
+    return fn;
 }
 
 template <typename T, bool DROP>
@@ -540,9 +678,18 @@ static int product_wide(const mx_product_launch &L, int sms, cudaStream_t s) {
     auto kern = k_mx_product_wide<T, DROP>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
     if (e != cudaSuccess) return e;
-    const int64_t tiles_n = (L.b.rows + C::BN - 1) / C::BN, tiles = tiles_n * ((L.a.rows + 127) / 128);
+    const int64_t tiles_n = (L.b.rows + C::BN - 1) / C::BN, tiles = tiles_n * ((L.a.rows + 255) / 256);
     if (tiles > 0x3FFFFFFF) return cudaErrorInvalidValue;
-    kern<<<(unsigned)(tiles < sms ? tiles : sms), MX_WIDE_THREADS, C::SMEM, s>>>(L, (int)tiles_n, (int)tiles);
+    const int pairs = (int)(tiles < sms / 2 ? tiles : sms / 2);
+    const int64_t panels = (L.a.cols + MX_PANEL - 1) / MX_PANEL;
+    const mx_encode_fn encode = encoder();
+    mx_maps M;
+    if (!encode || !map_rows(encode, &M.a_codes, L.a.codes, panels * ((L.a.rows + 7) / 8 * 8), 32, 128) ||
+        !map_rows(encode, &M.b_codes, L.b.codes, panels * ((L.b.rows + 7) / 8 * 8), 32, C::BN / 2) ||
+        !map_rows(encode, &M.a_scales, L.a.scales, panels * ((L.a.rows + 127) / 128), 256, 1) ||
+        !map_rows(encode, &M.b_scales, L.b.scales, panels * ((L.b.rows + 127) / 128), 256, 2))
+        return cudaErrorNotSupported;
+    kern<<<(unsigned)(2 * pairs), C::THREADS, C::SMEM, s>>>(L, M, (int)tiles_n, (int)tiles);
     return cudaGetLastError();
 }
 
@@ -580,7 +727,7 @@ static int product_for(const mx_product_launch &L, int sms, cudaStream_t s) {
     if (t <= 32) return product_as<T, 32, DROP>(L, sms, s);
     if (t <= 64) return product_as<T, 64, DROP>(L, sms, s);
     if (t <= 128) return product_as<T, 128, DROP>(L, sms, s);
-    const int64_t tiles = (L.b.rows + 255) / 256 * ((t + 127) / 128);
+    const int64_t tiles = (L.b.rows + 255) / 256 * ((t + 255) / 256) * 2;
     // fewer tiles than SMs: their panels are shared out
     if (tiles * 2 <= sms || L.a.cols == 0 || L.b.rows <= 128) return product_as<T, 256, DROP>(L, sms, s);
     return product_wide<T, DROP>(L, sms, s);

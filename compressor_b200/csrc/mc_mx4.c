@@ -122,6 +122,7 @@ static int drop_of(mx_call *c, mx_drop *out, const falcom_dropout_args *d) {
 }
 
 #define ROUNDING 0x9E3779B9u
+static const mx_powers g_powers = MX_POWERS;
 
 MC_EXPORT int falcom_mx4_encode(const void *x, int dtype, size_t n, float *base, const falcom_random *random,
                                 void *codes, void *scales, void *stream) {
@@ -143,6 +144,7 @@ MC_EXPORT int falcom_mx4_encode(const void *x, int dtype, size_t n, float *base,
     L.x = x;
     L.n = (int64_t)n;
     L.base = base;
+    L.powers = g_powers;
     L.codes = (uint8_t *)codes;
     L.scales = (uint8_t *)scales;
     return done(&c, prev, mc_launch_mx_encode(&L, dtype, sms, stream));
@@ -225,6 +227,7 @@ MC_EXPORT int falcom_mx4_quantize(const void *x, int dtype, size_t rows, size_t 
     L.rows = (int64_t)rows;
     L.cols = (int64_t)cols;
     L.ld = (int64_t)ld;
+    L.powers = g_powers;
     L.vectors = ((uintptr_t)x & 15) == 0 && (rows == 1 || ld * g_type_size[dtype] % 16 == 0);
     return done(&c, prev, mc_launch_mx_quantize(&L, dtype, stream));
 }
@@ -270,6 +273,7 @@ MC_EXPORT int falcom_mx4_product(const falcom_mx4_matrix *a, const falcom_mx4_ma
     if (rc) return rc;
     L.out = out;
     L.ld = (int64_t)ld;
+    L.powers = g_powers;
     return done(&c, prev, mc_launch_mx_product(&L, dtype, sms, stream));
 }
 
@@ -303,6 +307,7 @@ MC_EXPORT int falcom_dropout(const void *x, const void *residual, void *y, int d
     L.y = y;
     L.rows = (int64_t)rows;
     L.cols = (int64_t)cols;
+    L.powers = g_powers;
     L.vectors = (((uintptr_t)x | (uintptr_t)y | (uintptr_t)residual) & 15) == 0 && cols % 8 == 0;
     return done(&c, prev, mc_launch_mx_dropout(&L, dtype, sms, stream));
 }

@@ -45,7 +45,6 @@ __global__ void __launch_bounds__(MX_TPB) k_mx_encode(const __grid_constant__ mx
             if (in) raw[b] = x[e0 + 32 * b];
             if (BASE && in) held[b] = L.base[e0 + 32 * b];
         }
-        const mx_key k = RANDOM ? mx_key_at(key, (uint64_t)(c * 128)) : key;
         uint32_t codes = 0, scales[2] = {0, 0};
 #pragma unroll
         for (int b = 0; b < 8; b++) {
@@ -55,8 +54,8 @@ __global__ void __launch_bounds__(MX_TPB) k_mx_encode(const __grid_constant__ mx
             const float y = v[b] * mx_inverse(s);
             uint32_t code;
             if (RANDOM) {
-                const uint32_t w = mx_word(k, (uint32_t)(c * 128 + 16 * b + (lane >> 1)));
-                code = mx_code_random(y, lane & 1 ? w >> 16 : w & 0xFFFFu);
+                const mx_bits w = mx_bits_at(key, L.powers, (uint64_t)(c * 128 + 16 * b + (lane >> 1)));
+                code = mx_code_random(__fmul_rz(fabsf(y), MX_CUT), lane & 1 ? w.high : w.low, L.powers) | (__float_as_uint(y) >> 31 << 3);
             } else {
                 code = mx_code_near(y);
             }
@@ -130,11 +129,126 @@ __device__ __forceinline__ mx_vec8<T> load8(const T *p) {
     return v;
 }
 
+// 8 elements from any address: the aligned 16-byte pieces that they lie in,
+// and one more, which may lie outside of them by up to 16 bytes at either end.
+template <typename T>
+struct mx_pieces {
+    uint32_t w[2 * sizeof(T) + 4];
+};
+template <typename T>
+__device__ __forceinline__ mx_pieces<T> load_pieces(const T *p) {
+    mx_pieces<T> v;
+    const uint4 *q = (const uint4 *)((uintptr_t)p & ~(uintptr_t)15);
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(v) / 16); i++) ((uint4 *)&v)[i] = __ldg(q + i);
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ mx_vec8<T> from_pieces(mx_pieces<T> v, const T *p) {
+    constexpr int N = 2 * sizeof(T);
+    const uint32_t off = (uint32_t)(uintptr_t)p;
+    const bool two = off & 8, one = off & 4;
+#pragma unroll
+    for (int i = 0; i < N + 2; i++) v.w[i] = two ? v.w[i + 2] : v.w[i];
+#pragma unroll
+    for (int i = 0; i < N + 1; i++) v.w[i] = one ? v.w[i + 1] : v.w[i];
+    if (sizeof(T) == 2) {
+        const uint32_t pick = off & 2 ? 0x5432u : 0x3210u;
+#pragma unroll
+        for (int i = 0; i < N; i++) v.w[i] = __byte_perm(v.w[i], v.w[i + 1], pick);
+    }
+    mx_vec8<T> r;
+    memcpy(&r, v.w, sizeof(r));
+    return r;
+}
+
+// What rounding needs of elements: their magnitudes' bits, compared as whole
+// numbers (two at a time where they have 16 bits), and float32 values.
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b, float) { return max(a, b & 0x7FFFFFFFu); }
+template <typename T>
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b, T) { return __vmaxu2(a, b & 0x7FFF7FFFu); }
+// The float32 bits of the largest, by the two halves of a 32-bit word for 16-bit types.
+__device__ __forceinline__ uint32_t top_low(uint32_t m, __nv_bfloat16) { return m << 16; }
+__device__ __forceinline__ uint32_t top_low(uint32_t m, __half) { return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m))); }
+template <typename T>
+__device__ __forceinline__ uint32_t top_of(uint32_t m, T t) { return max(top_low(m & 0xFFFFu, t), top_low(m >> 16, t)); }
+__device__ __forceinline__ uint32_t top_of(uint32_t m, float) { return m; }
+// Float32 values of the two 16-bit elements of a word.
+__device__ __forceinline__ float2 two_of(uint32_t w, __nv_bfloat16) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)); }
+__device__ __forceinline__ float2 two_of(uint32_t w, __half) {
+    __half2 h;
+    memcpy(&h, &w, 4);
+    return __half22float2(h);
+}
+// Bit 7 of byte B of 8 words to bit 3 of the 8 nibbles of one, and of byte 3.
+template <int B>
+__device__ __forceinline__ uint32_t signs8(const uint32_t *w) {
+    constexpr uint32_t PICK = (uint32_t)(B | (B + 4) << 4);
+    const uint32_t e = __byte_perm(__byte_perm(w[0], w[2], PICK), __byte_perm(w[4], w[6], PICK), 0x5410);
+    const uint32_t o = __byte_perm(__byte_perm(w[1], w[3], PICK), __byte_perm(w[5], w[7], PICK), 0x5410);
+    return ((e >> 4) & 0x08080808u) | (o & 0x80808080u);
+}
+// The same of both halves of 4 words, in the order of the elements.
+__device__ __forceinline__ uint32_t signs4x2(const uint32_t *w) {
+    const uint32_t x = __byte_perm(w[0], w[1], 0x7351), y = __byte_perm(w[2], w[3], 0x7351);
+    return ((__byte_perm(x, y, 0x5410) >> 4) & 0x08080808u) | (__byte_perm(x, y, 0x7632) & 0x80808080u);
+}
+
+// The codes of 8 elements.  y: values (at random: magnitudes) times 1 / scale, two by two.
+template <bool RANDOM>
+__device__ __forceinline__ uint32_t codes8(const float2 *y, uint32_t signs, const uint32_t *bits16, const mx_powers &P) {
+    if (RANDOM) return mx_codes8_random(y, bits16, P) | signs;
+    return mx_codes8((const float *)y);
+}
+
+// The values of two words' elements, or of their magnitudes.
+template <typename T, bool RANDOM>
+__device__ __forceinline__ float2 two_values(const uint32_t *w, int i) {
+    if constexpr (sizeof(T) == 4) {
+        const uint32_t m = RANDOM ? 0x7FFFFFFFu : 0xFFFFFFFFu;
+        return make_float2(__uint_as_float(w[2 * i] & m), __uint_as_float(w[2 * i + 1] & m));
+    } else {
+        return two_of(RANDOM ? w[i] & 0x7FFF7FFFu : w[i], T());
+    }
+}
+
+// A row's 8 elements (raw words) to codes.
+template <typename T, bool RANDOM, bool DROP>
+__device__ __forceinline__ uint32_t row_codes(const uint32_t *w, float inv, float factor, const mx_bits *bits, const mx_powers &P) {
+    float2 y[4];
+    uint32_t bits16[8], signs = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        y[i] = two_values<T, RANDOM>(w, i);
+        if (DROP) y[i] = mx_mul2(y[i], make_float2(factor, factor));
+        y[i] = mx_mul2(y[i], make_float2(inv, inv));
+        if (RANDOM) {
+            bits16[2 * i] = bits[i].low;
+            bits16[2 * i + 1] = bits[i].high;
+        }
+    }
+    if (RANDOM) {
+        if constexpr (sizeof(T) == 4) signs = signs8<3>(w);
+        else signs = signs4x2(w);
+    }
+    return codes8<RANDOM>(y, signs, bits16, P);
+}
+
+// Shared memory of a tile: its elements, and its random words (of which a
+// column's rounding has the same as a row's).
+template <typename T, bool COLS, bool RANDOM>
+struct mx_tile {
+    static constexpr int ELEMENTS = COLS ? MX_TILE * MX_TILE * (int)sizeof(T) : 0;
+    static constexpr int BYTES = ELEMENTS + (COLS && RANDOM ? MX_TILE * MX_TILE * 2 : 0);
+};
+
 template <typename T, bool ROWS, bool COLS, bool RANDOM, bool DROP>
-__global__ void __launch_bounds__(MX_TPB) k_mx_quantize(const __grid_constant__ mx_quantize_launch L) {
+__global__ void __launch_bounds__(MX_TPB, COLS ? 3 : 4) k_mx_quantize(const __grid_constant__ mx_quantize_launch L) {
+    typedef mx_tile<T, COLS, RANDOM> S;
+    constexpr int W = 8 * sizeof(T) / 4;   // words of 8 elements
     extern __shared__ __align__(16) uint8_t s_tile[];
     __shared__ __align__(16) uint8_t s_rows[512], s_cols[512];
-    T *tile = (T *)s_tile;
+    uint32_t *s_words = (uint32_t *)(s_tile + S::ELEMENTS);
     const int tid = threadIdx.x;
     const uint32_t band = blockIdx.x / L.tiles;
     const int64_t r0 = (int64_t)band * MX_TILE, c0 = (int64_t)(blockIdx.x - band * L.tiles) * MX_TILE;
@@ -144,119 +258,178 @@ __global__ void __launch_bounds__(MX_TPB) k_mx_quantize(const __grid_constant__ 
     if (DROP) drop = mx_key_of(L.drop.random);
     const int tx = tid & 15, ty = tid >> 4;
     const int64_t c = c0 + 8 * tx;
-#pragma unroll 2
-    for (int i = 0; i < MX_TILE / 16; i++) {
+    const T *row = (const T *)L.x + (r0 + ty) * L.ld;
+    uint8_t *to = ROWS ? L.along_rows.codes + mx_code_at(L.rows, r0 + ty, c / MX_BLOCK) + (tx & 3) * 4 : NULL;
+    uint64_t pair = (uint64_t)((r0 + ty) * wide + c) / 2;
+    const int left = (int)min((int64_t)MX_TILE, L.rows - r0), left8 = (left + 7) & ~7;   // (below 0: a tile of padding)
+
+    // One row's 8 elements; `i` counts 16 rows.
+    auto one = [&](mx_vec8<T> v, int i, bool inside) {
         const int y = ty + 16 * i;
-        const int64_t r = r0 + y;
-        mx_vec8<T> v;
-        memset(&v, 0, sizeof(v));
-        if (r < L.rows && c < L.cols) {
-            const T *p = (const T *)L.x + r * L.ld + c;
-            if (L.vectors && c + 8 <= L.cols) {
-                v = load8(p);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; j++)
-                    if (c + j < L.cols) v.x[j] = p[j];
-            }
-        }
-        const uint64_t pair = (uint64_t)(r * wide + c) / 2;
+        uint32_t w[W];
+        mx_bits bits[4];
         if (DROP) {
-            const mx_key k = mx_key_at(drop, pair);
+            const uint32_t start = mx_start(drop, pair);
 #pragma unroll
             for (int j = 0; j < 8; j += 2) {
-                const uint32_t w = mx_word(k, (uint32_t)pair + j / 2);
-                if ((w & 0xFFFFu) < L.drop.threshold) memset(&v.x[j], 0, sizeof(T));
-                if ((w >> 16) < L.drop.threshold) memset(&v.x[j + 1], 0, sizeof(T));
+                const mx_bits u = mx_bits_of(drop, L.powers, start ^ (j / 2));
+                if (u.low < L.drop.threshold) memset(&v.x[j], 0, sizeof(T));
+                if (u.high < L.drop.threshold) memset(&v.x[j + 1], 0, sizeof(T));
             }
+        }
+        memcpy(w, &v, sizeof(v));
+        if (RANDOM) {
+            const uint32_t start = mx_start(key, pair);
+#pragma unroll
+            for (int j = 0; j < 4; j++) bits[j] = mx_bits_of(key, L.powers, start ^ j);
         }
         if (COLS) {
-            T *q = tile + y * MX_TILE + 8 * tx;
+            uint4 *q = (uint4 *)(s_tile + (y * MX_TILE + 8 * tx) * sizeof(T));
 #pragma unroll
-            for (int j = 0; j < (int)(sizeof(v) / 16); j++) ((uint4 *)q)[j] = ((const uint4 *)&v)[j];
+            for (int j = 0; j < W / 4; j++) q[j] = *(const uint4 *)(w + 4 * j);
+            if (RANDOM) {
+                uint32_t u[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) u[j] = bits[j].high * L.powers.p16 + bits[j].low;
+                *(uint4 *)(s_words + y * (MX_TILE / 2) + 4 * tx) = *(const uint4 *)u;
+            }
         }
         if (ROWS) {
-            float f[8];
-            uint32_t top = 0;
+            uint32_t m = 0;
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                f[j] = mx_f32(v.x[j]);
-                if (DROP) f[j] *= L.drop.factor;
-                top = max(top, __float_as_uint(f[j]) & 0x7FFFFFFFu);
-            }
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const uint32_t s = mx_scale(top);
-            const float inv = mx_inverse(s);
-#pragma unroll
-            for (int j = 0; j < 8; j++) f[j] *= inv;
-            uint32_t codes = 0;
-            if (RANDOM) {
-                const mx_key k = mx_key_at(key, pair);
-#pragma unroll
-                for (int j = 0; j < 8; j += 2) {
-                    const uint32_t w = mx_word(k, (uint32_t)pair + j / 2);
-                    codes |= mx_code_random(f[j], w & 0xFFFFu) << (4 * j) | mx_code_random(f[j + 1], w >> 16) << (4 * j + 4);
-                }
+            for (int j = 0; j < W; j++) m = larger(m, w[j], T());
+            if constexpr (sizeof(T) == 4) {
+                m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
             } else {
-                codes = mx_codes8(f);
+                m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 2));
             }
+            uint32_t top = top_of(m, T());
+            // (the largest product is the largest element's)
+            if (DROP) top = __float_as_uint(__uint_as_float(top) * L.drop.factor);
+            const uint32_t s = mx_scale(top);
+            uint32_t codes = row_codes<T, RANDOM, DROP>(w, mx_inverse(s), L.drop.factor, bits, L.powers);
             if (s == 255u) codes = 0;
-            const int64_t k = c / MX_BLOCK;
-            if (r < mx_rows8(L.rows)) *(uint32_t *)(L.along_rows.codes + mx_code_at(L.rows, r, k) + (tx & 3) * 4) = codes;
+            if (inside) *(uint32_t *)(to + i * 16 * 128) = codes;   // (16 rows on the pieces of a row lie alike)
             if ((tx & 3) == 0) s_rows[(y & 31) * 16 + (y >> 5) * 4 + (tx >> 2)] = (uint8_t)s;
+        }
+        pair += 8 * wide;
+    };
+    // Whole tiles: loads a batch ahead of their use.
+    constexpr int BATCH = 8 / sizeof(T);
+    if (left == MX_TILE && L.vectors && c0 + MX_TILE <= L.cols) {
+        row += c;
+#pragma unroll 1
+        for (int i = 0; i < MX_TILE / 16; i += BATCH) {
+            mx_vec8<T> v[BATCH];
+#pragma unroll
+            for (int j = 0; j < BATCH; j++, row += 16 * L.ld) v[j] = load8(row);
+#pragma unroll
+            for (int j = 0; j < BATCH; j++) one(v[j], i + j, true);
+        }
+    } else if (left == MX_TILE && c0 > 0 && c0 + MX_TILE + 16 <= L.cols) {   // rows on any boundary, and room beside
+        row += c;
+#pragma unroll 1
+        for (int i = 0; i < MX_TILE / 16; i += BATCH) {
+            mx_pieces<T> v[BATCH];
+#pragma unroll
+            for (int j = 0; j < BATCH; j++) v[j] = load_pieces(row + 16 * j * L.ld);
+#pragma unroll
+            for (int j = 0; j < BATCH; j++, row += 16 * L.ld) one(from_pieces(v[j], row), i + j, true);
+        }
+    } else {
+#pragma unroll 1
+        for (int i = 0; i < MX_TILE / 16; i++, row += 16 * L.ld) {
+            mx_vec8<T> v;
+            memset(&v, 0, sizeof(v));
+            if (ty + 16 * i < left && c < L.cols) {
+                if (L.vectors && c + 8 <= L.cols) {
+                    v = load8(row + c);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        if (c + j < L.cols) v.x[j] = row[c + j];
+                }
+            }
+            one(v, i, ty + 16 * i < left8);
         }
     }
     __syncthreads();
     if (COLS) {
         const int p = tid & 63, b = tid >> 6;
-        const int64_t cc = c0 + 2 * p, rr = r0 + 32 * b;
-        T v[32][2];
-        const T *q = tile + 32 * b * MX_TILE + 2 * p;
+        const int64_t cc = c0 + 2 * p;
+        uint32_t s[2];
+        const uint32_t *q = (const uint32_t *)(s_tile + (32 * b * MX_TILE + 2 * p) * sizeof(T));
+        constexpr int PITCH = MX_TILE * sizeof(T) / 4;
+        if constexpr (sizeof(T) == 4) {
+            uint32_t m[2] = {0, 0};
 #pragma unroll
-        for (int i = 0; i < 32; i++) memcpy(v[i], q + i * MX_TILE, 2 * sizeof(T));
-        uint32_t top[2] = {0, 0};
-#pragma unroll
-        for (int i = 0; i < 32; i++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                float f = mx_f32(v[i][h]);
-                if (DROP) f *= L.drop.factor;
-                top[h] = max(top[h], __float_as_uint(f) & 0x7FFFFFFFu);
+            for (int i = 0; i < 32; i++) {
+                const uint2 w = *(const uint2 *)(q + i * PITCH);
+                m[0] = larger(m[0], w.x, T());
+                m[1] = larger(m[1], w.y, T());
             }
-        const uint32_t s[2] = {mx_scale(top[0]), mx_scale(top[1])};
-        const float inv[2] = {mx_inverse(s[0]), mx_inverse(s[1])};
+            s[0] = m[0];
+            s[1] = m[1];
+        } else {
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < 32; i++) m = larger(m, q[i * PITCH], T());
+            s[0] = top_low(m & 0xFFFFu, T());
+            s[1] = top_low(m >> 16, T());
+        }
+        float inv[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            if (DROP) s[h] = __float_as_uint(__uint_as_float(s[h]) * L.drop.factor);
+            s[h] = mx_scale(s[h]);
+            inv[h] = mx_inverse(s[h]);
+        }
         uint32_t codes[2][4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            float f[2][8];
+            float2 f[2][4];
+            uint32_t bits16[2][8], signs[2] = {0, 0}, w[2][8];
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    f[h][j] = mx_f32(v[8 * i + j][h]);
-                    if (DROP) f[h][j] *= L.drop.factor;
-                    f[h][j] *= inv[h];
+            for (int j = 0; j < 8; j++) {
+                float2 x;
+                if constexpr (sizeof(T) == 4) {
+                    const uint2 u = *(const uint2 *)(q + (8 * i + j) * PITCH);
+                    w[0][j] = u.x;
+                    w[1][j] = u.y;
+                    x = two_values<T, RANDOM>((const uint32_t *)&u, 0);
+                } else {
+                    w[0][j] = q[(8 * i + j) * PITCH];
+                    x = two_of(RANDOM ? w[0][j] & 0x7FFF7FFFu : w[0][j], T());
                 }
-            if (RANDOM) {
-                codes[0][i] = codes[1][i] = 0;
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const uint64_t pair = (uint64_t)((rr + 8 * i + j) * wide + cc) / 2;
-                    const uint32_t w = mx_word(mx_key_at(key, pair), (uint32_t)pair);
-                    codes[0][i] |= mx_code_random(f[0][j], w & 0xFFFFu) << (4 * j);
-                    codes[1][i] |= mx_code_random(f[1][j], w >> 16) << (4 * j);
+                if (DROP) x = mx_mul2(x, make_float2(L.drop.factor, L.drop.factor));
+                x = mx_mul2(x, make_float2(inv[0], inv[1]));
+                if (j & 1) f[0][j / 2].y = x.x, f[1][j / 2].y = x.y;
+                else f[0][j / 2].x = x.x, f[1][j / 2].x = x.y;
+                if (RANDOM) {
+                    const uint32_t u = s_words[(32 * b + 8 * i + j) * (MX_TILE / 2) + p];
+                    bits16[1][j] = __umulhi(u, L.powers.p16);
+                    bits16[0][j] = u & 0xFFFFu;
                 }
-            } else {
-                codes[0][i] = mx_codes8(f[0]);
-                codes[1][i] = mx_codes8(f[1]);
             }
+            if (RANDOM) {
+                if constexpr (sizeof(T) == 4) {
+                    signs[0] = signs8<3>(w[0]);
+                    signs[1] = signs8<3>(w[1]);
+                } else {
+                    signs[0] = signs8<1>(w[0]);
+                    signs[1] = signs8<3>(w[0]);
+                }
+            }
+            codes[0][i] = codes8<RANDOM>(f[0], signs[0], bits16[0], L.powers);
+            codes[1][i] = codes8<RANDOM>(f[1], signs[1], bits16[1], L.powers);
         }
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             if (s[h] == 255u) codes[h][0] = codes[h][1] = codes[h][2] = codes[h][3] = 0;
             if (cc + h < mx_rows8(L.cols))
-                *(uint4 *)(L.along_cols.codes + mx_code_at(L.cols, cc + h, rr / MX_BLOCK)) =
+                *(uint4 *)(L.along_cols.codes + mx_code_at(L.cols, cc + h, r0 / MX_BLOCK + b)) =
                     make_uint4(codes[h][0], codes[h][1], codes[h][2], codes[h][3]);
             const int y = 2 * p + h;
             s_cols[(y & 31) * 16 + (y >> 5) * 4 + b] = (uint8_t)s[h];
@@ -287,10 +460,10 @@ __global__ void __launch_bounds__(MX_TPB) k_mx_dequantize(const __grid_constant_
 // -------------------------------------------------------------- dropout
 template <typename T, bool RES>
 __device__ __forceinline__ void drop_pair(const mx_dropout_launch &L, mx_key key, uint64_t pair, const T *x, const T *res, T *y) {
-    const uint32_t w = mx_word(mx_key_at(key, pair), (uint32_t)pair);
+    const mx_bits w = mx_bits_at(key, L.powers, pair);
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-        float f = (h ? w >> 16 : w & 0xFFFFu) < L.drop.threshold ? 0.0f : mx_f32(x[h]) * L.drop.factor;
+        float f = (h ? w.high : w.low) < L.drop.threshold ? 0.0f : mx_f32(x[h]) * L.drop.factor;
         if (RES) f = f + mx_f32(res[h]);
         mx_from(&y[h], f);
     }
@@ -366,7 +539,7 @@ static int quantize_as(mx_quantize_launch L, cudaStream_t s) {
     const int64_t y = COLS ? (L.rows + 255) / 256 * 2 : (L.rows + 127) / 128;
     if (x * y > 0x7FFFFFFF) return cudaErrorInvalidValue;
     L.tiles = (uint32_t)x;
-    const size_t smem = COLS ? MX_TILE * MX_TILE * sizeof(T) : 0;
+    const size_t smem = mx_tile<T, COLS, RANDOM>::BYTES;
     if (smem > 48 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(k_mx_quantize<T, ROWS, COLS, RANDOM, DROP>,
                                                    cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);

@@ -29,31 +29,45 @@ __host__ __device__ __forceinline__ uint32_t mx_mix(uint32_t x) {
     return x ^ (x >> 16);
 }
 
-// The two key words of a purpose, seed and counter.  The second one enters
-// between the two products, so that two keys do not give the same words in
-// another order.
+// The key of a purpose, seed and counter: two words, each with its own shift
+// folded in, since (x ^ a) ^ ((x ^ a) >> n) = x ^ (x >> n) ^ (a ^ (a >> n)).
+// The second enters between the two products, so that two keys do not give
+// the same words in another order.
 struct mx_key {
-    uint32_t a, b;
+    uint32_t a, b;   // a ^ (a >> 16), b ^ (b >> 13)
 };
 __device__ __forceinline__ mx_key mx_key_of(const mx_random &r) {
     const uint64_t c = r.counter ? (uint64_t)*r.counter : 0;
+    const uint32_t a = mx_mix(mx_mix(r.key ^ (uint32_t)c) ^ (uint32_t)(c >> 32)), b = mx_mix(a ^ 0x85EBCA77u);
     mx_key k;
-    k.a = mx_mix(mx_mix(r.key ^ (uint32_t)c) ^ (uint32_t)(c >> 32));
-    k.b = mx_mix(k.a ^ 0x85EBCA77u);
+    k.a = a ^ (a >> 16);
+    k.b = b ^ (b >> 13);
     return k;
 }
-// The key for positions with these high bits.
-__device__ __forceinline__ mx_key mx_key_at(mx_key k, uint64_t pair) {
-    if (pair >> 32) k.a ^= mx_mix((uint32_t)(pair >> 32));
-    return k;
+// The start of the words of positions from `pair` on, a multiple of 4: word j
+// (0 to 3) is mx_word(key, start ^ j).
+__device__ __forceinline__ uint32_t mx_start(mx_key k, uint64_t pair) {
+    const uint32_t low = (uint32_t)pair, high = (uint32_t)(pair >> 32);
+    uint32_t s = low ^ (low >> 16) ^ k.a;
+    if (high) {
+        const uint32_t m = mx_mix(high);
+        s ^= m ^ (m >> 16);
+    }
+    return s;
 }
-// The word of a pair of elements: 16 bits for each, the even one's below.
-__device__ __forceinline__ uint32_t mx_word(mx_key k, uint32_t pair) {
-    uint32_t x = pair ^ k.a;
-    x = ((x ^ (x >> 16)) * 0x85EBCA6Bu) ^ k.b;
-    x = (x ^ (x >> 13)) * 0xC2B2AE35u;
-    return x ^ (x >> 16);
+// The 16 bits of each of a pair of elements.
+struct mx_bits {
+    uint32_t low, high;
+};
+__device__ __forceinline__ mx_bits mx_bits_of(mx_key k, const mx_powers &P, uint32_t start) {
+    uint32_t x = start * 0x85EBCA6Bu;
+    x = (x ^ __umulhi(x, P.p19) ^ k.b) * 0xC2B2AE35u;   // x >> 13
+    mx_bits r;
+    r.high = __umulhi(x, P.p16);                        // x >> 16
+    r.low = (x ^ r.high) & 0xFFFFu;
+    return r;
 }
+__device__ __forceinline__ mx_bits mx_bits_at(mx_key k, const mx_powers &P, uint64_t pair) { return mx_bits_of(k, P, mx_start(k, pair)); }
 __device__ __forceinline__ int64_t mx_wide(int64_t cols) { return (cols + MX_BLOCK - 1) / MX_BLOCK * MX_BLOCK; }
 
 // ---------------------------------------------------------- 4-bit rounding
@@ -91,14 +105,45 @@ __device__ __forceinline__ uint32_t mx_code_near(float y) {
     return r & 15u;
 }
 
-// One code, rounded up with the probability that its distance asks for.
-// Times 2^-126 the codes 0 to 7 are the float32 bits 22 and up (0.5 a
-// subnormal number): the bits below are the distance, and a carry from adding
-// the random bits to them rounds up.  Digits below 2^-149 are cut off, which
-// changes no carry: the random bits (16, and a half) end far above.
-__device__ __forceinline__ uint32_t mx_code_random(float y, uint32_t bits16) {
-    const uint32_t b = __float_as_uint(__fmul_rz(fabsf(y), 1.17549435e-38f));
-    return ((b + (bits16 << 6) + 32u) >> 22) | (__float_as_uint(y) >> 31 << 3);
+__device__ __forceinline__ float2 mx_mul2(float2 a, float2 b) {
+    float2 r;
+    asm("{.reg .b64 a, b, r;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 r, a, b;\n\t"
+        "mov.b64 {%0, %1}, r;}" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 mx_mul2_cut(float2 a, float2 b) {   // towards 0
+    float2 r;
+    asm("{.reg .b64 a, b, r;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rz.f32x2 r, a, b;\n\t"
+        "mov.b64 {%0, %1}, r;}" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+
+// Rounding at random.  Times 2^-126 the magnitudes 0, 0.5, 1, ... 6 have the
+// codes 0 to 7 in the float32's bits 22 and up (0.5 is a subnormal number); the
+// bits below are the distance from the value below, and where adding the
+// random bits to them carries, the code is rounded up.  Digits below 2^-149
+// are cut off, which changes no carry: the random bits (16, and a half) end
+// far above.
+#define MX_CUT 1.17549435e-38f
+// The magnitude code of y * 2^-126 with these 16 bits: its bits + 64 * bits16
+// + 32, shifted right by 22.
+__device__ __forceinline__ uint32_t mx_code_random(float cut, uint32_t bits16, const mx_powers &P) {
+    const uint32_t t = bits16 * P.p6 + __float_as_uint(cut);
+    return (uint32_t)(((uint64_t)t * P.p10 + (32u << 10)) >> 32);
+}
+// Magnitude codes of 8 elements: y their magnitudes times 1 / scale, two by
+// two, and the bits of each.
+__device__ __forceinline__ uint32_t mx_codes8_random(const float2 *y, const uint32_t *bits16, const mx_powers &P) {
+    uint32_t r[2];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const float2 a = mx_mul2_cut(y[2 * h], make_float2(MX_CUT, MX_CUT)), b = mx_mul2_cut(y[2 * h + 1], make_float2(MX_CUT, MX_CUT));
+        r[h] = mx_code_random(b.y, bits16[4 * h + 3], P);
+        r[h] = r[h] * P.p4 + mx_code_random(b.x, bits16[4 * h + 2], P);
+        r[h] = r[h] * P.p4 + mx_code_random(a.y, bits16[4 * h + 1], P);
+        r[h] = r[h] * P.p4 + mx_code_random(a.x, bits16[4 * h], P);
+    }
+    return r[1] * P.p16 + r[0];
 }
 
 // The value of the code in bits 0 to 3, without its scale.

@@ -145,9 +145,8 @@ struct mx_cfg {
 template <typename T, bool DROP>
 __device__ __forceinline__ void put(const mx_product_launch &L, mx_key key, int64_t wide, int64_t t, int64_t n, float v) {
     if (DROP) {
-        const uint64_t pair = (uint64_t)(t * wide + n) / 2;
-        const uint32_t w = mx_word(mx_key_at(key, pair), (uint32_t)pair);
-        v = ((n & 1) ? w >> 16 : w & 0xFFFFu) < L.drop.threshold ? 0.0f : v * L.drop.factor;
+        const mx_bits w = mx_bits_at(key, L.powers, (uint64_t)(t * wide + n) / 2);
+        v = ((n & 1) ? w.high : w.low) < L.drop.threshold ? 0.0f : v * L.drop.factor;
     }
     mx_from((T *)L.out + t * L.ld + n, v);
 }
@@ -621,12 +620,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mx_wide_cfg::THREADS
                 if (!some) continue;
                 if (DROP) {
                     const uint64_t pos = (uint64_t)((t0 + lane) * wide + n0 + c) / 2;
-                    const mx_key q = mx_key_at(key, pos);   // (a chunk's pairs have the same high bits: they are aligned)
+                    uint32_t start = 0;
 #pragma unroll
                     for (int j = 0; j < CHUNK; j += 2) {
-                        const uint32_t w = mx_word(q, (uint32_t)pos + j / 2);
-                        v[j] = (w & 0xFFFFu) < L.drop.threshold ? 0.0f : v[j] * L.drop.factor;
-                        v[j + 1] = (w >> 16) < L.drop.threshold ? 0.0f : v[j + 1] * L.drop.factor;
+                        if (j % 8 == 0) start = mx_start(key, pos + j / 2);
+                        const mx_bits w = mx_bits_of(key, L.powers, start ^ (j / 2 & 3));
+                        v[j] = w.low < L.drop.threshold ? 0.0f : v[j] * L.drop.factor;
+                        v[j + 1] = w.high < L.drop.threshold ? 0.0f : v[j + 1] * L.drop.factor;
                     }
                 }
                 __syncwarp();   // the last part has left the buffer

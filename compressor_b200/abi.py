@@ -616,15 +616,35 @@ class Mx4MatrixC(ctypes.Structure):
     ]
 
 
+class Mx4LinearC(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_size_t),
+        ("cols", ctypes.c_size_t),
+        ("outs", ctypes.c_size_t),
+        ("x_type", ctypes.c_int),
+        ("weight_type", ctypes.c_int),
+        ("want_dx", ctypes.c_int),
+        ("want_dw", ctypes.c_int),
+        ("p", ctypes.c_double),
+        ("random", RandomC),
+    ]
+
+
 def bind_mx4(lib: ctypes.CDLL) -> None:
     """4-bit entry points (falcom_mx4_*) and falcom_dropout; no instance needed."""
     P = ctypes.POINTER
     c_vp, size, c_int = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int
     lib.falcom_mx4_encode.argtypes = [c_vp, c_int, size, c_vp, P(RandomC), c_vp, c_vp, c_vp]
     lib.falcom_mx4_decode.argtypes = [c_vp, c_vp, size, ctypes.c_float, c_int, c_vp, c_int, c_vp]
-    for fn in (lib.falcom_mx4_codes_bytes, lib.falcom_mx4_scales_bytes):
+    for fn in (lib.falcom_mx4_codes_bytes, lib.falcom_mx4_scales_bytes, lib.falcom_mx4_work_bytes):
         fn.argtypes = [size, size]
         fn.restype = size
+    lib.falcom_mx4_linear_kept_bytes.argtypes = [P(Mx4LinearC)]
+    lib.falcom_mx4_linear_work_bytes.argtypes = [P(Mx4LinearC), c_int]
+    lib.falcom_mx4_linear_kept_bytes.restype = lib.falcom_mx4_linear_work_bytes.restype = size
+    lib.falcom_mx4_product_of.argtypes = [c_vp, c_int, size, size, P(Mx4MatrixC), c_vp, c_int, size, c_vp, c_vp]
+    lib.falcom_mx4_linear_forward.argtypes = [P(Mx4LinearC), c_vp, size, c_vp, size, c_vp, c_vp, c_vp, c_vp]
+    lib.falcom_mx4_linear_backward.argtypes = [P(Mx4LinearC), c_vp, size, c_vp, c_vp, c_vp, c_vp, c_vp]
     lib.falcom_mx4_quantize.argtypes = [c_vp, c_int, size, size, size, P(RandomC), P(DropoutArgsC), P(Mx4MatrixC),
                                         P(Mx4MatrixC), c_vp]
     lib.falcom_mx4_dequantize.argtypes = [P(Mx4MatrixC), c_vp, c_int, size, c_vp]
@@ -632,7 +652,8 @@ def bind_mx4(lib: ctypes.CDLL) -> None:
     lib.falcom_mx4_errors.argtypes = []
     lib.falcom_dropout.argtypes = [c_vp, c_vp, c_vp, c_int, size, size, P(DropoutArgsC), c_vp]
     for fn in (lib.falcom_mx4_encode, lib.falcom_mx4_decode, lib.falcom_mx4_quantize, lib.falcom_mx4_dequantize,
-               lib.falcom_mx4_product, lib.falcom_mx4_errors, lib.falcom_dropout):
+               lib.falcom_mx4_product, lib.falcom_mx4_product_of, lib.falcom_mx4_linear_forward,
+               lib.falcom_mx4_linear_backward, lib.falcom_mx4_errors, lib.falcom_dropout):
         fn.restype = c_int
 
 

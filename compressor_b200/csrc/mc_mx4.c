@@ -13,7 +13,8 @@
 #include "mc_mx4.h"
 
 static const size_t g_type_size[MX_TYPES] = {4, 2, 2};
-#define MX_MOST ((size_t)1 << 31)   /* rows or columns */
+#define MX_MOST ((size_t)1 << 31)       /* rows or columns */
+#define MX_ELEMENTS ((size_t)1 << 46)   /* of a matrix */
 
 static int invalid(const char *who, const char *what) {
     fprintf(stderr, "[ERROR] %s: %s\n", who, what);
@@ -53,7 +54,7 @@ static void array(mx_call *c, const char *what, const void *p, size_t bytes, siz
         c->device = at.device;
     }
     const uintptr_t lo = (uintptr_t)p, hi = lo + bytes;
-    if (!check_argument(c->who, what, p, bytes, align, c->device)) {
+    if (!p || !check_argument(c->who, what, p, bytes, align, c->device)) {
         c->ok = 0;
         return;
     }
@@ -122,7 +123,6 @@ static int drop_of(mx_call *c, mx_drop *out, const falcom_dropout_args *d) {
 }
 
 #define ROUNDING 0x9E3779B9u
-static const mx_powers g_powers = MX_POWERS;
 
 MC_EXPORT int falcom_mx4_encode(const void *x, int dtype, size_t n, float *base, const falcom_random *random,
                                 void *codes, void *scales, void *stream) {
@@ -144,9 +144,9 @@ MC_EXPORT int falcom_mx4_encode(const void *x, int dtype, size_t n, float *base,
     L.x = x;
     L.n = (int64_t)n;
     L.base = base;
-    L.powers = g_powers;
     L.codes = (uint8_t *)codes;
     L.scales = (uint8_t *)scales;
+    L.vectors = (((uintptr_t)x | (uintptr_t)base) & 15) == 0;
     return done(&c, prev, mc_launch_mx_encode(&L, dtype, sms, stream));
 }
 
@@ -171,6 +171,7 @@ MC_EXPORT int falcom_mx4_decode(const void *codes, const void *scales, size_t n,
     L.out = out;
     L.weight = weight;
     L.accumulate = accumulate != 0;
+    L.vectors = ((uintptr_t)out & 15) == 0;
     return done(&c, prev, mc_launch_mx_decode(&L, dtype, sms, stream));
 }
 
@@ -193,10 +194,40 @@ static void matrix_of(mx_call *c, mx_matrix *out, const falcom_mx4_matrix *m, co
     out->cols = (int64_t)m->cols;
 }
 
-/* Bytes from the first to the last element; 0 when the rows overlap. */
+/* Bytes from the first to the last element; 0 when the rows overlap or lie too far apart. */
 static size_t extent(size_t rows, size_t cols, size_t ld, size_t size) {
-    if (rows > 1 && (ld < cols || ld > (size_t)1 << 40)) return 0;
+    if (rows > 1 && (ld < cols || ld > MX_ELEMENTS / rows)) return 0;
     return ((rows - 1) * (rows > 1 ? ld : 0) + cols) * size;
+}
+
+static int quantize(const void *x, int dtype, size_t rows, size_t cols, size_t ld, const mx_random *random,
+                    const mx_drop *drop, const mx_matrix *along_rows, const mx_matrix *along_cols, void *stream) {
+    mx_quantize_launch L;
+    memset(&L, 0, sizeof(L));
+    if (rows == 0 || cols == 0 || (!along_rows && !along_cols)) return 0;
+    L.x = x;
+    L.rows = (int64_t)rows;
+    L.cols = (int64_t)cols;
+    L.ld = (int64_t)ld;
+    if (random) L.random = *random;
+    if (drop) L.drop = *drop;
+    if (along_rows) L.along_rows = *along_rows;
+    if (along_cols) L.along_cols = *along_cols;
+    L.vectors = ((uintptr_t)x & 15) == 0 && (rows == 1 || ld * g_type_size[dtype] % 16 == 0);
+    return mc_launch_mx_quantize(&L, dtype, stream);
+}
+
+static int product(const mx_matrix *a, const mx_matrix *b, void *out, int dtype, size_t ld, const mx_drop *drop, int sms,
+                   void *stream) {
+    mx_product_launch L;
+    memset(&L, 0, sizeof(L));
+    if (a->rows == 0 || b->rows == 0) return 0;
+    L.a = *a;
+    L.b = *b;
+    L.out = out;
+    L.ld = (int64_t)ld;
+    if (drop) L.drop = *drop;
+    return mc_launch_mx_product(&L, dtype, sms, stream);
 }
 
 MC_EXPORT int falcom_mx4_quantize(const void *x, int dtype, size_t rows, size_t cols, size_t ld,
@@ -209,27 +240,23 @@ MC_EXPORT int falcom_mx4_quantize(const void *x, int dtype, size_t rows, size_t 
     if ((along_rows && (along_rows->rows != rows || along_rows->cols != cols)) ||
         (along_cols && (along_cols->rows != cols || along_cols->cols != rows)))
         return invalid(who, "a result has other sizes than x");
+    mx_random r = {0};
+    mx_drop d = {{0}, 0, 0};
+    mx_matrix by_rows, by_cols;
+    mx_call c;
+    begin(&c, who);
+    if (!drop_of(&c, &d, drop)) return invalid(who, "p must lie in [0, 1)");
     if (rows == 0 || cols == 0 || (!along_rows && !along_cols)) return ERROR_NONE;
     const size_t bytes = extent(rows, cols, ld, g_type_size[dtype]);
-    if (bytes == 0) return invalid(who, "rows of x overlap");
-    mx_call c;
-    mx_quantize_launch L;
-    memset(&L, 0, sizeof(L));
-    begin(&c, who);
+    if (bytes == 0) return invalid(who, "rows of x overlap, or lie too far apart");
     array(&c, "x", x, bytes, g_type_size[dtype], 0);
-    if (along_rows) matrix_of(&c, &L.along_rows, along_rows, "along_rows", 1);
-    if (along_cols) matrix_of(&c, &L.along_cols, along_cols, "along_cols", 1);
-    random_of(&c, &L.random, random, ROUNDING);
-    if (!drop_of(&c, &L.drop, drop)) return invalid(who, "p must lie in [0, 1)");
+    if (along_rows) matrix_of(&c, &by_rows, along_rows, "along_rows", 1);
+    if (along_cols) matrix_of(&c, &by_cols, along_cols, "along_cols", 1);
+    random_of(&c, &r, random, ROUNDING);
     int prev, sms, rc = go(&c, &prev, &sms);
     if (rc) return rc;
-    L.x = x;
-    L.rows = (int64_t)rows;
-    L.cols = (int64_t)cols;
-    L.ld = (int64_t)ld;
-    L.powers = g_powers;
-    L.vectors = ((uintptr_t)x & 15) == 0 && (rows == 1 || ld * g_type_size[dtype] % 16 == 0);
-    return done(&c, prev, mc_launch_mx_quantize(&L, dtype, stream));
+    return done(&c, prev, quantize(x, dtype, rows, cols, ld, &r, &d, along_rows ? &by_rows : NULL,
+                                   along_cols ? &by_cols : NULL, stream));
 }
 
 MC_EXPORT int falcom_mx4_dequantize(const falcom_mx4_matrix *m, void *out, int dtype, size_t ld, void *stream) {
@@ -238,7 +265,7 @@ MC_EXPORT int falcom_mx4_dequantize(const falcom_mx4_matrix *m, void *out, int d
     if (m->rows > MX_MOST || m->cols > MX_MOST) return invalid(who, "too many rows or columns");
     if (m->rows == 0 || m->cols == 0) return ERROR_NONE;
     const size_t bytes = extent(m->rows, m->cols, ld, g_type_size[dtype]);
-    if (bytes == 0) return invalid(who, "rows of out overlap");
+    if (bytes == 0) return invalid(who, "rows of out overlap, or lie too far apart");
     mx_call c;
     mx_dequantize_launch L;
     memset(&L, 0, sizeof(L));
@@ -258,23 +285,162 @@ MC_EXPORT int falcom_mx4_product(const falcom_mx4_matrix *a, const falcom_mx4_ma
     if (!a || !b || !known_type(dtype)) return invalid(who, "a factor is missing, or an unknown type");
     if (a->cols != b->cols) return invalid(who, "the factors have different numbers of columns");
     if (a->rows > MX_MOST || b->rows > MX_MOST || a->cols > MX_MOST) return invalid(who, "too many rows or columns");
+    mx_drop d = {{0}, 0, 0};
+    mx_matrix ma, mb;
+    mx_call c;
+    begin(&c, who);
+    if (!drop_of(&c, &d, drop)) return invalid(who, "p must lie in [0, 1)");
     if (a->rows == 0 || b->rows == 0) return ERROR_NONE;
     const size_t bytes = extent(a->rows, b->rows, ld, g_type_size[dtype]);
-    if (bytes == 0) return invalid(who, "rows of out overlap");
-    mx_call c;
-    mx_product_launch L;
-    memset(&L, 0, sizeof(L));
-    begin(&c, who);
+    if (bytes == 0) return invalid(who, "rows of out overlap, or lie too far apart");
     array(&c, "out", out, bytes, g_type_size[dtype], 1);
-    matrix_of(&c, &L.a, a, "a", 0);
-    matrix_of(&c, &L.b, b, "b", 0);
-    if (!drop_of(&c, &L.drop, drop)) return invalid(who, "p must lie in [0, 1)");
+    matrix_of(&c, &ma, a, "a", 0);
+    matrix_of(&c, &mb, b, "b", 0);
     int prev, sms, rc = go(&c, &prev, &sms);
     if (rc) return rc;
-    L.out = out;
-    L.ld = (int64_t)ld;
-    L.powers = g_powers;
-    return done(&c, prev, mc_launch_mx_product(&L, dtype, sms, stream));
+    return done(&c, prev, product(&ma, &mb, out, dtype, ld, &d, sms, stream));
+}
+
+/* A matrix at *at, which moves behind it. */
+static size_t matrix_bytes(size_t rows, size_t cols) {
+    return falcom_mx4_codes_bytes(rows, cols) + falcom_mx4_scales_bytes(rows, cols);
+}
+
+static mx_matrix matrix_in(uint8_t **at, size_t rows, size_t cols) {
+    mx_matrix m;
+    m.codes = *at;
+    m.scales = *at + falcom_mx4_codes_bytes(rows, cols);
+    m.rows = (int64_t)rows;
+    m.cols = (int64_t)cols;
+    *at += matrix_bytes(rows, cols);
+    return m;
+}
+
+MC_EXPORT size_t falcom_mx4_work_bytes(size_t rows, size_t cols) { return matrix_bytes(rows, cols); }
+
+MC_EXPORT int falcom_mx4_product_of(const void *x, int x_type, size_t rows, size_t ld_x, const falcom_mx4_matrix *b,
+                                    void *out, int dtype, size_t ld, void *work, void *stream) {
+    static const char *who = "falcom_mx4_product_of";
+    if (!b || !known_type(dtype) || !known_type(x_type)) return invalid(who, "a factor is missing, or an unknown type");
+    if (rows > MX_MOST || b->rows > MX_MOST || b->cols > MX_MOST) return invalid(who, "too many rows or columns");
+    if (rows == 0 || b->rows == 0) return ERROR_NONE;
+    const size_t from = b->cols ? extent(rows, b->cols, ld_x, g_type_size[x_type]) : 0;
+    const size_t bytes = extent(rows, b->rows, ld, g_type_size[dtype]);
+    if (bytes == 0 || (from == 0 && b->cols)) return invalid(who, "rows of x or of out overlap, or lie too far apart");
+    mx_matrix mb;
+    mx_call c;
+    begin(&c, who);
+    array(&c, "out", out, bytes, g_type_size[dtype], 1);
+    array(&c, "x", x, from, g_type_size[x_type], 0);
+    array(&c, "work", work, matrix_bytes(rows, b->cols), 16, 1);
+    matrix_of(&c, &mb, b, "b", 0);
+    int prev, sms, rc = go(&c, &prev, &sms);
+    if (rc) return rc;
+    uint8_t *at = (uint8_t *)work;
+    const mx_matrix a = matrix_in(&at, rows, b->cols);
+    int e = quantize(x, x_type, rows, b->cols, ld_x, NULL, NULL, &a, NULL, stream);
+    if (e == 0) e = product(&a, &mb, out, dtype, ld, NULL, sms, stream);
+    return done(&c, prev, e);
+}
+
+/* ------------------------------------------------------------------ layers */
+static int layer_ok(const char *who, const falcom_mx4_linear *l) {
+    if (!l || !known_type(l->x_type) || !known_type(l->weight_type))
+        return invalid(who, "no layer, or an unknown type"), 0;
+    if (l->rows > MX_MOST || l->cols > MX_MOST || l->outs > MX_MOST)
+        return invalid(who, "too many rows, columns or outputs"), 0;
+    return 1;
+}
+
+MC_EXPORT size_t falcom_mx4_linear_kept_bytes(const falcom_mx4_linear *l) {
+    if (!l) return 0;
+    return (l->want_dx ? matrix_bytes(l->cols, l->outs) : 0) + (l->want_dw ? matrix_bytes(l->cols, l->rows) : 0);
+}
+
+MC_EXPORT size_t falcom_mx4_linear_work_bytes(const falcom_mx4_linear *l, int backward) {
+    if (!l) return 0;
+    if (backward) return (l->want_dx ? matrix_bytes(l->rows, l->outs) : 0) + (l->want_dw ? matrix_bytes(l->outs, l->rows) : 0);
+    return matrix_bytes(l->rows, l->cols) + matrix_bytes(l->outs, l->cols);
+}
+
+static int layer_drop(mx_call *c, mx_drop *out, const falcom_mx4_linear *l) {
+    falcom_dropout_args d;
+    d.p = l->p;
+    d.random = l->random;
+    if (l->p == 0.0) d.random.counter = NULL;   /* nothing reads it */
+    return drop_of(c, out, &d);
+}
+
+MC_EXPORT int falcom_mx4_linear_forward(const falcom_mx4_linear *l, const void *x, size_t ld_x, const void *weight,
+                                        size_t ld_weight, void *y, void *kept, void *work, void *stream) {
+    static const char *who = "falcom_mx4_linear_forward";
+    if (!layer_ok(who, l)) return ERROR_INVALID_PARAM;
+    const size_t xs = g_type_size[l->x_type], ws = g_type_size[l->weight_type];
+    const int no_x = l->rows == 0 || l->cols == 0, no_w = l->outs == 0 || l->cols == 0;
+    const size_t x_bytes = no_x ? 0 : extent(l->rows, l->cols, ld_x, xs), w_bytes = no_w ? 0 : extent(l->outs, l->cols, ld_weight, ws);
+    if ((!no_x && x_bytes == 0) || (!no_w && w_bytes == 0) || l->rows * l->outs > MX_ELEMENTS)
+        return invalid(who, "rows of x or of the weight overlap, or sizes are out of range");
+    mx_drop d = {{0}, 0, 0};
+    mx_call c;
+    begin(&c, who);
+    if (!layer_drop(&c, &d, l)) return invalid(who, "p must lie in [0, 1)");
+    array(&c, "y", y, l->rows * l->outs * xs, xs, 1);
+    array(&c, "x", x, x_bytes, xs, 0);
+    array(&c, "weight", weight, w_bytes, ws, 0);
+    array(&c, "kept", kept, falcom_mx4_linear_kept_bytes(l), 16, 1);
+    array(&c, "work", work, falcom_mx4_linear_work_bytes(l, 0), 16, 1);
+    if (c.ok && c.n == 0) return ERROR_NONE;   /* nothing at all */
+    int prev, sms, rc = go(&c, &prev, &sms);
+    if (rc) return rc;
+    uint8_t *at = (uint8_t *)work, *keep = (uint8_t *)kept;
+    const mx_matrix a = matrix_in(&at, l->rows, l->cols), b = matrix_in(&at, l->outs, l->cols);
+    mx_matrix bt, atr;
+    if (l->want_dx) bt = matrix_in(&keep, l->cols, l->outs);
+    if (l->want_dw) atr = matrix_in(&keep, l->cols, l->rows);
+    int e = quantize(weight, l->weight_type, l->outs, l->cols, ld_weight, NULL, NULL, &b, l->want_dx ? &bt : NULL, stream);
+    if (e == 0) e = quantize(x, l->x_type, l->rows, l->cols, ld_x, NULL, &d, &a, l->want_dw ? &atr : NULL, stream);
+    if (e == 0) e = product(&a, &b, y, l->x_type, l->outs, NULL, sms, stream);
+    return done(&c, prev, e);
+}
+
+MC_EXPORT int falcom_mx4_linear_backward(const falcom_mx4_linear *l, const void *dy, size_t ld_dy, const void *kept,
+                                         void *dx, void *dw, void *work, void *stream) {
+    static const char *who = "falcom_mx4_linear_backward";
+    if (!layer_ok(who, l)) return ERROR_INVALID_PARAM;
+    if ((dx && !l->want_dx) || (dw && !l->want_dw)) return invalid(who, "forward kept nothing for this gradient");
+    const size_t xs = g_type_size[l->x_type], ws = g_type_size[l->weight_type];
+    const int none = l->rows == 0 || l->outs == 0;
+    const size_t dy_bytes = none ? 0 : extent(l->rows, l->outs, ld_dy, xs);
+    if ((!none && dy_bytes == 0) || l->rows * l->cols > MX_ELEMENTS || l->outs * l->cols > MX_ELEMENTS)
+        return invalid(who, "rows of dy overlap, or sizes are out of range");
+    mx_random r = {0};
+    mx_drop d = {{0}, 0, 0};
+    mx_call c;
+    begin(&c, who);
+    if (!layer_drop(&c, &d, l)) return invalid(who, "p must lie in [0, 1)");
+    if (dx) array(&c, "dx", dx, l->rows * l->cols * xs, xs, 1);
+    if (dw) array(&c, "dw", dw, l->outs * l->cols * ws, ws, 1);
+    array(&c, "dy", dy, dy_bytes, xs, 0);
+    array(&c, "kept", kept, falcom_mx4_linear_kept_bytes(l), 16, 0);
+    array(&c, "work", work, falcom_mx4_linear_work_bytes(l, 1), 16, 1);
+    random_of(&c, &r, &l->random, ROUNDING);
+    if (c.ok && c.n == 0) return ERROR_NONE;
+    int prev, sms, rc = go(&c, &prev, &sms);
+    if (rc) return rc;
+    uint8_t *at = (uint8_t *)work, *keep = (uint8_t *)kept;
+    mx_matrix g, gt, bt, atr;
+    if (l->want_dx) {
+        g = matrix_in(&at, l->rows, l->outs);
+        bt = matrix_in(&keep, l->cols, l->outs);
+    }
+    if (l->want_dw) {
+        gt = matrix_in(&at, l->outs, l->rows);
+        atr = matrix_in(&keep, l->cols, l->rows);
+    }
+    int e = quantize(dy, l->x_type, l->rows, l->outs, ld_dy, &r, NULL, dx ? &g : NULL, dw ? &gt : NULL, stream);
+    if (e == 0 && dx) e = product(&g, &bt, dx, l->x_type, l->cols, &d, sms, stream);
+    if (e == 0 && dw) e = product(&gt, &atr, dw, l->weight_type, l->cols, NULL, sms, stream);
+    return done(&c, prev, e);
 }
 
 MC_EXPORT int falcom_mx4_errors(void) {
@@ -289,7 +455,7 @@ MC_EXPORT int falcom_dropout(const void *x, const void *residual, void *y, int d
                              const falcom_dropout_args *drop, void *stream) {
     static const char *who = "falcom_dropout";
     if (!drop || !known_type(dtype)) return invalid(who, "no arguments, or an unknown type");
-    if (rows > MX_MOST || cols > MX_MOST) return invalid(who, "too many rows or columns");
+    if (rows > MX_MOST || cols > MX_MOST || rows * cols > MX_ELEMENTS) return invalid(who, "too many rows or columns");
     mx_call c;
     mx_dropout_launch L;
     memset(&L, 0, sizeof(L));
@@ -307,7 +473,7 @@ MC_EXPORT int falcom_dropout(const void *x, const void *residual, void *y, int d
     L.y = y;
     L.rows = (int64_t)rows;
     L.cols = (int64_t)cols;
-    L.powers = g_powers;
     L.vectors = (((uintptr_t)x | (uintptr_t)y | (uintptr_t)residual) & 15) == 0 && cols % 8 == 0;
+    L.flat = rows == 1 || cols % MX_BLOCK == 0;
     return done(&c, prev, mc_launch_mx_dropout(&L, dtype, sms, stream));
 }

@@ -8,114 +8,7 @@ namespace {
 
 #define MX_TPB 256
 
-// ------------------------------------------------------------- vectors
-// A warp has 8 blocks; lane i has element i of each, so loads and stores are
-// whole lines at any alignment, and a block's largest magnitude is one
-// reduction.  The codes then change lanes: those of 8 elements of a block
-// that make up a 32-bit word lie on 8 lanes, one for each block.
-
-// Lane i of a group of 8 holds 8 nibbles, one for each of 8 words; returns
-// word i of the group, nibble j from lane j.
-__device__ __forceinline__ uint32_t transpose8(uint32_t v, int lane) {
-    uint32_t o = __shfl_xor_sync(0xffffffffu, v, 4);
-    v = lane & 4 ? (o >> 16) | (v & 0xFFFF0000u) : (v & 0x0000FFFFu) | (o << 16);
-    o = __shfl_xor_sync(0xffffffffu, v, 2);
-    v = lane & 2 ? ((o >> 8) & 0x00FF00FFu) | (v & 0xFF00FF00u) : (v & 0x00FF00FFu) | ((o << 8) & 0xFF00FF00u);
-    o = __shfl_xor_sync(0xffffffffu, v, 1);
-    return lane & 1 ? ((o >> 4) & 0x0F0F0F0Fu) | (v & 0xF0F0F0F0u) : (v & 0x0F0F0F0Fu) | ((o << 4) & 0xF0F0F0F0u);
-}
-
-template <typename T, bool BASE, bool RANDOM>
-__global__ void __launch_bounds__(MX_TPB) k_mx_encode(const __grid_constant__ mx_encode_launch L) {
-    const int lane = threadIdx.x & 31;
-    const T *x = (const T *)L.x;
-    mx_key key = {};
-    if (RANDOM) key = mx_key_of(L.random);
-    const int64_t chunks = (L.n + 255) / 256, step = (int64_t)gridDim.x * (MX_TPB / 32);
-    for (int64_t c = (int64_t)blockIdx.x * (MX_TPB / 32) + (threadIdx.x >> 5); c < chunks; c += step) {
-        const int64_t e0 = c * 256 + lane;
-        const int left = (int)min(L.n - c * 256, (int64_t)256);
-        float v[8], held[8];
-        T raw[8];
-#pragma unroll
-        for (int b = 0; b < 8; b++) {
-            const bool in = 32 * b + lane < left;
-            memset(&raw[b], 0, sizeof(T));
-            held[b] = 0.0f;
-            if (in) raw[b] = x[e0 + 32 * b];
-            if (BASE && in) held[b] = L.base[e0 + 32 * b];
-        }
-        uint32_t codes = 0, scales[2] = {0, 0};
-#pragma unroll
-        for (int b = 0; b < 8; b++) {
-            v[b] = BASE ? mx_f32(raw[b]) - held[b] : mx_f32(raw[b]);
-            const uint32_t s = mx_scale(__reduce_max_sync(0xffffffffu, __float_as_uint(v[b]) & 0x7FFFFFFFu));
-            scales[b >> 2] |= s << (8 * (b & 3));
-            const float y = v[b] * mx_inverse(s);
-            uint32_t code;
-            if (RANDOM) {
-                const mx_bits w = mx_bits_at(key, L.powers, (uint64_t)(c * 128 + 16 * b + (lane >> 1)));
-                code = mx_code_random(__fmul_rz(fabsf(y), MX_CUT), lane & 1 ? w.high : w.low, L.powers) | (__float_as_uint(y) >> 31 << 3);
-            } else {
-                code = mx_code_near(y);
-            }
-            if (s == 255u) code = 0;
-            codes |= code << (4 * b);
-            if (BASE && 32 * b + lane < left) L.base[e0 + 32 * b] = held[b] + mx_value(code) * mx_scale_value(s);
-        }
-        // lane 8 g + b: elements 8 g .. 8 g + 7 of block b
-        codes = transpose8(codes, lane);
-        const int word = (lane & 7) * 4 + (lane >> 3);   // of the chunk's 32
-        const int bytes = (left + 1) / 2;
-        uint8_t *out = L.codes + c * 128 + 4 * word;
-        if (4 * word + 4 <= bytes) *(uint32_t *)out = codes;
-        else
-            for (int i = 0; 4 * word + i < bytes; i++) out[i] = (uint8_t)(codes >> (8 * i));
-        if (lane < (left + 31) / 32) L.scales[c * 8 + lane] = (uint8_t)((lane & 4 ? scales[1] : scales[0]) >> (8 * (lane & 3)));
-    }
-}
-
-template <typename T, bool ADD>
-__global__ void __launch_bounds__(MX_TPB) k_mx_decode(const __grid_constant__ mx_decode_launch L) {
-    const int lane = threadIdx.x & 31;
-    T *out = (T *)L.out;
-    const int64_t chunks = (L.n + 255) / 256, step = (int64_t)gridDim.x * (MX_TPB / 32);
-    for (int64_t c = (int64_t)blockIdx.x * (MX_TPB / 32) + (threadIdx.x >> 5); c < chunks; c += step) {
-        const int left = (int)min(L.n - c * 256, (int64_t)256);
-        const int bytes = (left + 1) / 2;
-        const uint8_t *in = L.codes + c * 128 + 4 * lane;
-        uint32_t word = 0, scale = 0;
-        if (4 * lane + 4 <= bytes) word = *(const uint32_t *)in;
-        else
-            for (int i = 0; 4 * lane + i < bytes; i++) word |= (uint32_t)in[i] << (8 * i);
-        if (lane < (left + 31) / 32) scale = L.scales[c * 8 + lane];
-        T held[8];
-        if (ADD) {
-#pragma unroll
-            for (int b = 0; b < 8; b++)
-                if (32 * b + lane < left) held[b] = out[c * 256 + 32 * b + lane];
-        }
-#pragma unroll
-        for (int b = 0; b < 8; b++) {
-            const uint32_t code = __shfl_sync(0xffffffffu, word, 4 * b + (lane >> 3)) >> (4 * (lane & 7));
-            const float v = L.weight * (mx_value(code) * mx_scale_value(__shfl_sync(0xffffffffu, scale, b)));
-            if (32 * b + lane < left) {
-                T r;
-                mx_from(&r, ADD ? mx_f32(held[b]) + v : v);
-                out[c * 256 + 32 * b + lane] = r;
-            }
-        }
-    }
-}
-
-// ------------------------------------------------------------- matrices
-// A CTA has 128 x 128 elements: 4 blocks of every row and of every column,
-// whose scales are one 512-byte piece of either layout.  Rows are rounded as
-// they come in (8 elements a thread, 4 threads a block); for the columns the
-// tile goes through shared memory, where a thread has a block of each of two
-// neighbouring columns, which share their random words.
-#define MX_TILE 128
-
+// ------------------------------------------------------------- elements
 template <typename T>
 struct mx_vec8 {
     T x[8];
@@ -196,8 +89,8 @@ __device__ __forceinline__ uint32_t signs4x2(const uint32_t *w) {
 
 // The codes of 8 elements.  y: values (at random: magnitudes) times 1 / scale, two by two.
 template <bool RANDOM>
-__device__ __forceinline__ uint32_t codes8(const float2 *y, uint32_t signs, const uint32_t *bits16, const mx_powers &P) {
-    if (RANDOM) return mx_codes8_random(y, bits16, P) | signs;
+__device__ __forceinline__ uint32_t codes8(const float2 *y, uint32_t signs, const uint32_t *bits16) {
+    if (RANDOM) return mx_codes8_random(y, bits16) | signs;
     return mx_codes8((const float *)y);
 }
 
@@ -214,7 +107,7 @@ __device__ __forceinline__ float2 two_values(const uint32_t *w, int i) {
 
 // A row's 8 elements (raw words) to codes.
 template <typename T, bool RANDOM, bool DROP>
-__device__ __forceinline__ uint32_t row_codes(const uint32_t *w, float inv, float factor, const mx_bits *bits, const mx_powers &P) {
+__device__ __forceinline__ uint32_t row_codes(const uint32_t *w, float inv, float factor, const mx_bits *bits) {
     float2 y[4];
     uint32_t bits16[8], signs = 0;
 #pragma unroll
@@ -231,8 +124,240 @@ __device__ __forceinline__ uint32_t row_codes(const uint32_t *w, float inv, floa
         if constexpr (sizeof(T) == 4) signs = signs8<3>(w);
         else signs = signs4x2(w);
     }
-    return codes8<RANDOM>(y, signs, bits16, P);
+    return codes8<RANDOM>(y, signs, bits16);
 }
+
+// ------------------------------------------------------------- vectors
+// A warp has 8 blocks.  On 16-byte boundaries a lane has 8 elements, 4 lanes a
+// block, as in a matrix's rows.  On others lane i has element i of each block,
+// so that loads and stores are whole lines at any alignment, and a block's
+// largest magnitude is one reduction.  The codes then change lanes: those of 8 elements of a block
+// that make up a 32-bit word lie on 8 lanes, one for each block.
+
+// Lane i of a group of 8 holds 8 nibbles, one for each of 8 words; returns
+// word i of the group, nibble j from lane j.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v, int lane) {
+    uint32_t o = __shfl_xor_sync(0xffffffffu, v, 4);
+    v = lane & 4 ? (o >> 16) | (v & 0xFFFF0000u) : (v & 0x0000FFFFu) | (o << 16);
+    o = __shfl_xor_sync(0xffffffffu, v, 2);
+    v = lane & 2 ? ((o >> 8) & 0x00FF00FFu) | (v & 0xFF00FF00u) : (v & 0x00FF00FFu) | ((o << 8) & 0xFF00FF00u);
+    o = __shfl_xor_sync(0xffffffffu, v, 1);
+    return lane & 1 ? ((o >> 4) & 0x0F0F0F0Fu) | (v & 0xF0F0F0F0u) : (v & 0x0F0F0F0Fu) | ((o << 4) & 0xF0F0F0F0u);
+}
+
+__device__ __forceinline__ void store8(float *p, const float *v) {
+    ((float4 *)p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    ((float4 *)p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+template <typename T>
+__device__ __forceinline__ void store8(T *p, const float *v) {
+    mx_vec8<T> r;
+#pragma unroll
+    for (int j = 0; j < 8; j++) mx_from(&r.x[j], v[j]);
+    *(uint4 *)p = *(const uint4 *)&r;
+}
+// 8 elements, or as many as there are (0 for the others)
+template <typename T>
+__device__ __forceinline__ mx_vec8<T> load_up_to_8(const T *p, int n) {
+    if (n >= 8) return load8(p);
+    mx_vec8<T> v;
+    memset(&v, 0, sizeof(v));
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+        if (j < n) v.x[j] = p[j];
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ void store_up_to_8(T *p, const float *v, int n) {
+    if (n >= 8) {
+        store8(p, v);
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+        if (j < n) mx_from(&p[j], v[j]);
+}
+
+template <typename T, bool BASE, bool RANDOM>
+__global__ void __launch_bounds__(MX_TPB) k_mx_encode8(const __grid_constant__ mx_encode_launch L) {
+    mx_key key = {};
+    if (RANDOM) key = mx_key_of(L.random);
+    // whole warps: 4 lanes find a block's largest magnitude together
+    const int64_t lanes = (L.n + 255) / 256 * 32, step = (int64_t)gridDim.x * MX_TPB;
+    for (int64_t i = (int64_t)blockIdx.x * MX_TPB + threadIdx.x; i < lanes; i += step) {
+        const int left = (int)max((int64_t)0, min(L.n - 8 * i, (int64_t)8));
+        mx_vec8<float> v, held;
+        memset(&held, 0, sizeof(held));
+        if constexpr (sizeof(T) == 4) {
+            v = load_up_to_8((const float *)L.x + 8 * i, left);
+        } else {
+            const mx_vec8<T> raw = load_up_to_8((const T *)L.x + 8 * i, left);
+#pragma unroll
+            for (int j = 0; j < 8; j++) v.x[j] = mx_f32(raw.x[j]);
+        }
+        if (BASE) {
+            if (left == 8) {   // (not through the read-only cache: the values are written below)
+                ((float4 *)held.x)[0] = ((const float4 *)(L.base + 8 * i))[0];
+                ((float4 *)held.x)[1] = ((const float4 *)(L.base + 8 * i))[1];
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (j < left) held.x[j] = L.base[8 * i + j];
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++) v.x[j] -= held.x[j];
+        }
+        uint32_t w[8], m = 0;
+        memcpy(w, &v, sizeof(v));
+#pragma unroll
+        for (int j = 0; j < 8; j++) m = larger(m, w[j], 0.0f);
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        const uint32_t s = mx_scale(m);
+        mx_bits bits[4];
+        if (RANDOM) {
+            const uint32_t start = mx_start(key, (uint64_t)(4 * i));
+#pragma unroll
+            for (int j = 0; j < 4; j++) bits[j] = mx_bits_of(key, start ^ j);
+        }
+        uint32_t codes = row_codes<float, RANDOM, false>(w, mx_inverse(s), 1.0f, bits);
+        if (s == 255u) codes = 0;
+        if (BASE) {
+            const float unit = mx_scale_value(s);
+#pragma unroll
+            for (int j = 0; j < 8; j++) held.x[j] += mx_value(codes >> (4 * j)) * unit;
+            store_up_to_8(L.base + 8 * i, held.x, left);
+        }
+        if (left == 8) ((uint32_t *)L.codes)[i] = codes;
+        else
+            for (int j = 0; j < (left + 1) / 2; j++) L.codes[4 * i + j] = (uint8_t)(codes >> (8 * j));
+        if ((i & 3) == 0 && left > 0) L.scales[i / 4] = (uint8_t)s;
+    }
+}
+
+template <typename T, bool ADD>
+__global__ void __launch_bounds__(MX_TPB) k_mx_decode8(const __grid_constant__ mx_decode_launch L) {
+    const int64_t lanes = (L.n + 7) / 8, step = (int64_t)gridDim.x * MX_TPB;
+    T *out = (T *)L.out;
+    for (int64_t i = (int64_t)blockIdx.x * MX_TPB + threadIdx.x; i < lanes; i += step) {
+        const int left = (int)min(L.n - 8 * i, (int64_t)8);
+        uint32_t codes = 0;
+        if (left == 8) codes = __ldg((const uint32_t *)L.codes + i);
+        else
+            for (int j = 0; j < (left + 1) / 2; j++) codes |= (uint32_t)L.codes[4 * i + j] << (8 * j);
+        const float unit = mx_scale_value(__ldg(L.scales + i / 4));
+        mx_vec8<T> held;
+        memset(&held, 0, sizeof(held));
+        if (ADD) {
+            if (left == 8) {
+#pragma unroll
+                for (int j = 0; j < (int)(sizeof(held) / 16); j++) ((uint4 *)&held)[j] = ((const uint4 *)(out + 8 * i))[j];
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (j < left) held.x[j] = out[8 * i + j];
+            }
+        }
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            v[j] = L.weight * (mx_value(codes >> (4 * j)) * unit);
+            if (ADD) v[j] = mx_f32(held.x[j]) + v[j];
+        }
+        store_up_to_8(out + 8 * i, v, left);
+    }
+}
+
+template <typename T, bool BASE, bool RANDOM>
+__global__ void __launch_bounds__(MX_TPB) k_mx_encode(const __grid_constant__ mx_encode_launch L) {
+    const int lane = threadIdx.x & 31;
+    const T *x = (const T *)L.x;
+    mx_key key = {};
+    if (RANDOM) key = mx_key_of(L.random);
+    const int64_t chunks = (L.n + 255) / 256, step = (int64_t)gridDim.x * (MX_TPB / 32);
+    for (int64_t c = (int64_t)blockIdx.x * (MX_TPB / 32) + (threadIdx.x >> 5); c < chunks; c += step) {
+        const int64_t e0 = c * 256 + lane;
+        const int left = (int)min(L.n - c * 256, (int64_t)256);
+        float v[8], held[8];
+        T raw[8];
+#pragma unroll
+        for (int b = 0; b < 8; b++) {
+            const bool in = 32 * b + lane < left;
+            memset(&raw[b], 0, sizeof(T));
+            held[b] = 0.0f;
+            if (in) raw[b] = x[e0 + 32 * b];
+            if (BASE && in) held[b] = L.base[e0 + 32 * b];
+        }
+        uint32_t codes = 0, scales[2] = {0, 0};
+#pragma unroll
+        for (int b = 0; b < 8; b++) {
+            v[b] = BASE ? mx_f32(raw[b]) - held[b] : mx_f32(raw[b]);
+            const uint32_t s = mx_scale(__reduce_max_sync(0xffffffffu, __float_as_uint(v[b]) & 0x7FFFFFFFu));
+            scales[b >> 2] |= s << (8 * (b & 3));
+            const float y = v[b] * mx_inverse(s);
+            uint32_t code;
+            if (RANDOM) {
+                const mx_bits w = mx_bits_at(key, (uint64_t)(c * 128 + 16 * b + (lane >> 1)));
+                code = mx_code_random(__fmul_rz(fabsf(y), MX_CUT), lane & 1 ? w.high : w.low) | (__float_as_uint(y) >> 31 << 3);
+            } else {
+                code = mx_code_near(y);
+            }
+            if (s == 255u) code = 0;
+            codes |= code << (4 * b);
+            if (BASE && 32 * b + lane < left) L.base[e0 + 32 * b] = held[b] + mx_value(code) * mx_scale_value(s);
+        }
+        // lane 8 g + b: elements 8 g .. 8 g + 7 of block b
+        codes = transpose8(codes, lane);
+        const int word = (lane & 7) * 4 + (lane >> 3);   // of the chunk's 32
+        const int bytes = (left + 1) / 2;
+        uint8_t *out = L.codes + c * 128 + 4 * word;
+        if (4 * word + 4 <= bytes) *(uint32_t *)out = codes;
+        else
+            for (int i = 0; 4 * word + i < bytes; i++) out[i] = (uint8_t)(codes >> (8 * i));
+        if (lane < (left + 31) / 32) L.scales[c * 8 + lane] = (uint8_t)((lane & 4 ? scales[1] : scales[0]) >> (8 * (lane & 3)));
+    }
+}
+
+template <typename T, bool ADD>
+__global__ void __launch_bounds__(MX_TPB) k_mx_decode(const __grid_constant__ mx_decode_launch L) {
+    const int lane = threadIdx.x & 31;
+    T *out = (T *)L.out;
+    const int64_t chunks = (L.n + 255) / 256, step = (int64_t)gridDim.x * (MX_TPB / 32);
+    for (int64_t c = (int64_t)blockIdx.x * (MX_TPB / 32) + (threadIdx.x >> 5); c < chunks; c += step) {
+        const int left = (int)min(L.n - c * 256, (int64_t)256);
+        const int bytes = (left + 1) / 2;
+        const uint8_t *in = L.codes + c * 128 + 4 * lane;
+        uint32_t word = 0, scale = 0;
+        if (4 * lane + 4 <= bytes) word = *(const uint32_t *)in;
+        else
+            for (int i = 0; 4 * lane + i < bytes; i++) word |= (uint32_t)in[i] << (8 * i);
+        if (lane < (left + 31) / 32) scale = L.scales[c * 8 + lane];
+        T held[8];
+        if (ADD) {
+#pragma unroll
+            for (int b = 0; b < 8; b++)
+                if (32 * b + lane < left) held[b] = out[c * 256 + 32 * b + lane];
+        }
+#pragma unroll
+        for (int b = 0; b < 8; b++) {
+            const uint32_t code = __shfl_sync(0xffffffffu, word, 4 * b + (lane >> 3)) >> (4 * (lane & 7));
+            const float v = L.weight * (mx_value(code) * mx_scale_value(__shfl_sync(0xffffffffu, scale, b)));
+            if (32 * b + lane < left) {
+                T r;
+                mx_from(&r, ADD ? mx_f32(held[b]) + v : v);
+                out[c * 256 + 32 * b + lane] = r;
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------- matrices
+// A CTA has 128 x 128 elements: 4 blocks of every row and of every column,
+// whose scales are one 512-byte piece of either layout.  Rows are rounded as
+// they come in (8 elements a thread, 4 threads a block); for the columns the
+// tile goes through shared memory, where a thread has a block of each of two
+// neighbouring columns, which share their random words.
+#define MX_TILE 128
 
 // Shared memory of a tile: its elements, and its random words (of which a
 // column's rounding has the same as a row's).
@@ -272,7 +397,7 @@ __global__ void __launch_bounds__(MX_TPB, COLS ? 3 : 4) k_mx_quantize(const __gr
             const uint32_t start = mx_start(drop, pair);
 #pragma unroll
             for (int j = 0; j < 8; j += 2) {
-                const mx_bits u = mx_bits_of(drop, L.powers, start ^ (j / 2));
+                const mx_bits u = mx_bits_of(drop, start ^ (j / 2));
                 if (u.low < L.drop.threshold) memset(&v.x[j], 0, sizeof(T));
                 if (u.high < L.drop.threshold) memset(&v.x[j + 1], 0, sizeof(T));
             }
@@ -281,7 +406,7 @@ __global__ void __launch_bounds__(MX_TPB, COLS ? 3 : 4) k_mx_quantize(const __gr
         if (RANDOM) {
             const uint32_t start = mx_start(key, pair);
 #pragma unroll
-            for (int j = 0; j < 4; j++) bits[j] = mx_bits_of(key, L.powers, start ^ j);
+            for (int j = 0; j < 4; j++) bits[j] = mx_bits_of(key, start ^ j);
         }
         if (COLS) {
             uint4 *q = (uint4 *)(s_tile + (y * MX_TILE + 8 * tx) * sizeof(T));
@@ -290,7 +415,7 @@ __global__ void __launch_bounds__(MX_TPB, COLS ? 3 : 4) k_mx_quantize(const __gr
             if (RANDOM) {
                 uint32_t u[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) u[j] = bits[j].high * L.powers.p16 + bits[j].low;
+                for (int j = 0; j < 4; j++) u[j] = bits[j].high << 16 | bits[j].low;
                 *(uint4 *)(s_words + y * (MX_TILE / 2) + 4 * tx) = *(const uint4 *)u;
             }
         }
@@ -309,7 +434,7 @@ __global__ void __launch_bounds__(MX_TPB, COLS ? 3 : 4) k_mx_quantize(const __gr
             // (the largest product is the largest element's)
             if (DROP) top = __float_as_uint(__uint_as_float(top) * L.drop.factor);
             const uint32_t s = mx_scale(top);
-            uint32_t codes = row_codes<T, RANDOM, DROP>(w, mx_inverse(s), L.drop.factor, bits, L.powers);
+            uint32_t codes = row_codes<T, RANDOM, DROP>(w, mx_inverse(s), L.drop.factor, bits);
             if (s == 255u) codes = 0;
             if (inside) *(uint32_t *)(to + i * 16 * 128) = codes;   // (16 rows on the pieces of a row lie alike)
             if ((tx & 3) == 0) s_rows[(y & 31) * 16 + (y >> 5) * 4 + (tx >> 2)] = (uint8_t)s;
@@ -409,7 +534,7 @@ __global__ void __launch_bounds__(MX_TPB, COLS ? 3 : 4) k_mx_quantize(const __gr
                 else f[0][j / 2].x = x.x, f[1][j / 2].x = x.y;
                 if (RANDOM) {
                     const uint32_t u = s_words[(32 * b + 8 * i + j) * (MX_TILE / 2) + p];
-                    bits16[1][j] = __umulhi(u, L.powers.p16);
+                    bits16[1][j] = u >> 16;
                     bits16[0][j] = u & 0xFFFFu;
                 }
             }
@@ -422,8 +547,8 @@ __global__ void __launch_bounds__(MX_TPB, COLS ? 3 : 4) k_mx_quantize(const __gr
                     signs[1] = signs8<3>(w[0]);
                 }
             }
-            codes[0][i] = codes8<RANDOM>(f[0], signs[0], bits16[0], L.powers);
-            codes[1][i] = codes8<RANDOM>(f[1], signs[1], bits16[1], L.powers);
+            codes[0][i] = codes8<RANDOM>(f[0], signs[0], bits16[0]);
+            codes[1][i] = codes8<RANDOM>(f[1], signs[1], bits16[1]);
         }
 #pragma unroll
         for (int h = 0; h < 2; h++) {
@@ -459,8 +584,7 @@ __global__ void __launch_bounds__(MX_TPB) k_mx_dequantize(const __grid_constant_
 
 // -------------------------------------------------------------- dropout
 template <typename T, bool RES>
-__device__ __forceinline__ void drop_pair(const mx_dropout_launch &L, mx_key key, uint64_t pair, const T *x, const T *res, T *y) {
-    const mx_bits w = mx_bits_at(key, L.powers, pair);
+__device__ __forceinline__ void drop_pair(const mx_dropout_launch &L, mx_bits w, const T *x, const T *res, T *y) {
 #pragma unroll
     for (int h = 0; h < 2; h++) {
         float f = (h ? w.high : w.low) < L.drop.threshold ? 0.0f : mx_f32(x[h]) * L.drop.factor;
@@ -479,20 +603,30 @@ __global__ void __launch_bounds__(MX_TPB) k_mx_dropout(const __grid_constant__ m
     if (L.vectors) {   // 8 elements a thread
         const int64_t words = L.cols / 8, all = L.rows * words;
         for (int64_t i = first; i < all; i += step) {
-            const int64_t r = i / words, c = (i - r * words) * 8;
-            const mx_vec8<T> v = load8(x + i * 8);
-            mx_vec8<T> o, z;
-            if (RES) z = load8(res + i * 8);
-            const uint64_t pair = (uint64_t)(r * wide + c) / 2;
+            mx_vec8<T> v, z;   // (not through the read-only cache: y may be either)
 #pragma unroll
-            for (int j = 0; j < 8; j += 2) drop_pair<T, RES>(L, key, pair + j / 2, v.x + j, z.x + j, o.x + j);
+            for (int j = 0; j < (int)(sizeof(v) / 16); j++) ((uint4 *)&v)[j] = ((const uint4 *)(x + i * 8))[j];
+            if (RES) {
+#pragma unroll
+                for (int j = 0; j < (int)(sizeof(z) / 16); j++) ((uint4 *)&z)[j] = ((const uint4 *)(res + i * 8))[j];
+            }
+            int64_t at = i * 8;
+            if (!L.flat) {
+                const int64_t r = all >> 31 ? i / words : (int64_t)((uint32_t)i / (uint32_t)words);
+                at = r * wide + (i - r * words) * 8;
+            }
+            const uint32_t start = mx_start(key, (uint64_t)at / 2);
+            mx_vec8<T> o;
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) drop_pair<T, RES>(L, mx_bits_of(key, start ^ (j / 2)), v.x + j, z.x + j, o.x + j);
 #pragma unroll
             for (int j = 0; j < (int)(sizeof(o) / 16); j++) ((uint4 *)(y + i * 8))[j] = ((const uint4 *)&o)[j];
         }
     } else {
         const int64_t pairs = (L.cols + 1) / 2, all = L.rows * pairs;
         for (int64_t i = first; i < all; i += step) {
-            const int64_t r = i / pairs, c = (i - r * pairs) * 2, at = r * L.cols + c;
+            const int64_t r = all >> 31 ? i / pairs : (int64_t)((uint32_t)i / (uint32_t)pairs);
+            const int64_t c = (i - r * pairs) * 2, at = r * L.cols + c;
             const bool two = c + 1 < L.cols;
             T v[2], z[2], o[2];
             v[0] = x[at];
@@ -501,7 +635,7 @@ __global__ void __launch_bounds__(MX_TPB) k_mx_dropout(const __grid_constant__ m
                 z[0] = res[at];
                 z[1] = two ? res[at + 1] : z[0];
             }
-            drop_pair<T, RES>(L, key, (uint64_t)(r * wide + c) / 2, v, z, o);
+            drop_pair<T, RES>(L, mx_bits_at(key, (uint64_t)(r * wide + c) / 2), v, z, o);
             y[at] = o[0];
             if (two) y[at + 1] = o[1];
         }
@@ -516,20 +650,24 @@ static int grid_for(int64_t units, int per_cta, int sms, int per_sm) {
 template <typename T>
 static void encode(const mx_encode_launch &L, int sms, cudaStream_t s) {
     const int grid = grid_for((L.n + 255) / 256, MX_TPB / 32, sms, 8);
-    if (L.base) {
-        if (L.random.on) k_mx_encode<T, true, true><<<grid, MX_TPB, 0, s>>>(L);
-        else k_mx_encode<T, true, false><<<grid, MX_TPB, 0, s>>>(L);
+    void (*kern)(const mx_encode_launch);
+    if (L.vectors) {
+        if (L.base) kern = L.random.on ? k_mx_encode8<T, true, true> : k_mx_encode8<T, true, false>;
+        else kern = L.random.on ? k_mx_encode8<T, false, true> : k_mx_encode8<T, false, false>;
     } else {
-        if (L.random.on) k_mx_encode<T, false, true><<<grid, MX_TPB, 0, s>>>(L);
-        else k_mx_encode<T, false, false><<<grid, MX_TPB, 0, s>>>(L);
+        if (L.base) kern = L.random.on ? k_mx_encode<T, true, true> : k_mx_encode<T, true, false>;
+        else kern = L.random.on ? k_mx_encode<T, false, true> : k_mx_encode<T, false, false>;
     }
+    kern<<<grid, MX_TPB, 0, s>>>(L);
 }
 
 template <typename T>
 static void decode(const mx_decode_launch &L, int sms, cudaStream_t s) {
     const int grid = grid_for((L.n + 255) / 256, MX_TPB / 32, sms, 8);
-    if (L.accumulate) k_mx_decode<T, true><<<grid, MX_TPB, 0, s>>>(L);
-    else k_mx_decode<T, false><<<grid, MX_TPB, 0, s>>>(L);
+    void (*kern)(const mx_decode_launch);
+    if (L.vectors) kern = L.accumulate ? k_mx_decode8<T, true> : k_mx_decode8<T, false>;
+    else kern = L.accumulate ? k_mx_decode<T, true> : k_mx_decode<T, false>;
+    kern<<<grid, MX_TPB, 0, s>>>(L);
 }
 
 template <typename T, bool ROWS, bool COLS, bool RANDOM, bool DROP>

@@ -20,14 +20,6 @@ extern "C" {
 #define MX_GROUP 128                /* rows whose scales lie together */
 #define MX_TYPES 3
 
-/* Powers of two that the compiler does not know: multiplying by them moves
- * shifts from the pipe of logic operations, which bounds the rounding at
- * random, to that of multiplications. */
-typedef struct {
-    uint32_t p4, p6, p10, p16, p19;
-} mx_powers;
-#define MX_POWERS {1u << 4, 1u << 6, 1u << 10, 1u << 16, 1u << 19}
-
 /* Random bits of one purpose; counter NULL counts as 0. */
 typedef struct {
     uint32_t key;              /* hash of purpose and seed */
@@ -53,7 +45,7 @@ typedef struct {
     float *base;               /* or NULL */
     uint8_t *codes, *scales;
     mx_random random;
-    mx_powers powers;
+    int32_t vectors;           /* x and base on 16-byte boundaries */
 } mx_encode_launch;
 
 typedef struct {
@@ -62,6 +54,7 @@ typedef struct {
     void *out;
     float weight;
     int32_t accumulate;
+    int32_t vectors;           /* out on a 16-byte boundary */
 } mx_decode_launch;
 
 typedef struct {
@@ -72,7 +65,6 @@ typedef struct {
     mx_drop drop;
     int32_t vectors;           /* every row starts on a 16-byte boundary */
     uint32_t tiles;            /* of 128 columns */
-    mx_powers powers;
 } mx_quantize_launch;
 
 typedef struct {
@@ -86,7 +78,6 @@ typedef struct {
     void *out;                 /* [a.rows][ld] */
     int64_t ld;
     mx_drop drop;
-    mx_powers powers;
 } mx_product_launch;
 
 typedef struct {
@@ -95,7 +86,7 @@ typedef struct {
     int64_t rows, cols;
     mx_drop drop;
     int32_t vectors;           /* rows are whole 16-byte vectors of aligned memory */
-    mx_powers powers;
+    int32_t flat;              /* an element's place is its index: rows are whole blocks, or one */
 } mx_dropout_launch;
 
 /* All return a CUDA error code (0: queued). */

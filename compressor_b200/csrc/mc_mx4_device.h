@@ -59,15 +59,15 @@ __device__ __forceinline__ uint32_t mx_start(mx_key k, uint64_t pair) {
 struct mx_bits {
     uint32_t low, high;
 };
-__device__ __forceinline__ mx_bits mx_bits_of(mx_key k, const mx_powers &P, uint32_t start) {
+__device__ __forceinline__ mx_bits mx_bits_of(mx_key k, uint32_t start) {
     uint32_t x = start * 0x85EBCA6Bu;
-    x = (x ^ __umulhi(x, P.p19) ^ k.b) * 0xC2B2AE35u;   // x >> 13
+    x = (x ^ (x >> 13) ^ k.b) * 0xC2B2AE35u;
     mx_bits r;
-    r.high = __umulhi(x, P.p16);                        // x >> 16
+    r.high = x >> 16;
     r.low = (x ^ r.high) & 0xFFFFu;
     return r;
 }
-__device__ __forceinline__ mx_bits mx_bits_at(mx_key k, const mx_powers &P, uint64_t pair) { return mx_bits_of(k, P, mx_start(k, pair)); }
+__device__ __forceinline__ mx_bits mx_bits_at(mx_key k, uint64_t pair) { return mx_bits_of(k, mx_start(k, pair)); }
 __device__ __forceinline__ int64_t mx_wide(int64_t cols) { return (cols + MX_BLOCK - 1) / MX_BLOCK * MX_BLOCK; }
 
 // ---------------------------------------------------------- 4-bit rounding
@@ -127,23 +127,19 @@ __device__ __forceinline__ float2 mx_mul2_cut(float2 a, float2 b) {   // towards
 #define MX_CUT 1.17549435e-38f
 // The magnitude code of y * 2^-126 with these 16 bits: its bits + 64 * bits16
 // + 32, shifted right by 22.
-__device__ __forceinline__ uint32_t mx_code_random(float cut, uint32_t bits16, const mx_powers &P) {
-    const uint32_t t = bits16 * P.p6 + __float_as_uint(cut);
-    return (uint32_t)(((uint64_t)t * P.p10 + (32u << 10)) >> 32);
+__device__ __forceinline__ uint32_t mx_code_random(float cut, uint32_t bits16) {
+    return (__float_as_uint(cut) + ((bits16 << 6) | 32u)) >> 22;
 }
 // Magnitude codes of 8 elements: y their magnitudes times 1 / scale, two by
 // two, and the bits of each.
-__device__ __forceinline__ uint32_t mx_codes8_random(const float2 *y, const uint32_t *bits16, const mx_powers &P) {
-    uint32_t r[2];
+__device__ __forceinline__ uint32_t mx_codes8_random(const float2 *y, const uint32_t *bits16) {
+    uint32_t p[4];
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-        const float2 a = mx_mul2_cut(y[2 * h], make_float2(MX_CUT, MX_CUT)), b = mx_mul2_cut(y[2 * h + 1], make_float2(MX_CUT, MX_CUT));
-        r[h] = mx_code_random(b.y, bits16[4 * h + 3], P);
-        r[h] = r[h] * P.p4 + mx_code_random(b.x, bits16[4 * h + 2], P);
-        r[h] = r[h] * P.p4 + mx_code_random(a.y, bits16[4 * h + 1], P);
-        r[h] = r[h] * P.p4 + mx_code_random(a.x, bits16[4 * h], P);
+    for (int i = 0; i < 4; i++) {
+        const float2 m = mx_mul2_cut(y[i], make_float2(MX_CUT, MX_CUT));
+        p[i] = mx_code_random(m.x, bits16[2 * i]) + (mx_code_random(m.y, bits16[2 * i + 1]) << 4);
     }
-    return r[1] * P.p16 + r[0];
+    return (p[0] + (p[1] << 8)) + ((p[2] + (p[3] << 8)) << 16);
 }
 
 // The value of the code in bits 0 to 3, without its scale.

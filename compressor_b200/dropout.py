@@ -17,29 +17,33 @@ from . import mx4 as _mx4
 
 
 def _run(x: torch.Tensor, residual: Optional[torch.Tensor], p: float, seed: int, counter) -> torch.Tensor:
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    x = x.contiguous()
+    y = torch.empty_like(x)
     cols = x.shape[-1] if x.dim() else 1
     args = abi.DropoutArgsC(p, _mx4._seeded(seed, counter, x.device))
     _mx4._done(_mx4._library().falcom_dropout(
-        x.data_ptr(), residual.data_ptr() if residual is not None else None, y.data_ptr(), _mx4._TYPES[x.dtype],
-        x.numel() // cols if cols else 0, cols, ctypes.byref(args), _mx4._stream(x.device)), "falcom_dropout")
+        x.data_ptr(), residual.contiguous().data_ptr() if residual is not None else None, y.data_ptr(),
+        _mx4._TYPES[x.dtype], x.numel() // cols if cols else 0, cols, ctypes.byref(args), _mx4._stream(x.device)),
+        "falcom_dropout")
     return y
 
 
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, p, seed, counter):
-        ctx.p, ctx.seed = p, seed
-        # the counter as it is now, whatever it is when the gradient is asked for
-        ctx.save_for_backward(counter.clone() if counter is not None else None)
-        return _run(x.contiguous(), residual.contiguous() if residual is not None else None, p, seed, counter)
+        ctx.p, ctx.seed, ctx.counter = p, seed, None
+        if counter is not None:   # as it is now, whatever it is when the gradient is asked for
+            ctx.counter = counter.clone()
+        return _run(x, residual, p, seed, counter)
 
     @staticmethod
     def backward(ctx, dy):
-        counter, = ctx.saved_tensors
-        # through apply: the gradient of the gradient is the same operation again
-        dx = _Dropout.apply(dy, None, ctx.p, ctx.seed, counter) if ctx.needs_input_grad[0] else None
-        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
+        need_x, need_residual = ctx.needs_input_grad[:2]
+        dx = None
+        if need_x:
+            # through apply where a graph is wanted: the gradient of the gradient is the same operation again
+            dx = (_Dropout.apply if torch.is_grad_enabled() else _run)(dy, None, ctx.p, ctx.seed, ctx.counter)
+        return dx, dy if need_residual else None, None, None, None
 
 
 def dropout(x: torch.Tensor, p: float = 0.5, seed: int = 0, counter: Optional[torch.Tensor] = None,
@@ -49,12 +53,14 @@ def dropout(x: torch.Tensor, p: float = 0.5, seed: int = 0, counter: Optional[to
     dimension.  A dropped element is 0 whatever x holds there, infinity and NaN
     included, and so is its gradient.  Give each step and place a seed of its
     own, or a counter (an int64 tensor on the device, read when the work runs)
-    that is counted up."""
+    that is counted up.  Without a residual p = 0 returns x itself."""
     _mx4._check(x, "x")
     if residual is not None:
         _mx4._check(residual, "residual")
         if residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device:
             raise ValueError(f"residual is {residual.dtype} {tuple(residual.shape)} on {residual.device}, x {x.dtype} "
                              f"{tuple(x.shape)} on {x.device}")
-    _mx4._drop(p, seed, counter, x.device)
+    _mx4._check_p(p)
+    if p == 0 and residual is None:
+        return x
     return _Dropout.apply(x, residual, float(p), int(seed), counter)

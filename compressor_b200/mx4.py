@@ -88,10 +88,9 @@ def _seeded(seed: int, counter: Optional[torch.Tensor], device) -> abi.RandomC:
     return abi.RandomC(int(seed), at)
 
 
-def _drop(p: float, seed: int, counter: Optional[torch.Tensor], device) -> Optional[abi.DropoutArgsC]:
+def _check_p(p: float) -> None:
     if not (p >= 0 and int(p * 65536 + 0.5) < 65536):
-        raise ValueError(f"p must lie in [0, 1), got {p}")
-    return abi.DropoutArgsC(float(p), _seeded(seed, counter, device)) if p > 0 else None
+        raise ValueError(f"p must lie in [0, 1) to 16 bits, got {p}")
 
 
 def _ref(c):
@@ -113,12 +112,18 @@ class Mx4Vector:
     holds `codes` and, from the next multiple of 16 on, `scales`."""
 
     def __init__(self, n: int, buffer: torch.Tensor):
-        self.n, self.buffer = n, buffer
         if buffer.dtype != torch.uint8 or buffer.dim() != 1 or buffer.numel() != self.size_of(n) \
                 or not buffer.is_contiguous():
             raise ValueError(f"the buffer of {n} elements is {self.size_of(n)} contiguous bytes")
-        self.codes = buffer[:(n + 1) // 2]
-        self.scales = buffer[_scales_from(n):]
+        self.n, self.buffer = n, buffer
+
+    @property
+    def codes(self) -> torch.Tensor:
+        return self.buffer[:(self.n + 1) // 2]
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self.buffer[_scales_from(self.n):]
 
     @staticmethod
     def size_of(n: int) -> int:
@@ -140,14 +145,18 @@ class Mx4Vector:
 
 class Mx4Matrix:
     """A matrix [rows, cols] in 4 bits, rounded along its rows, in the layout
-    of the tensor cores (include/falcom_b200.h)."""
+    of the tensor cores (include/falcom_b200.h): `buffer`, one run of bytes,
+    holds `codes` and `scales`."""
 
-    def __init__(self, rows: int, cols: int, codes: torch.Tensor, scales: torch.Tensor):
-        self.rows, self.cols, self.codes, self.scales = rows, cols, codes, scales
-        for what, t, size in (("codes", codes, self.sizes_of(rows, cols)[0]), ("scales", scales, self.sizes_of(rows, cols)[1])):
-            if t.dtype != torch.uint8 or t.dim() != 1 or t.numel() != size or not t.is_contiguous() or t.device != codes.device:
-                raise ValueError(f"the {what} of {rows} x {cols} are {size} contiguous bytes")
-        self._c = abi.Mx4MatrixC(codes.data_ptr(), scales.data_ptr(), rows, cols)
+    def __init__(self, rows: int, cols: int, buffer: torch.Tensor):
+        codes, scales = self.sizes_of(rows, cols)
+        if buffer.dtype != torch.uint8 or buffer.dim() != 1 or buffer.numel() != codes + scales \
+                or not buffer.is_contiguous():
+            raise ValueError(f"the buffer of {rows} x {cols} is {codes + scales} contiguous bytes")
+        self.rows, self.cols, self.buffer = rows, cols, buffer
+        at = buffer.data_ptr()
+        self._c = abi.Mx4MatrixC(at, at + codes, rows, cols)
+        self._ref = ctypes.byref(self._c)
 
     @staticmethod
     def sizes_of(rows: int, cols: int) -> Tuple[int, int]:
@@ -157,9 +166,16 @@ class Mx4Matrix:
 
     @staticmethod
     def empty(rows: int, cols: int, device) -> "Mx4Matrix":
-        codes, scales = Mx4Matrix.sizes_of(rows, cols)
-        both = torch.empty(codes + scales, dtype=torch.uint8, device=device)
-        return Mx4Matrix(rows, cols, both[:codes], both[codes:])
+        """Room for a matrix (of a receiver, of a checkpoint)."""
+        return Mx4Matrix(rows, cols, torch.empty(sum(Mx4Matrix.sizes_of(rows, cols)), dtype=torch.uint8, device=device))
+
+    @property
+    def codes(self) -> torch.Tensor:
+        return self.buffer[:self.sizes_of(self.rows, self.cols)[0]]
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self.buffer[self.sizes_of(self.rows, self.cols)[0]:]
 
     @property
     def shape(self) -> Tuple[int, int]:
@@ -167,12 +183,12 @@ class Mx4Matrix:
 
     @property
     def device(self) -> torch.device:
-        return self.codes.device
+        return self.buffer.device
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         _check_type(dtype)
         out = torch.empty(self.rows, self.cols, dtype=dtype, device=self.device)
-        _done(_library().falcom_mx4_dequantize(ctypes.byref(self._c), out.data_ptr(), _TYPES[dtype], self.cols,
+        _done(_library().falcom_mx4_dequantize(self._ref, out.data_ptr(), _TYPES[dtype], self.cols,
                                                _stream(self.device)), "falcom_mx4_dequantize")
         return out
 
@@ -242,14 +258,13 @@ def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
     return x
 
 
-def _quantize(x: torch.Tensor, along: str, random, drop) -> Tuple[Optional[Mx4Matrix], Optional[Mx4Matrix]]:
+def _quantize(x: torch.Tensor, along: str, random) -> Tuple[Optional[Mx4Matrix], Optional[Mx4Matrix]]:
     rows, cols = x.shape
     by_rows = Mx4Matrix.empty(rows, cols, x.device) if along != "columns" else None
     by_cols = Mx4Matrix.empty(cols, rows, x.device) if along != "rows" else None
     _done(_library().falcom_mx4_quantize(x.data_ptr(), _TYPES[x.dtype], rows, cols, x.stride(0) if rows > 1 else cols,
-                                         _ref(random), _ref(drop), _ref(by_rows._c) if by_rows else None,
-                                         _ref(by_cols._c) if by_cols else None, _stream(x.device)),
-          "falcom_mx4_quantize")
+                                         _ref(random), None, by_rows._ref if by_rows else None,
+                                         by_cols._ref if by_cols else None, _stream(x.device)), "falcom_mx4_quantize")
     return by_rows, by_cols
 
 
@@ -261,7 +276,7 @@ def quantize(x: torch.Tensor, along: str = "rows", rounding: str = "nearest", se
     if along not in ("rows", "columns", "both"):
         raise ValueError(f"along is 'rows', 'columns' or 'both', got {along!r}")
     x = _rows(x, "x")
-    both = _quantize(x, along, _random(rounding, seed, counter, x.device), None)
+    both = _quantize(x, along, _random(rounding, seed, counter, x.device))
     return both if along == "both" else both[0] or both[1]
 
 
@@ -271,36 +286,42 @@ def product(a: Union[torch.Tensor, Mx4Matrix], b: Mx4Matrix, dtype: torch.dtype 
     nearest 4-bit values on the way; its leading dimensions stay."""
     if not isinstance(b, Mx4Matrix):
         raise TypeError("b is not an Mx4Matrix: quantize it")
-    lead = None
-    if isinstance(a, torch.Tensor):
-        lead = a.shape[:-1]
-        x = _rows(a, "a")
-        if x.shape[1] != b.cols:
-            raise ValueError(f"a has {x.shape[1]} columns, b {b.cols}")
-        _same_device(b.device, a=x)
-        a = _quantize(x, "rows", None, None)[0]
-    elif not isinstance(a, Mx4Matrix):
-        raise TypeError("a is neither a tensor nor an Mx4Matrix")
-    y = _product(a, b, dtype, None, out)
-    return y if lead is None or out is not None else y.view(*lead, b.rows)
+    if isinstance(a, Mx4Matrix):
+        return _product(a, b, dtype, out)
+    x = _rows(a, "a")
+    rows, cols = x.shape
+    if cols != b.cols:
+        raise ValueError(f"a has {cols} columns, b {b.cols}")
+    device = b.device
+    _same_device(device, a=x)
+    y = _out(rows, b, dtype, out, a.shape[:-1])
+    work = torch.empty(sum(Mx4Matrix.sizes_of(rows, cols)), dtype=torch.uint8, device=device)
+    _done(_library().falcom_mx4_product_of(x.data_ptr(), _TYPES[x.dtype], rows, x.stride(0) if rows > 1 else cols,
+                                           b._ref, y.data_ptr(), _TYPES[y.dtype], b.rows, work.data_ptr(),
+                                           _stream(device)), "falcom_mx4_product_of")
+    return y
 
 
-def _product(a: Mx4Matrix, b: Mx4Matrix, dtype: torch.dtype, drop, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+def _out(rows: int, b: Mx4Matrix, dtype: torch.dtype, out: Optional[torch.Tensor], lead) -> torch.Tensor:
+    if out is None:
+        _check_type(dtype)
+        return torch.empty((*lead, b.rows), dtype=dtype, device=b.device)
+    _check(out, "out")
+    if out.numel() != rows * b.rows or not out.is_contiguous():
+        raise ValueError(f"out must be {rows} x {b.rows} contiguous values, got {tuple(out.shape)} with strides "
+                         f"{out.stride()}")
+    _same_device(b.device, out=out)
+    torch.autograd.graph.increment_version(out)
+    return out
+
+
+def _product(a: Mx4Matrix, b: Mx4Matrix, dtype: torch.dtype, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     if a.cols != b.cols:
         raise ValueError(f"a has {a.cols} columns, b {b.cols}")
     _same_device(b.device, a=a)
-    if out is None:
-        _check_type(dtype)
-        out = torch.empty(a.rows, b.rows, dtype=dtype, device=b.device)
-    else:
-        _check(out, "out")
-        if out.numel() != a.rows * b.rows or not out.is_contiguous():
-            raise ValueError(f"out must be {a.rows} x {b.rows} contiguous values, got {tuple(out.shape)} with strides "
-                             f"{out.stride()}")
-        _same_device(b.device, out=out)
-        torch.autograd.graph.increment_version(out)
-    _done(_library().falcom_mx4_product(ctypes.byref(a._c), ctypes.byref(b._c), out.data_ptr(), _TYPES[out.dtype],
-                                        b.rows, _ref(drop), _stream(b.device)), "falcom_mx4_product")
+    out = _out(a.rows, b, dtype, out, (a.rows,))
+    _done(_library().falcom_mx4_product(a._ref, b._ref, out.data_ptr(), _TYPES[out.dtype], b.rows, None,
+                                        _stream(b.device)), "falcom_mx4_product")
     return out
 
 
@@ -314,39 +335,47 @@ def errors() -> int:
 # ------------------------------------------------------------------- layers
 
 class _Linear(torch.autograd.Function):
-    """y = Q(D(x)) Q(w)^T, dx = D'(Q(dy) Q(w^T)^T), dw = Q(dy^T) Q(D(x)^T)^T:
-    Q rounds along the summed dimension, the gradient at random, the rest to
-    the nearest; D is dropout.  Rounding counts as the identity in the
-    gradients.  What is kept for them is in 4 bits."""
+    """falcom_mx4_linear_forward and _backward.  Rounding counts as the
+    identity in the gradients; what is kept for them is in 4 bits."""
 
     @staticmethod
     def forward(ctx, x, w, p, seed, counter):
-        m = _rows(x, "x")
-        drop = _drop(p, seed, counter, m.device)
-        a, at = _quantize(m, "both" if ctx.needs_input_grad[1] else "rows", None, drop)
-        b, bt = _quantize(_rows(w, "weight"), "both" if ctx.needs_input_grad[0] else "rows", None, None)
-        ctx.p, ctx.seed, ctx.shapes, ctx.types = p, seed, (x.shape, w.shape), (x.dtype, w.dtype)
-        # the counter as it is now, whatever it is when the gradients are asked for
-        counter = counter.clone() if counter is not None else None
-        ctx.save_for_backward(counter, *(t for m in (at, bt) for t in ((m.codes, m.scales) if m else (None, None))))
-        return _product(a, b, x.dtype, None).view(*x.shape[:-1], w.shape[0])
+        lib, device = _library(), x.device
+        m, v = _rows(x, "x"), _rows(w, "weight")
+        (rows, cols), outs = m.shape, v.shape[0]
+        need_x, need_w = ctx.needs_input_grad[:2]
+        random = _seeded(seed, counter, device)
+        layer = abi.Mx4LinearC(rows, cols, outs, _TYPES[x.dtype], _TYPES[w.dtype], need_x, need_w, p, random)
+        ref = ctypes.byref(layer)
+        kept = torch.empty(lib.falcom_mx4_linear_kept_bytes(ref), dtype=torch.uint8, device=device)
+        work = torch.empty(lib.falcom_mx4_linear_work_bytes(ref, 0), dtype=torch.uint8, device=device)
+        y = torch.empty((*x.shape[:-1], outs), dtype=x.dtype, device=device)
+        _done(lib.falcom_mx4_linear_forward(ref, m.data_ptr(), m.stride(0) if rows > 1 else cols, v.data_ptr(),
+                                            v.stride(0) if outs > 1 else cols, y.data_ptr(), kept.data_ptr(),
+                                            work.data_ptr(), _stream(device)), "falcom_mx4_linear_forward")
+        if need_x or need_w:
+            # the counter as it is now, whatever it is when the gradients are asked for
+            ctx.save_for_backward(kept, counter.clone() if counter is not None else None)
+            ctx.layer, ctx.of = layer, (x.shape, x.dtype, w.shape, w.dtype)
+        return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        counter, a_codes, a_scales, b_codes, b_scales = ctx.saved_tensors
-        (*lead, k), (n, _) = ctx.shapes
-        g = _rows(dy, "the gradient")
-        t = g.shape[0]
+        lib, device, layer = _library(), dy.device, ctx.layer
+        kept, counter = ctx.saved_tensors
+        x_shape, x_type, w_shape, w_type = ctx.of
         need_x, need_w = ctx.needs_input_grad[:2]
-        along = "both" if need_x and need_w else "rows" if need_x else "columns"
-        by_rows, by_cols = _quantize(g, along, _seeded(ctx.seed, counter, g.device), None)
-        dx = dw = None
-        if need_x:
-            dx = _product(by_rows, Mx4Matrix(k, n, b_codes, b_scales), ctx.types[0],
-                          _drop(ctx.p, ctx.seed, counter, g.device)).view(*lead, k)
-        if need_w:
-            dw = _product(by_cols, Mx4Matrix(k, t, a_codes, a_scales), ctx.types[1], None)
+        g = _rows(dy, "the gradient")
+        layer.random.counter = counter.data_ptr() if counter is not None else None
+        ref = ctypes.byref(layer)
+        work = torch.empty(lib.falcom_mx4_linear_work_bytes(ref, 1), dtype=torch.uint8, device=device)
+        dx = torch.empty(x_shape, dtype=x_type, device=device) if need_x else None
+        dw = torch.empty(w_shape, dtype=w_type, device=device) if need_w else None
+        _done(lib.falcom_mx4_linear_backward(ref, g.data_ptr(), g.stride(0) if layer.rows > 1 else layer.outs,
+                                             kept.data_ptr(), dx.data_ptr() if need_x else None,
+                                             dw.data_ptr() if need_w else None, work.data_ptr(), _stream(device)),
+              "falcom_mx4_linear_backward")
         return dx, dw, None, None, None
 
 
@@ -361,5 +390,5 @@ def linear(x: torch.Tensor, weight: torch.Tensor, p: float = 0.0, seed: int = 0,
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} do not go together")
     _same_device(x.device, weight=weight)
-    _drop(p, seed, counter, x.device)
+    _check_p(p)
     return _Linear.apply(x, weight, float(p), int(seed), counter)

@@ -548,6 +548,40 @@ int falcom_mx4_dequantize(const falcom_mx4_matrix *m, void *out, int dtype, size
  * A sum over no columns is 0. */
 int falcom_mx4_product(const falcom_mx4_matrix *a, const falcom_mx4_matrix *b, void *out, int dtype, size_t ld,
                        const falcom_dropout_args *drop, void *stream);
+/* The same with a matrix that is not in 4 bits yet: x (rows x b->cols, rows
+ * `ld_x` elements apart) is rounded to the nearest along its rows into `work`,
+ * falcom_mx4_work_bytes(rows, b->cols) bytes on a 16-byte boundary. */
+size_t falcom_mx4_work_bytes(size_t rows, size_t cols);
+int falcom_mx4_product_of(const void *x, int x_type, size_t rows, size_t ld_x, const falcom_mx4_matrix *b, void *out,
+                          int dtype, size_t ld, void *work, void *stream);
+
+/* A layer's training step, y = D(x) weight^T with all factors in 4 bits.
+ * With Q rounding along the summed dimension and D dropout:
+ *   y  = Q(D(x)) Q(weight)^T                      (rows x outs, x's type)
+ *   dx = D'(Q*(dy) Q(weight^T)^T)                 (rows x cols, x's type)
+ *   dw = Q*(dy^T) Q(D(x)^T)^T                     (outs x cols, weight's type)
+ * Q rounds to the nearest, Q* at random (by `random`, by the places in dy),
+ * D' multiplies by the same mask and factor as D (p, by `random` too).
+ * forward rounds x and weight and leaves in `kept` what backward needs: the
+ * weight's columns if want_dx, x's columns if want_dw.  backward computes the
+ * gradients whose pointers are not NULL; `random` has to be what it was (the
+ * counter's value too).  x, weight and dy have rows `ld` elements apart, y, dx
+ * and dw are contiguous.  kept and work are device memory on 16-byte
+ * boundaries of the sizes given below (work may be shared with other calls
+ * on the same stream). */
+typedef struct falcom_mx4_linear {
+    size_t rows, cols, outs;
+    int x_type, weight_type;
+    int want_dx, want_dw;
+    double p;
+    falcom_random random;
+} falcom_mx4_linear;
+size_t falcom_mx4_linear_kept_bytes(const falcom_mx4_linear *layer);
+size_t falcom_mx4_linear_work_bytes(const falcom_mx4_linear *layer, int backward);
+int falcom_mx4_linear_forward(const falcom_mx4_linear *layer, const void *x, size_t ld_x, const void *weight,
+                              size_t ld_weight, void *y, void *kept, void *work, void *stream);
+int falcom_mx4_linear_backward(const falcom_mx4_linear *layer, const void *dy, size_t ld_dy, const void *kept, void *dx,
+                               void *dw, void *work, void *stream);
 /* 1 when a product on the current device gave up waiting for its own copies
  * (some seconds; its result is then not to be used), else 0; negative when
  * the device cannot be asked.  Waits for the device, so it does not belong

@@ -276,7 +276,7 @@ MC_EXPORT int falcom_mx4_dequantize(const falcom_mx4_matrix *m, void *out, int d
     if (rc) return rc;
     L.out = out;
     L.ld = (int64_t)ld;
-    return done(&c, prev, mc_launch_mx_dequantize(&L, dtype, stream));
+    return done(&c, prev, mc_launch_mx_dequantize(&L, dtype, sms, stream));
 }
 
 MC_EXPORT int falcom_mx4_product(const falcom_mx4_matrix *a, const falcom_mx4_matrix *b, void *out, int dtype,

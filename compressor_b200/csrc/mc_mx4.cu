@@ -180,6 +180,7 @@ __device__ __forceinline__ void store_up_to_8(T *p, const float *v, int n) {
 
 template <typename T, bool BASE, bool RANDOM>
 __global__ void __launch_bounds__(MX_TPB) k_mx_encode8(const __grid_constant__ mx_encode_launch L) {
+    mx_begin();
     mx_key key = {};
     if (RANDOM) key = mx_key_of(L.random);
     // whole warps: 4 lanes find a block's largest magnitude together
@@ -237,6 +238,7 @@ __global__ void __launch_bounds__(MX_TPB) k_mx_encode8(const __grid_constant__ m
 
 template <typename T, bool ADD>
 __global__ void __launch_bounds__(MX_TPB) k_mx_decode8(const __grid_constant__ mx_decode_launch L) {
+    mx_begin();
     const int64_t lanes = (L.n + 7) / 8, step = (int64_t)gridDim.x * MX_TPB;
     T *out = (T *)L.out;
     for (int64_t i = (int64_t)blockIdx.x * MX_TPB + threadIdx.x; i < lanes; i += step) {
@@ -270,6 +272,7 @@ __global__ void __launch_bounds__(MX_TPB) k_mx_decode8(const __grid_constant__ m
 
 template <typename T, bool BASE, bool RANDOM>
 __global__ void __launch_bounds__(MX_TPB) k_mx_encode(const __grid_constant__ mx_encode_launch L) {
+    mx_begin();
     const int lane = threadIdx.x & 31;
     const T *x = (const T *)L.x;
     mx_key key = {};
@@ -320,6 +323,7 @@ __global__ void __launch_bounds__(MX_TPB) k_mx_encode(const __grid_constant__ mx
 
 template <typename T, bool ADD>
 __global__ void __launch_bounds__(MX_TPB) k_mx_decode(const __grid_constant__ mx_decode_launch L) {
+    mx_begin();
     const int lane = threadIdx.x & 31;
     T *out = (T *)L.out;
     const int64_t chunks = (L.n + 255) / 256, step = (int64_t)gridDim.x * (MX_TPB / 32);
@@ -369,6 +373,7 @@ struct mx_tile {
 
 template <typename T, bool ROWS, bool COLS, bool RANDOM, bool DROP>
 __global__ void __launch_bounds__(MX_TPB, COLS ? 3 : 4) k_mx_quantize(const __grid_constant__ mx_quantize_launch L) {
+    mx_begin();
     typedef mx_tile<T, COLS, RANDOM> S;
     constexpr int W = 8 * sizeof(T) / 4;   // words of 8 elements
     extern __shared__ __align__(16) uint8_t s_tile[];
@@ -570,6 +575,7 @@ __global__ void __launch_bounds__(MX_TPB, COLS ? 3 : 4) k_mx_quantize(const __gr
 
 template <typename T>
 __global__ void __launch_bounds__(MX_TPB) k_mx_dequantize(const __grid_constant__ mx_dequantize_launch L) {
+    mx_begin();
     const int64_t words = (L.m.cols + 7) / 8, all = L.m.rows * words, step = (int64_t)gridDim.x * MX_TPB;
     for (int64_t i = (int64_t)blockIdx.x * MX_TPB + threadIdx.x; i < all; i += step) {
         const int64_t r = i / words, c = (i - r * words) * 8, k = c / MX_BLOCK;
@@ -595,6 +601,7 @@ __device__ __forceinline__ void drop_pair(const mx_dropout_launch &L, mx_bits w,
 
 template <typename T, bool RES>
 __global__ void __launch_bounds__(MX_TPB) k_mx_dropout(const __grid_constant__ mx_dropout_launch L) {
+    mx_begin();
     const mx_key key = mx_key_of(L.drop.random);
     const int64_t wide = mx_wide(L.cols), step = (int64_t)gridDim.x * MX_TPB;
     const int64_t first = (int64_t)blockIdx.x * MX_TPB + threadIdx.x;
@@ -648,7 +655,7 @@ static int grid_for(int64_t units, int per_cta, int sms, int per_sm) {
 }
 
 template <typename T>
-static void encode(const mx_encode_launch &L, int sms, cudaStream_t s) {
+static int encode(const mx_encode_launch &L, int sms, cudaStream_t s) {
     const int grid = grid_for((L.n + 255) / 256, MX_TPB / 32, sms, 8);
     void (*kern)(const mx_encode_launch);
     if (L.vectors) {
@@ -658,16 +665,16 @@ static void encode(const mx_encode_launch &L, int sms, cudaStream_t s) {
         if (L.base) kern = L.random.on ? k_mx_encode<T, true, true> : k_mx_encode<T, true, false>;
         else kern = L.random.on ? k_mx_encode<T, false, true> : k_mx_encode<T, false, false>;
     }
-    kern<<<grid, MX_TPB, 0, s>>>(L);
+    return mx_launch(kern, grid, MX_TPB, 0, 0, s, L);
 }
 
 template <typename T>
-static void decode(const mx_decode_launch &L, int sms, cudaStream_t s) {
+static int decode(const mx_decode_launch &L, int sms, cudaStream_t s) {
     const int grid = grid_for((L.n + 255) / 256, MX_TPB / 32, sms, 8);
     void (*kern)(const mx_decode_launch);
     if (L.vectors) kern = L.accumulate ? k_mx_decode8<T, true> : k_mx_decode8<T, false>;
     else kern = L.accumulate ? k_mx_decode<T, true> : k_mx_decode<T, false>;
-    kern<<<grid, MX_TPB, 0, s>>>(L);
+    return mx_launch(kern, grid, MX_TPB, 0, 0, s, L);
 }
 
 template <typename T, bool ROWS, bool COLS, bool RANDOM, bool DROP>
@@ -683,8 +690,7 @@ static int quantize_as(mx_quantize_launch L, cudaStream_t s) {
                                                    cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
     }
-    k_mx_quantize<T, ROWS, COLS, RANDOM, DROP><<<(unsigned)(x * y), MX_TPB, smem, s>>>(L);
-    return cudaSuccess;
+    return mx_launch(k_mx_quantize<T, ROWS, COLS, RANDOM, DROP>, x * y, MX_TPB, smem, 0, s, L);
 }
 
 template <typename T, bool RANDOM, bool DROP>
@@ -701,11 +707,10 @@ static int quantize(const mx_quantize_launch &L, cudaStream_t s) {
 }
 
 template <typename T>
-static void dropout(const mx_dropout_launch &L, int sms, cudaStream_t s) {
+static int dropout(const mx_dropout_launch &L, int sms, cudaStream_t s) {
     const int64_t units = L.vectors ? L.rows * (L.cols / 8) : L.rows * ((L.cols + 1) / 2);
     const int grid = grid_for(units, MX_TPB, sms, 32);
-    if (L.residual) k_mx_dropout<T, true><<<grid, MX_TPB, 0, s>>>(L);
-    else k_mx_dropout<T, false><<<grid, MX_TPB, 0, s>>>(L);
+    return mx_launch(L.residual ? k_mx_dropout<T, true> : k_mx_dropout<T, false>, grid, MX_TPB, 0, 0, s, L);
 }
 
 }  // namespace
@@ -713,42 +718,31 @@ static void dropout(const mx_dropout_launch &L, int sms, cudaStream_t s) {
 extern "C" uint32_t mc_mx_hash(uint32_t x) { return mx_mix(x); }
 
 extern "C" int mc_launch_mx_encode(const mx_encode_launch *L, int type, int sms, void *stream) {
-    if (type == FALCOM_TYPE_F32) encode<float>(*L, sms, (cudaStream_t)stream);
-    else if (type == FALCOM_TYPE_BF16) encode<__nv_bfloat16>(*L, sms, (cudaStream_t)stream);
-    else encode<__half>(*L, sms, (cudaStream_t)stream);
-    return cudaGetLastError();
+    if (type == FALCOM_TYPE_F32) return encode<float>(*L, sms, (cudaStream_t)stream);
+    if (type == FALCOM_TYPE_BF16) return encode<__nv_bfloat16>(*L, sms, (cudaStream_t)stream);
+    return encode<__half>(*L, sms, (cudaStream_t)stream);
 }
 
 extern "C" int mc_launch_mx_decode(const mx_decode_launch *L, int type, int sms, void *stream) {
-    if (type == FALCOM_TYPE_F32) decode<float>(*L, sms, (cudaStream_t)stream);
-    else if (type == FALCOM_TYPE_BF16) decode<__nv_bfloat16>(*L, sms, (cudaStream_t)stream);
-    else decode<__half>(*L, sms, (cudaStream_t)stream);
-    return cudaGetLastError();
+    if (type == FALCOM_TYPE_F32) return decode<float>(*L, sms, (cudaStream_t)stream);
+    if (type == FALCOM_TYPE_BF16) return decode<__nv_bfloat16>(*L, sms, (cudaStream_t)stream);
+    return decode<__half>(*L, sms, (cudaStream_t)stream);
 }
 
 extern "C" int mc_launch_mx_quantize(const mx_quantize_launch *L, int type, void *stream) {
-    int e;
-    if (type == FALCOM_TYPE_F32) e = quantize<float>(*L, (cudaStream_t)stream);
-    else if (type == FALCOM_TYPE_BF16) e = quantize<__nv_bfloat16>(*L, (cudaStream_t)stream);
-    else e = quantize<__half>(*L, (cudaStream_t)stream);
-    const int late = cudaGetLastError();
-    return e ? e : late;
+    if (type == FALCOM_TYPE_F32) return quantize<float>(*L, (cudaStream_t)stream);
+    if (type == FALCOM_TYPE_BF16) return quantize<__nv_bfloat16>(*L, (cudaStream_t)stream);
+    return quantize<__half>(*L, (cudaStream_t)stream);
 }
 
-extern "C" int mc_launch_mx_dequantize(const mx_dequantize_launch *L, int type, void *stream) {
-    const int64_t all = L->m.rows * ((L->m.cols + 7) / 8), most = 148 * 64;
-    const int64_t want = (all + MX_TPB - 1) / MX_TPB;
-    const int grid = (int)(want < most ? want : most);
-    cudaStream_t s = (cudaStream_t)stream;
-    if (type == FALCOM_TYPE_F32) k_mx_dequantize<float><<<grid, MX_TPB, 0, s>>>(*L);
-    else if (type == FALCOM_TYPE_BF16) k_mx_dequantize<__nv_bfloat16><<<grid, MX_TPB, 0, s>>>(*L);
-    else k_mx_dequantize<__half><<<grid, MX_TPB, 0, s>>>(*L);
-    return cudaGetLastError();
+extern "C" int mc_launch_mx_dequantize(const mx_dequantize_launch *L, int type, int sms, void *stream) {
+    const int grid = grid_for(L->m.rows * ((L->m.cols + 7) / 8), MX_TPB, sms, 8);
+    return mx_launch(type == FALCOM_TYPE_F32 ? k_mx_dequantize<float> : type == FALCOM_TYPE_BF16 ? k_mx_dequantize<__nv_bfloat16>
+                     : k_mx_dequantize<__half>, grid, MX_TPB, 0, 0, (cudaStream_t)stream, *L);
 }
 
 extern "C" int mc_launch_mx_dropout(const mx_dropout_launch *L, int type, int sms, void *stream) {
-    if (type == FALCOM_TYPE_F32) dropout<float>(*L, sms, (cudaStream_t)stream);
-    else if (type == FALCOM_TYPE_BF16) dropout<__nv_bfloat16>(*L, sms, (cudaStream_t)stream);
-    else dropout<__half>(*L, sms, (cudaStream_t)stream);
-    return cudaGetLastError();
+    if (type == FALCOM_TYPE_F32) return dropout<float>(*L, sms, (cudaStream_t)stream);
+    if (type == FALCOM_TYPE_BF16) return dropout<__nv_bfloat16>(*L, sms, (cudaStream_t)stream);
+    return dropout<__half>(*L, sms, (cudaStream_t)stream);
 }

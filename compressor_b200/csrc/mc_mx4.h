@@ -93,7 +93,7 @@ typedef struct {
 int mc_launch_mx_encode(const mx_encode_launch *L, int type, int sms, void *stream);
 int mc_launch_mx_decode(const mx_decode_launch *L, int type, int sms, void *stream);
 int mc_launch_mx_quantize(const mx_quantize_launch *L, int type, void *stream);
-int mc_launch_mx_dequantize(const mx_dequantize_launch *L, int type, void *stream);
+int mc_launch_mx_dequantize(const mx_dequantize_launch *L, int type, int sms, void *stream);
 int mc_launch_mx_product(const mx_product_launch *L, int type, int sms, void *stream);
 int mc_launch_mx_dropout(const mx_dropout_launch *L, int type, int sms, void *stream);
 int mc_mx_errors(uint32_t *word);

@@ -12,6 +12,34 @@
 
 namespace {
 
+// Programmatic dependent launch: a kernel may start while its predecessor on
+// the stream finishes; it waits for it (mx_begin) before it touches memory.
+__device__ __forceinline__ void mx_begin() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+// `cluster` > 0: of so many CTAs.
+template <typename... P, typename... A>
+static cudaError_t mx_launch(void (*kern)(P...), int64_t grid, int threads, size_t smem, int cluster, cudaStream_t s, const A &...args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = (unsigned)cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = cluster > 0 ? 2 : 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+    const cudaError_t late = cudaGetLastError();
+    return e != cudaSuccess ? e : late;
+}
+
 __device__ __forceinline__ float mx_f32(float x) { return x; }
 __device__ __forceinline__ float mx_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float mx_f32(__half x) { return __half2float(x); }

@@ -181,6 +181,7 @@ __global__ void __launch_bounds__(MX_THREADS) k_mx_product(const __grid_constant
     __syncthreads();
     tc_after_sync();
     const uint32_t tmem = s_tmem;
+    mx_begin();
 
     if (warp == 4 && elect_one()) {
         const int64_t rows_b = mx_rows8(L.b.rows), rows_a = mx_rows8(L.a.rows);
@@ -497,6 +498,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mx_wide_cfg::THREADS
     cluster_sync();
     tc_after_sync();
     const uint32_t tmem = s_tmem;
+    mx_begin();
 
     if (warp == COPIES) {
         // One lane for each of a panel's four copies: codes of a and of b, scales of a and of b.  Boxes are whole: what
@@ -689,8 +691,7 @@ static int product_wide(const mx_product_launch &L, int sms, cudaStream_t s) {
         !map_rows(encode, &M.a_scales, L.a.scales, panels * ((L.a.rows + 127) / 128), 256, 1) ||
         !map_rows(encode, &M.b_scales, L.b.scales, panels * ((L.b.rows + 127) / 128), 256, 2))
         return cudaErrorNotSupported;
-    kern<<<(unsigned)(2 * pairs), C::THREADS, C::SMEM, s>>>(L, M, (int)tiles_n, (int)tiles);
-    return cudaGetLastError();
+    return mx_launch(kern, 2 * pairs, C::THREADS, C::SMEM, 0, s, L, M, (int)tiles_n, (int)tiles);
 }
 
 template <typename T, int BN, bool DROP>
@@ -704,20 +705,7 @@ static int product_as(const mx_product_launch &L, int sms, cudaStream_t s) {
     int split = 1;
     while (split < 8 && tiles * split * 2 <= sms && split * 2 <= panels) split *= 2;
     if (tiles * split > 0x7FFFFFFF) return cudaErrorInvalidValue;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(tiles * split));
-    cfg.blockDim = dim3(MX_THREADS);
-    cfg.dynamicSmemBytes = C::SMEM;
-    cfg.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)split;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kern, L, (int)tiles_n, split);
-    const cudaError_t late = cudaGetLastError();
-    return e != cudaSuccess ? e : late;
+    return mx_launch(kern, tiles * split, MX_THREADS, C::SMEM, split, s, L, (int)tiles_n, split);
 }
 
 template <typename T, bool DROP>

@@ -50,7 +50,7 @@ def _check(t, what: str) -> None:
         raise ValueError(f"{what} is {t.dtype}: float32, bfloat16 or float16 is wanted")
     if not t.is_cuda:
         raise ValueError(f"{what} is on {t.device}: a CUDA device is wanted")
-    if t.layout != torch.strided or t.is_neg():
+    if t.layout is not torch.strided or t.is_neg():
         raise ValueError(f"{what} does not hold its values as they are ({t.layout})")
 
 
@@ -61,7 +61,7 @@ def _check_type(dtype) -> None:
 
 def _same_device(device, **others) -> None:
     for what, t in others.items():
-        if t is not None and t.device != device:
+        if t.device != device:
             raise ValueError(f"{what} is on {t.device}, the rest of the call on {device}")
 
 
@@ -244,8 +244,10 @@ def decode(sent: Mx4Vector, out: Optional[torch.Tensor] = None, weight: float = 
 # ----------------------------------------------------------------- matrices
 
 def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
-    """x as a matrix whose rows are runs of memory."""
+    """x as a matrix whose rows are runs of memory (for its address alone)."""
     _check(x, what)
+    if x.dim() == 2 and x.is_contiguous():
+        return x
     if x.dim() < 1:
         raise ValueError(f"{what} has no dimensions")
     # (no reshape to -1: a last dimension of 0 leaves the rows undetermined)

@@ -455,7 +455,7 @@ MC_EXPORT int falcom_dropout(const void *x, const void *residual, void *y, int d
                              const falcom_dropout_args *drop, void *stream) {
     static const char *who = "falcom_dropout";
     if (!drop || !known_type(dtype)) return invalid(who, "no arguments, or an unknown type");
-    if (rows > MX_MOST || cols > MX_MOST || rows * cols > MX_ELEMENTS) return invalid(who, "too many rows or columns");
+    if (rows > 0 && cols > MX_ELEMENTS / rows) return invalid(who, "too many elements");
     mx_call c;
     mx_dropout_launch L;
     memset(&L, 0, sizeof(L));

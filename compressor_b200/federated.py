@@ -8,13 +8,14 @@ instance with the weighted aggregate fused into the decode
 (``falcom_set_aggregate``), and one sum all-reduce of the flat aggregate over
 NCCL finishes the global update.
 
-Everything here but PeerAggregate and ServerAdamW is plain host logic (which clients a rank
-owns, their weights, the aggregate layout and the collective); it runs the
-same under the ``gloo`` backend on CPU tensors.  PeerAggregate maps the
+Everything here but PeerAggregate, ServerAdamW and Downlink is plain host logic
+(which clients a rank owns, their weights, the aggregate layout and the
+collectives); it runs the same under the ``gloo`` backend on CPU tensors.  PeerAggregate maps the
 aggregate buffers between the ranks' GPUs for the two NVLink peer-memory
 sums (the reduce-scatter fused into the decoder, or the one-shot in-place
 all-reduce kernel); ServerAdamW takes an optimiser step on the global model
-with the finished aggregate.
+with the finished aggregate, and Downlink sends the result to the clients in 4
+bits.
 """
 from __future__ import annotations
 
@@ -431,6 +432,64 @@ class ServerAdamW:
         if self.norm is not None:
             self.norm.close()
         self.opt.close()
+
+
+class Downlink:
+    """The way down in 4 bits: the server sends its clients the difference of
+    its weights from what they hold, and follows what they then hold.
+
+    `weights` is the server's flat model on the GPU (float32, bfloat16 or
+    float16; ServerAdamW's, say), `held` (float32) the clients' copy as the
+    server knows it: the weights of the moment by default, for clients that
+    got them in full.  What one round rounds away is part of the next one's
+    difference, so clients stay within one rounding of the server.  Lay tensors
+    out with AggregateLayout.of(..., align=32) or a multiple: 32 consecutive
+    elements share a scale.
+
+        down = Downlink(weights)
+        sent = down.send()                     # a round
+        broadcast(sent, dist)                  # one run of bytes
+        Downlink.receive(sent, mine)           # a client: its float32 copy
+
+    rounding: "nearest", or "random" (from `seed` and the round's number,
+    which is on the device: send() may be captured in a CUDA graph).  After a
+    restart go on with the saved `held` and `round`.  A block in which a
+    difference is infinite or NaN arrives as NaN and stays so: send the model
+    in full then, and make a new Downlink."""
+
+    def __init__(self, weights, held=None, rounding: str = "nearest", seed: int = 0):
+        import torch
+        from . import mx4
+        self._mx4 = mx4
+        mx4._check(weights, "weights")
+        mx4._random(rounding, seed, None, weights.device)
+        self.weights = weights.detach()
+        if held is None:
+            held = self.weights.float() if self.weights.dtype != torch.float32 else self.weights.clone()
+        elif held.dtype != torch.float32 or held.numel() != weights.numel():
+            raise ValueError(f"held must be {weights.numel()} float32 values, got {held.dtype} {tuple(held.shape)}")
+        self.held, self.rounding, self.seed = held, rounding, seed
+        self.round = torch.zeros(1, dtype=torch.int64, device=weights.device)
+
+    def send(self):
+        """The difference (mx4.Mx4Vector), queued on the current stream; held
+        is brought forward by it."""
+        sent = self._mx4.encode(self.weights, base=self.held, rounding=self.rounding, seed=self.seed, counter=self.round)
+        self.round += 1
+        return sent
+
+    @staticmethod
+    def receive(sent, weights):
+        """Adds what was sent to a client's weights (returned)."""
+        from . import mx4
+        return mx4.decode(sent, out=weights, accumulate=True)
+
+
+def broadcast(sent, dist, src: int = 0, group=None) -> None:
+    """A 4-bit vector or matrix to every rank: those other than `src` pass an
+    empty one of the same size (mx4.Mx4Vector.empty)."""
+    if dist is not None and dist.is_initialized() and dist.get_world_size(group) > 1:
+        dist.broadcast(sent.buffer, src=src, group=group)
 
 
 class _DeviceFloats:

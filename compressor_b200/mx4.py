@@ -18,7 +18,10 @@ Calls queue work on the device's current stream and may be captured in a CUDA
 graph.  Random rounding and dropout are functions of (seed, counter, place):
 the same arguments give the same bits.  In a graph that is replayed a new seed
 has to come from the device: `counter`, an int64 tensor that the caller counts
-up, is read when the work runs.
+up, is read when the work runs.  As for any backward pass, torch can capture
+linear's and dropout's only while no eager autograd graph of the same leaves is
+alive (its nodes belong to another stream, and the capture ends with an
+error).
 """
 from __future__ import annotations
 

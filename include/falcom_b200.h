@@ -461,7 +461,8 @@ void falcom_adamw_destroy(falcom_adamw *plan);
  * which stands for 2^(s - 127): the smallest such power (2^-127 at least)
  * with which no magnitude of the block is above 6 times the scale.  An
  * element is 4 bits, sign above a magnitude code 0..7 for 0, 0.5, 1, 1.5, 2,
- * 3, 4, 6 (times the scale).  No value is clipped.  A block with an infinity
+ * 3, 4, 6 (times the scale).  No value is clipped (what is above the range
+ * of the type it is read back in becomes infinity there).  A block with an infinity
  * or NaN gets the scale byte 255, codes 0, and reads back as NaN throughout.
  * Elements are taken as float32 values of their type.  Rounding is to the
  * nearest value, ties to the even code; or, when a falcom_random is given, up

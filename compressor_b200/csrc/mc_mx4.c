@@ -109,6 +109,7 @@ static void random_of(mx_call *c, mx_random *out, const falcom_random *r, uint32
     out->key = mc_mx_hash(mc_mx_hash((uint32_t)r->seed ^ purpose) ^ (uint32_t)(r->seed >> 32));
     out->counter = r->counter;
     out->on = 1;
+    mc_mx_key(out);
 }
 
 /* p in [0, 1) that is not 1 after rounding to 16 bits; on only where something is dropped */
@@ -147,7 +148,7 @@ MC_EXPORT int falcom_mx4_encode(const void *x, int dtype, size_t n, float *base,
     L.codes = (uint8_t *)codes;
     L.scales = (uint8_t *)scales;
     L.vectors = (((uintptr_t)x | (uintptr_t)base) & 15) == 0;
-    return done(&c, prev, mc_launch_mx_encode(&L, dtype, sms, stream));
+    return done(&c, prev, mc_launch_mx_encode(&L, dtype, stream));
 }
 
 MC_EXPORT int falcom_mx4_decode(const void *codes, const void *scales, size_t n, float weight, int accumulate,
@@ -172,7 +173,7 @@ MC_EXPORT int falcom_mx4_decode(const void *codes, const void *scales, size_t n,
     L.weight = weight;
     L.accumulate = accumulate != 0;
     L.vectors = ((uintptr_t)out & 15) == 0;
-    return done(&c, prev, mc_launch_mx_decode(&L, dtype, sms, stream));
+    return done(&c, prev, mc_launch_mx_decode(&L, dtype, stream));
 }
 
 static int matrix_size_ok(size_t rows, size_t cols) { return rows > 0 && cols > 0 && rows <= MX_MOST && cols <= MX_MOST; }
@@ -240,8 +241,8 @@ MC_EXPORT int falcom_mx4_quantize(const void *x, int dtype, size_t rows, size_t 
     if ((along_rows && (along_rows->rows != rows || along_rows->cols != cols)) ||
         (along_cols && (along_cols->rows != cols || along_cols->cols != rows)))
         return invalid(who, "a result has other sizes than x");
-    mx_random r = {0};
-    mx_drop d = {{0}, 0, 0};
+    mx_random r = {0, 0, NULL, 0, 0};
+    mx_drop d = {{0, 0, NULL, 0, 0}, 0, 0};
     mx_matrix by_rows, by_cols;
     mx_call c;
     begin(&c, who);
@@ -285,7 +286,7 @@ MC_EXPORT int falcom_mx4_product(const falcom_mx4_matrix *a, const falcom_mx4_ma
     if (!a || !b || !known_type(dtype)) return invalid(who, "a factor is missing, or an unknown type");
     if (a->cols != b->cols) return invalid(who, "the factors have different numbers of columns");
     if (a->rows > MX_MOST || b->rows > MX_MOST || a->cols > MX_MOST) return invalid(who, "too many rows or columns");
-    mx_drop d = {{0}, 0, 0};
+    mx_drop d = {{0, 0, NULL, 0, 0}, 0, 0};
     mx_matrix ma, mb;
     mx_call c;
     begin(&c, who);
@@ -380,7 +381,7 @@ MC_EXPORT int falcom_mx4_linear_forward(const falcom_mx4_linear *l, const void *
     const size_t x_bytes = no_x ? 0 : extent(l->rows, l->cols, ld_x, xs), w_bytes = no_w ? 0 : extent(l->outs, l->cols, ld_weight, ws);
     if ((!no_x && x_bytes == 0) || (!no_w && w_bytes == 0) || l->rows * l->outs > MX_ELEMENTS)
         return invalid(who, "rows of x or of the weight overlap, or sizes are out of range");
-    mx_drop d = {{0}, 0, 0};
+    mx_drop d = {{0, 0, NULL, 0, 0}, 0, 0};
     mx_call c;
     begin(&c, who);
     if (!layer_drop(&c, &d, l)) return invalid(who, "p must lie in [0, 1)");
@@ -413,8 +414,8 @@ MC_EXPORT int falcom_mx4_linear_backward(const falcom_mx4_linear *l, const void 
     const size_t dy_bytes = none ? 0 : extent(l->rows, l->outs, ld_dy, xs);
     if ((!none && dy_bytes == 0) || l->rows * l->cols > MX_ELEMENTS || l->outs * l->cols > MX_ELEMENTS)
         return invalid(who, "rows of dy overlap, or sizes are out of range");
-    mx_random r = {0};
-    mx_drop d = {{0}, 0, 0};
+    mx_random r = {0, 0, NULL, 0, 0};
+    mx_drop d = {{0, 0, NULL, 0, 0}, 0, 0};
     mx_call c;
     begin(&c, who);
     if (!layer_drop(&c, &d, l)) return invalid(who, "p must lie in [0, 1)");

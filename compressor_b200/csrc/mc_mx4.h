@@ -20,11 +20,12 @@ extern "C" {
 #define MX_GROUP 128                /* rows whose scales lie together */
 #define MX_TYPES 3
 
-/* Random bits of one purpose; counter NULL counts as 0. */
+/* Random bits of one purpose. */
 typedef struct {
     uint32_t key;              /* hash of purpose and seed */
     int32_t on;
-    const int64_t *counter;    /* device memory */
+    const int64_t *counter;    /* device memory; NULL counts as 0, and then */
+    uint32_t a, b;             /* the key's two words */
 } mx_random;
 
 typedef struct {
@@ -90,14 +91,15 @@ typedef struct {
 } mx_dropout_launch;
 
 /* All return a CUDA error code (0: queued). */
-int mc_launch_mx_encode(const mx_encode_launch *L, int type, int sms, void *stream);
-int mc_launch_mx_decode(const mx_decode_launch *L, int type, int sms, void *stream);
+int mc_launch_mx_encode(const mx_encode_launch *L, int type, void *stream);
+int mc_launch_mx_decode(const mx_decode_launch *L, int type, void *stream);
 int mc_launch_mx_quantize(const mx_quantize_launch *L, int type, void *stream);
 int mc_launch_mx_dequantize(const mx_dequantize_launch *L, int type, int sms, void *stream);
 int mc_launch_mx_product(const mx_product_launch *L, int type, int sms, void *stream);
 int mc_launch_mx_dropout(const mx_dropout_launch *L, int type, int sms, void *stream);
 int mc_mx_errors(uint32_t *word);
 uint32_t mc_mx_hash(uint32_t x);
+void mc_mx_key(mx_random *r);   /* a and b of key and counter 0 */
 
 #ifdef __cplusplus
 }

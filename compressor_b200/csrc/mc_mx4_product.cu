@@ -308,8 +308,8 @@ struct mx_wide_cfg {
     static constexpr int BN = 256, THREADS = 320;                    // warps 0 to 7: results; 8: copies; 9: instructions
     static constexpr int A_BYTES = 128 * 128, B_BYTES = BN / 2 * 128;
     static constexpr int STAGE = A_BYTES + B_BYTES + 1024 + 2048, STAGES = 5;
-    static constexpr int PITCH = 128 + 16, OUT = 32 * PITCH;         // a warp's part of the results: 32 rows, 128 bytes each
-    static constexpr int SMEM = STAGES * STAGE + 8 * OUT + 1024;
+    static constexpr int PITCH = 256 + 16, OUT = 32 * PITCH;         // two warps' part of the results: 32 rows, 256 bytes each
+    static constexpr int SMEM = STAGES * STAGE + 4 * OUT + 1024;
     static constexpr int SECOND = 128, SCALES_AT = 384, SCALES = 24; // columns: a stage's scales have their own
     static constexpr uint32_t IDESC = 1u << 7 | 1u << 10 | (uint32_t)(BN / 8) << 17 | 1u << 23 | 2u << 27;
     static_assert(SMEM <= 227 * 1024 && SCALES_AT + STAGES * SCALES <= 512 && SECOND + BN <= SCALES_AT, "");
@@ -362,6 +362,8 @@ __device__ __forceinline__ uint4 ld_shared16(uint32_t at) {
     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at) : "memory");
     return r;
 }
+__device__ __forceinline__ void bar_pair(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+
 // 16 bytes of results.
 __device__ __forceinline__ uint4 pack16(const float *v, float) {
     return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
@@ -392,29 +394,30 @@ __device__ __forceinline__ uint4 joined(uint4 a, uint4 b, uint32_t from) {
                       __byte_perm(w[3], w[4], sel));
 }
 
-// A warp's 32 rows of up to 128 bytes (`count` elements) from shared memory to
-// `out` (of its first row).  8 lanes have a row, 16 bytes each.  A row that
-// does not begin on a 16-byte boundary leaves in the 7 whole pieces that lie
-// in it, put together from two, and 16 / SIZE elements at its two ends, one a
-// lane.
+// Every other of 32 rows of up to 256 bytes (`count` elements) from shared
+// memory to `out` (of the first row), from row `first` (0 or 1) on.  16 lanes
+// have a row, 16 bytes each.  A row that does not begin on a 16-byte boundary
+// leaves in the 15 whole pieces that lie in it, put together from two, and 16 /
+// SIZE elements at its two ends, one a lane (8192 x 50257 x 1024 to bf16: 304
+// us; with 4-byte stores of whole rows 750, on boundaries 225, at the rate of
+// a fill 213).
 template <typename T>
-__device__ __forceinline__ void rows_out(uint32_t buf, uint8_t *out, int64_t ld_bytes, int rows, int count, int lane, bool even) {
-    constexpr int SIZE = sizeof(T), PITCH = mx_wide_cfg::PITCH;
-    const int h = lane & 7;
-    uint8_t *g = out + (lane >> 3) * ld_bytes;
-    uint32_t at = buf + (lane >> 3) * PITCH;
+__device__ __forceinline__ void rows_out(uint32_t buf, uint8_t *out, int64_t ld_bytes, int rows, int count, int first, int lane, bool even) {
+    constexpr int SIZE = sizeof(T), PITCH = mx_wide_cfg::PITCH, BATCH = 4;
+    const int h = lane & 15, r0 = first + 2 * (lane >> 4);   // rows r0, r0 + 4, ...
+    uint8_t *g = out + r0 * ld_bytes;
+    uint32_t at = buf + r0 * PITCH;
     // (all loads of a batch before its stores: one after the other they would wait for each other)
-    if (even && count * SIZE == 128) {
+    if (even && count * SIZE == 256) {
         uint4 v[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) v[i] = ld_shared16(at + 4 * i * PITCH + 16 * h);
 #pragma unroll
         for (int i = 0; i < 8; i++, g += 4 * ld_bytes)
-            if (4 * i + (lane >> 3) < rows) *(uint4 *)(g + 16 * h) = v[i];
-    } else if (count * SIZE == 128) {
-        constexpr int BATCH = 4;
+            if (r0 + 4 * i < rows) *(uint4 *)(g + 16 * h) = v[i];
+    } else if (count * SIZE == 256) {
 #pragma unroll 1
-        for (int r = lane >> 3; r < rows + (lane >> 3); r += 4 * BATCH, at += 4 * BATCH * PITCH) {
+        for (int r = r0; r < 32; r += 4 * BATCH, at += 4 * BATCH * PITCH) {
             uint4 now[BATCH], last[BATCH];
             uint32_t end[BATCH], off[BATCH];
 #pragma unroll
@@ -422,27 +425,26 @@ __device__ __forceinline__ void rows_out(uint32_t buf, uint8_t *out, int64_t ld_
                 const uint32_t row = at + 4 * i * PITCH;
                 off[i] = ((uint32_t)(uintptr_t)g + 4 * i * (uint32_t)ld_bytes) & 15;
                 now[i] = ld_shared16(row + 16 * h);
-                last[i] = ld_shared16(row + 16 * h - (h ? 16 : 0));
+                last[i] = ld_shared16(row + 16 * h - (h && off[i] ? 16 : 0));   // (a row that is on a boundary: itself)
                 // the elements at the ends: 16 - off bytes of them in front
-                const uint32_t e = row + h * SIZE + (h * SIZE < 16 - off[i] ? 0 : 112);
+                const uint32_t e = row + (h * SIZE & 15) + (h * SIZE < 16 - off[i] ? 0 : 240);
                 if (SIZE == 4) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(end[i]) : "r"(e) : "memory");
                 else asm volatile("{\n\t.reg .b16 x;\n\tld.shared.b16 x, [%1];\n\tcvt.u32.u16 %0, x;\n\t}" : "=r"(end[i]) : "r"(e) : "memory");
             }
 #pragma unroll
-            for (int i = 0; i < BATCH; i++, g += 4 * ld_bytes) {
-                if (r + 4 * i >= rows) continue;
+            for (int i = 0; i < BATCH; i++, g += 4 * ld_bytes) {   // (no branches: the two rows of a warp may differ)
+                const bool in = r + 4 * i < rows;
                 const uint4 v = joined(last[i], now[i], 16 - off[i]);
-                if (off[i] == 0) *(uint4 *)(g + 16 * h) = now[i];
-                else if (h > 0) *(uint4 *)(g + 16 * h - off[i]) = v;
-                if (off[i] != 0 && h * SIZE < 16) {
-                    uint8_t *e = g + h * SIZE + (h * SIZE < 16 - off[i] ? 0 : 112);
+                if (in && (h > 0 || off[i] == 0)) *(uint4 *)(g + (int)(16 * h - off[i])) = v;
+                uint8_t *e = g + h * SIZE + (h * SIZE < 16 - off[i] ? 0 : 240);
+                if (in && off[i] != 0 && h * SIZE < 16) {
                     if (SIZE == 4) *(uint32_t *)e = end[i];
                     else *(uint16_t *)e = (uint16_t)end[i];
                 }
             }
         }
     } else {   // the last columns of the matrix
-        for (int r = 0; r < rows; r++)
+        for (int r = first; r < rows; r += 2)
             for (int i = lane; i < count; i += 32) {
                 if (SIZE == 4) {
                     uint32_t v;
@@ -591,7 +593,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mx_wide_cfg::THREADS
     __syncwarp();
     if (warp < COPIES) {
         const int set = warp >> 2, quarter = warp & 3;
-        const uint32_t buf = smem + C::STAGES * C::STAGE + warp * C::OUT;
+        const uint32_t buf = smem + C::STAGES * C::STAGE + quarter * C::OUT;
         const int64_t ld_bytes = L.ld * (int64_t)sizeof(T), wide = mx_wide(L.b.rows);
         const bool even = (((uintptr_t)L.out | (uintptr_t)ld_bytes) & 15) == 0;
         mx_key key = {};
@@ -604,17 +606,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mx_wide_cfg::THREADS
             if (!s_failed && !mbar_wait(smem_u32(&s_done[count & 1]), count >> 1 & 1, 20)) s_failed = 1;
             tc_after_sync();
             const uint32_t mine = tmem + (count & 1) * C::SECOND + ((uint32_t)(32 * quarter) << 16);
-            // both sets begin with half of the overlap: columns 128 on of even tiles, the first 128 of odd ones
+            // first the overlap: columns 128 on of even tiles, the first 128 of odd ones
             for (int k = 0; k < 2 * PARTS; k++) {
-                const int c = 64 * set + ((k < PARTS) == ((count & 1) == 0) ? 128 : 0) + k % PARTS * CHUNK;
-                const bool some = c < columns && rows > 0;
+                const int both = ((k < PARTS) == ((count & 1) == 0) ? 128 : 0) + k % PARTS * 2 * CHUNK, c = both + set * CHUNK;
+                const bool some = both < columns && rows > 0;   // the same for both warps
                 float v[CHUNK];
                 if (some) {
 #pragma unroll
                     for (int j = 0; j < CHUNK; j += 16) tc_ld16(mine + c + j, (uint32_t *)v + j);
                     tc_wait_ld();
                 }
-                if (k == PARTS - 1) {   // read, and all of the tile before
+                if (k == PARTS - 1) {   // the overlap is read, and all of the tile before
                     tc_before_sync();
                     __syncwarp();
                     if (lane == 0) mbar_arrive_first(smem_u32(&s_free[count & 1]));
@@ -631,11 +633,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mx_wide_cfg::THREADS
                         v[j + 1] = w.high < L.drop.threshold ? 0.0f : v[j + 1] * L.drop.factor;
                     }
                 }
-                __syncwarp();   // the last part has left the buffer
+                bar_pair(1 + quarter);   // the last part has left the buffer
 #pragma unroll
-                for (int j = 0; j < CHUNK; j += E) st_shared16(buf + lane * C::PITCH + j * sizeof(T), pack16(v + j, T()));
-                __syncwarp();
-                if (!s_failed) rows_out<T>(buf, out + c * (int64_t)sizeof(T), ld_bytes, rows, min(CHUNK, columns - c), lane, even);
+                for (int j = 0; j < CHUNK; j += E) st_shared16(buf + lane * C::PITCH + (set * CHUNK + j) * sizeof(T), pack16(v + j, T()));
+                bar_pair(1 + quarter);
+                if (!s_failed)
+                    rows_out<T>(buf, out + both * (int64_t)sizeof(T), ld_bytes, rows, min(2 * CHUNK, columns - both), set, lane, even);
             }
         }
     }

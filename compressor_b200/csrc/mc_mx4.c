@@ -317,7 +317,13 @@ static mx_matrix matrix_in(uint8_t **at, size_t rows, size_t cols) {
     return m;
 }
 
-MC_EXPORT size_t falcom_mx4_work_bytes(size_t rows, size_t cols) { return matrix_bytes(rows, cols); }
+static int rounds_inside(size_t rows, size_t cols) {
+    return rows <= MX_ROUND_ROWS && cols <= MX_ROUND_COLS && rows * cols <= MX_ROUND_ELEMENTS;
+}
+
+MC_EXPORT size_t falcom_mx4_work_bytes(size_t rows, size_t cols) {
+    return rounds_inside(rows, cols) ? 0 : matrix_bytes(rows, cols);
+}
 
 MC_EXPORT int falcom_mx4_product_of(const void *x, int x_type, size_t rows, size_t ld_x, const falcom_mx4_matrix *b,
                                     void *out, int dtype, size_t ld, void *work, void *stream) {
@@ -333,10 +339,24 @@ MC_EXPORT int falcom_mx4_product_of(const void *x, int x_type, size_t rows, size
     begin(&c, who);
     array(&c, "out", out, bytes, g_type_size[dtype], 1);
     array(&c, "x", x, from, g_type_size[x_type], 0);
-    array(&c, "work", work, matrix_bytes(rows, b->cols), 16, 1);
+    array(&c, "work", work, falcom_mx4_work_bytes(rows, b->cols), 16, 1);
     matrix_of(&c, &mb, b, "b", 0);
     int prev, sms, rc = go(&c, &prev, &sms);
     if (rc) return rc;
+    if (rounds_inside(rows, b->cols)) {
+        mx_product_launch L;
+        memset(&L, 0, sizeof(L));
+        L.a.rows = (int64_t)rows;
+        L.a.cols = mb.cols;
+        L.b = mb;
+        L.out = out;
+        L.ld = (int64_t)ld;
+        L.x = x;
+        L.ld_x = (int64_t)ld_x;
+        L.x_type = x_type;
+        L.vectors = ((uintptr_t)x & 15) == 0 && (rows == 1 || ld_x * g_type_size[x_type] % 16 == 0);
+        return done(&c, prev, mc_launch_mx_product(&L, dtype, sms, stream));
+    }
     uint8_t *at = (uint8_t *)work;
     const mx_matrix a = matrix_in(&at, rows, b->cols);
     int e = quantize(x, x_type, rows, b->cols, ld_x, NULL, NULL, &a, NULL, stream);

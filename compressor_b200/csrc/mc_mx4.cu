@@ -8,125 +8,6 @@ namespace {
 
 #define MX_TPB 256
 
-// ------------------------------------------------------------- elements
-template <typename T>
-struct mx_vec8 {
-    T x[8];
-};
-
-template <typename T>
-__device__ __forceinline__ mx_vec8<T> load8(const T *p) {
-    mx_vec8<T> v;
-#pragma unroll
-    for (int i = 0; i < (int)(sizeof(v) / 16); i++) ((uint4 *)&v)[i] = __ldg((const uint4 *)p + i);
-    return v;
-}
-
-// 8 elements from any address: the aligned 16-byte pieces that they lie in,
-// and one more, which may lie outside of them by up to 16 bytes at either end.
-template <typename T>
-struct mx_pieces {
-    uint32_t w[2 * sizeof(T) + 4];
-};
-template <typename T>
-__device__ __forceinline__ mx_pieces<T> load_pieces(const T *p) {
-    mx_pieces<T> v;
-    const uint4 *q = (const uint4 *)((uintptr_t)p & ~(uintptr_t)15);
-#pragma unroll
-    for (int i = 0; i < (int)(sizeof(v) / 16); i++) ((uint4 *)&v)[i] = __ldg(q + i);
-    return v;
-}
-template <typename T>
-__device__ __forceinline__ mx_vec8<T> from_pieces(mx_pieces<T> v, const T *p) {
-    constexpr int N = 2 * sizeof(T);
-    const uint32_t off = (uint32_t)(uintptr_t)p;
-    const bool two = off & 8, one = off & 4;
-#pragma unroll
-    for (int i = 0; i < N + 2; i++) v.w[i] = two ? v.w[i + 2] : v.w[i];
-#pragma unroll
-    for (int i = 0; i < N + 1; i++) v.w[i] = one ? v.w[i + 1] : v.w[i];
-    if (sizeof(T) == 2) {
-        const uint32_t pick = off & 2 ? 0x5432u : 0x3210u;
-#pragma unroll
-        for (int i = 0; i < N; i++) v.w[i] = __byte_perm(v.w[i], v.w[i + 1], pick);
-    }
-    mx_vec8<T> r;
-    memcpy(&r, v.w, sizeof(r));
-    return r;
-}
-
-// What rounding needs of elements: their magnitudes' bits, compared as whole
-// numbers (two at a time where they have 16 bits), and float32 values.
-__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b, float) { return max(a, b & 0x7FFFFFFFu); }
-template <typename T>
-__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b, T) { return __vmaxu2(a, b & 0x7FFF7FFFu); }
-// The float32 bits of the largest, by the two halves of a 32-bit word for 16-bit types.
-__device__ __forceinline__ uint32_t top_low(uint32_t m, __nv_bfloat16) { return m << 16; }
-__device__ __forceinline__ uint32_t top_low(uint32_t m, __half) { return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m))); }
-template <typename T>
-__device__ __forceinline__ uint32_t top_of(uint32_t m, T t) { return max(top_low(m & 0xFFFFu, t), top_low(m >> 16, t)); }
-__device__ __forceinline__ uint32_t top_of(uint32_t m, float) { return m; }
-// Float32 values of the two 16-bit elements of a word.
-__device__ __forceinline__ float2 two_of(uint32_t w, __nv_bfloat16) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)); }
-__device__ __forceinline__ float2 two_of(uint32_t w, __half) {
-    __half2 h;
-    memcpy(&h, &w, 4);
-    return __half22float2(h);
-}
-// Bit 7 of byte B of 8 words to bit 3 of the 8 nibbles of one, and of byte 3.
-template <int B>
-__device__ __forceinline__ uint32_t signs8(const uint32_t *w) {
-    constexpr uint32_t PICK = (uint32_t)(B | (B + 4) << 4);
-    const uint32_t e = __byte_perm(__byte_perm(w[0], w[2], PICK), __byte_perm(w[4], w[6], PICK), 0x5410);
-    const uint32_t o = __byte_perm(__byte_perm(w[1], w[3], PICK), __byte_perm(w[5], w[7], PICK), 0x5410);
-    return ((e >> 4) & 0x08080808u) | (o & 0x80808080u);
-}
-// The same of both halves of 4 words, in the order of the elements.
-__device__ __forceinline__ uint32_t signs4x2(const uint32_t *w) {
-    const uint32_t x = __byte_perm(w[0], w[1], 0x7351), y = __byte_perm(w[2], w[3], 0x7351);
-    return ((__byte_perm(x, y, 0x5410) >> 4) & 0x08080808u) | (__byte_perm(x, y, 0x7632) & 0x80808080u);
-}
-
-// The codes of 8 elements.  y: values (at random: magnitudes) times 1 / scale, two by two.
-template <bool RANDOM>
-__device__ __forceinline__ uint32_t codes8(const float2 *y, uint32_t signs, const uint32_t *bits16) {
-    if (RANDOM) return mx_codes8_random(y, bits16) | signs;
-    return mx_codes8((const float *)y);
-}
-
-// The values of two words' elements, or of their magnitudes.
-template <typename T, bool RANDOM>
-__device__ __forceinline__ float2 two_values(const uint32_t *w, int i) {
-    if constexpr (sizeof(T) == 4) {
-        const uint32_t m = RANDOM ? 0x7FFFFFFFu : 0xFFFFFFFFu;
-        return make_float2(__uint_as_float(w[2 * i] & m), __uint_as_float(w[2 * i + 1] & m));
-    } else {
-        return two_of(RANDOM ? w[i] & 0x7FFF7FFFu : w[i], T());
-    }
-}
-
-// A row's 8 elements (raw words) to codes.
-template <typename T, bool RANDOM, bool DROP>
-__device__ __forceinline__ uint32_t row_codes(const uint32_t *w, float inv, float factor, const mx_bits *bits) {
-    float2 y[4];
-    uint32_t bits16[8], signs = 0;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        y[i] = two_values<T, RANDOM>(w, i);
-        if (DROP) y[i] = mx_mul2(y[i], make_float2(factor, factor));
-        y[i] = mx_mul2(y[i], make_float2(inv, inv));
-        if (RANDOM) {
-            bits16[2 * i] = bits[i].low;
-            bits16[2 * i + 1] = bits[i].high;
-        }
-    }
-    if (RANDOM) {
-        if constexpr (sizeof(T) == 4) signs = signs8<3>(w);
-        else signs = signs4x2(w);
-    }
-    return codes8<RANDOM>(y, signs, bits16);
-}
-
 // ------------------------------------------------------------- vectors
 // A warp has 8 blocks.  On 16-byte boundaries a lane has 8 elements, 4 lanes a
 // block, as in a matrix's rows.  On others lane i has element i of each block,
@@ -363,6 +244,39 @@ __global__ void __launch_bounds__(MX_TPB) k_mx_decode(const __grid_constant__ mx
 // neighbouring columns, which share their random words.
 #define MX_TILE 128
 
+// 8 elements from any address: the aligned 16-byte pieces that they lie in,
+// and one more, which may lie outside of them by up to 16 bytes at either end.
+template <typename T>
+struct mx_pieces {
+    uint32_t w[2 * sizeof(T) + 4];
+};
+template <typename T>
+__device__ __forceinline__ mx_pieces<T> load_pieces(const T *p) {
+    mx_pieces<T> v;
+    const uint4 *q = (const uint4 *)((uintptr_t)p & ~(uintptr_t)15);
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(v) / 16); i++) ((uint4 *)&v)[i] = __ldg(q + i);
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ mx_vec8<T> from_pieces(mx_pieces<T> v, const T *p) {
+    constexpr int N = 2 * sizeof(T);
+    const uint32_t off = (uint32_t)(uintptr_t)p;
+    const bool two = off & 8, one = off & 4;
+#pragma unroll
+    for (int i = 0; i < N + 2; i++) v.w[i] = two ? v.w[i + 2] : v.w[i];
+#pragma unroll
+    for (int i = 0; i < N + 1; i++) v.w[i] = one ? v.w[i + 1] : v.w[i];
+    if (sizeof(T) == 2) {
+        const uint32_t pick = off & 2 ? 0x5432u : 0x3210u;
+#pragma unroll
+        for (int i = 0; i < N; i++) v.w[i] = __byte_perm(v.w[i], v.w[i + 1], pick);
+    }
+    mx_vec8<T> r;
+    memcpy(&r, v.w, sizeof(r));
+    return r;
+}
+
 // Shared memory of a tile: its elements, and its random words (of which a
 // column's rounding has the same as a row's).
 template <typename T, bool COLS, bool RANDOM>
@@ -469,20 +383,34 @@ __global__ void __launch_bounds__(MX_TPB, COLS && sizeof(T) == 4 ? 3 : 4) k_mx_q
             for (int j = 0; j < BATCH; j++, row += 16 * L.ld) one(from_pieces(v[j], row), i + j, true);
         }
     } else {
+        // part of a tile; 16 rows that are all padding need no rounding
 #pragma unroll 1
-        for (int i = 0; i < MX_TILE / 16; i++, row += 16 * L.ld) {
-            mx_vec8<T> v;
-            memset(&v, 0, sizeof(v));
-            if (ty + 16 * i < left && c < L.cols) {
-                if (L.vectors && c + 8 <= L.cols) {
-                    v = load8(row + c);
-                } else {
+        for (int i = 0; i < MX_TILE / 16; i += BATCH) {
+            mx_vec8<T> v[BATCH];
 #pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        if (c + j < L.cols) v.x[j] = row[c + j];
+            for (int j = 0; j < BATCH; j++, row += 16 * L.ld) {
+                memset(&v[j], 0, sizeof(v[j]));
+                if (ty + 16 * (i + j) < left && c < L.cols) {
+                    if (L.vectors && c + 8 <= L.cols) {
+                        v[j] = load8(row + c);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 8; k++)
+                            if (c + k < L.cols) v[j].x[k] = row[c + k];
+                    }
                 }
             }
-            one(v, i, ty + 16 * i < left8);
+#pragma unroll
+            for (int j = 0; j < BATCH; j++) {
+                if (16 * (i + j) < left8) {
+                    one(v[j], i + j, ty + 16 * (i + j) < left8);
+                } else {
+                    const int y = ty + 16 * (i + j);
+                    if (COLS) memset(s_tile + (y * MX_TILE + 8 * tx) * sizeof(T), 0, 8 * sizeof(T));
+                    if (COLS && RANDOM) *(uint4 *)(s_words + y * (MX_TILE / 2) + 4 * tx) = make_uint4(0, 0, 0, 0);
+                    if (ROWS && (tx & 3) == 0) s_rows[(y & 31) * 16 + (y >> 5) * 4 + (tx >> 2)] = 0;
+                }
+            }
         }
     }
     __syncthreads();

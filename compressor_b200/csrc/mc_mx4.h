@@ -74,11 +74,21 @@ typedef struct {
     int64_t ld;
 } mx_dequantize_launch;
 
+/* Few enough rows and columns to be rounded inside the product, by every CTA
+ * for itself. */
+#define MX_ROUND_ROWS 16
+#define MX_ROUND_COLS 4096
+#define MX_ROUND_ELEMENTS 32768
+
 typedef struct {
     mx_matrix a, b;
     void *out;                 /* [a.rows][ld] */
     int64_t ld;
     mx_drop drop;
+    const void *x;             /* not NULL: a as it is before rounding (then without codes and scales) */
+    int64_t ld_x;
+    int32_t x_type;
+    int32_t vectors;           /* every row of x starts on a 16-byte boundary */
 } mx_product_launch;
 
 typedef struct {

@@ -6,12 +6,10 @@
 // panels of 256 columns, in a panel 128 bytes a row with the 128-byte swizzle
 // already applied, and the scales in pieces of 128 rows by 4.  So a tile of
 // any rows is one contiguous run, and a bulk copy brings it in.
-//
-// b's rows are the instruction's M (128 lanes of the accumulator), a's rows
-// its N: neighbouring lanes are neighbouring elements of a row of `out`, and
-// few rows of a (tokens) cost a narrow instruction instead of an empty one.
 
 #include <cuda.h>
+
+#include <type_traits>
 
 #include "mc_mx4_device.h"
 
@@ -123,19 +121,29 @@ __device__ __forceinline__ uint64_t desc_scales(uint32_t at) {
 
 __device__ uint32_t g_mx_error;   // a wait ran out
 
-// --------------------------------------------------------------- constants
-// BN: rows of a in a tile.
-template <int BN>
+// ------------------------------------------------------------------ narrow
+// Few tiles.  One tile of 128 x BN a CTA: b's rows are the instruction's M (128
+// lanes of the sum), a's rows its N, so that neighbouring lanes are
+// neighbouring elements of a row of `out`, and few rows of a (tokens) cost a
+// narrow instruction instead of an empty one.  What bounds it is the way to b:
+// the stages of the CTAs of an SM (3 at most) take all its shared memory.  The
+// CTAs of a cluster have the same tile and a share of the panels each; their
+// sums meet in the order of the ranks.  TX: a is not in 4 bits yet but has elements of this type; each
+// CTA rounds what it needs (void: it is).
+template <int BN, bool ROUND>
 struct mx_cfg {
     static constexpr int GROUPS = BN > 128 ? 2 : 1;                  // of a's rows with scales
-    static constexpr int B_BYTES = 128 * 128, A_BYTES = BN * 128;    // codes of a panel
-    static constexpr int STAGE = B_BYTES + A_BYTES + 1024 + GROUPS * 1024;
-    static constexpr int ROOM = BN == 256 ? 225 * 1024 : BN == 128 ? 112 * 1024 : 100 * 1024;
-    static constexpr int STAGES = ROOM / STAGE < 8 ? ROOM / STAGE : 8;
-    static constexpr int SMEM = STAGES * STAGE + 1024;
-    static constexpr int SCALES = 8 + 8 * GROUPS;                    // columns of a panel's scales
-    static constexpr int NEED = BN + 2 * SCALES;
-    static constexpr int COLUMNS = NEED <= 64 ? 64 : NEED <= 128 ? 128 : NEED <= 256 ? 256 : 512;
+    static constexpr int B_BYTES = 128 * 128, A_BYTES = BN * 128, A_ALL = A_BYTES + GROUPS * 1024;   // of a panel
+    static constexpr int STAGE = B_BYTES + 1024 + (ROUND ? 0 : A_ALL);
+    static constexpr int SUMS = (BN * 512 + STAGE - 1) / STAGE;      // stages that a cluster's sums lie over
+    static constexpr int SCALES = 8 + 8 * GROUPS;                    // columns of a panel's scales: each stage has its own
+    static constexpr int COLUMNS = BN <= 64 ? 128 : 2 * BN;
+    static constexpr int SLOTS = (COLUMNS - BN) / SCALES, FIT = 222 * 1024 / STAGE;
+    static constexpr int MOST = SLOTS < FIT ? SLOTS : FIT;
+    // CTAs that wait for columns may hold up others of their cluster, which have theirs: so whatever CTAs share an SM
+    // have columns for all, each taking at least as large a share of the shared memory (228 KB, 1 KB a CTA) as of the 512.
+    static constexpr int LEAST = BN == 256 ? 200 * 1024 : COLUMNS * 456 - 1024;
+    static_assert(SUMS <= MOST, "");
     // E2M1 both, E8M0 scales, M = 128
     static constexpr uint32_t IDESC = 1u << 7 | 1u << 10 | (uint32_t)(BN / 8) << 17 | 1u << 23 | 1u << 27;
 };
@@ -151,16 +159,78 @@ __device__ __forceinline__ void put(const mx_product_launch &L, mx_key key, int6
     mx_from((T *)L.out + t * L.ld + n, v);
 }
 
-// One tile of 128 x BN a CTA.  The CTAs of a cluster have the same tile and a
-// share of the panels each; their sums meet in the order of the ranks.
-template <typename T, int BN, bool DROP>
-__global__ void __launch_bounds__(MX_THREADS) k_mx_product(const __grid_constant__ mx_product_launch L, int tiles_n, int split) {
-    typedef mx_cfg<BN> C;
+// Rounds a's rows (all of them, 16 at most) of panels p0 to p1 to shared
+// memory, `stride` bytes a panel: BN rows of codes, then scales.
+template <typename TX, int BN>
+__device__ __forceinline__ void round_rows(const mx_product_launch &L, uint32_t to, int stride, int p0, int p1) {
+    const int units = (p1 - p0) * 32, all = (int)L.a.rows * units;   // of 8 elements; whole warps
+    for (int u = threadIdx.x; u < all; u += 128) {
+        const int r = u / units, q = u - r * units;
+        const int64_t c = (int64_t)p0 * MX_PANEL + 8 * q;
+        const TX *x = (const TX *)L.x + r * L.ld_x + c;
+        mx_vec8<TX> v;
+        memset(&v, 0, sizeof(v));
+        if (L.vectors && c + 8 <= L.a.cols) {
+            v = load8(x);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (c + j < L.a.cols) v.x[j] = x[j];
+        }
+        uint32_t w[2 * sizeof(TX)], m = 0;
+        memcpy(w, &v, sizeof(v));
+#pragma unroll
+        for (int j = 0; j < (int)(2 * sizeof(TX)); j++) m = larger(m, w[j], TX());
+        uint32_t top = top_of(m, TX());
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const uint32_t s = mx_scale(top);
+        uint32_t codes = row_codes<TX, false, false>(w, mx_inverse(s), 1.0f, NULL);
+        if (s == 255u) codes = 0;
+        const int j = q / 4 & 7;   // block of the panel
+        const uint32_t at = to + q / 32 * stride;
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + r * 128 + ((j ^ (r & 7)) * 16) + (q & 3) * 4), "r"(codes) : "memory");
+        if ((q & 3) == 0)
+            asm volatile("st.shared.b8 [%0], %1;" ::"r"(at + BN * 128 + (j >> 2) * 512 + r * 16 + (j & 3)), "r"(s) : "memory");
+    }
+}
+
+// This rank's share of the rows [from, to) of a cluster's sums, [row][128]
+// float32 at `sums` of each rank, added in the order of the ranks.  The others'
+// come from far: 16 loads at a time.
+template <typename T, int SPLIT, bool DROP>
+__device__ __forceinline__ void meet(const mx_product_launch &L, mx_key key, int64_t wide, uint32_t sums, int64_t t0, int64_t n, int from, int to,
+                                     bool inside) {
+    constexpr int ROWS = 16 / SPLIT;
+    const uint32_t mine = sums + threadIdx.x * 4;
+#pragma unroll 1
+    for (int c = from; c < to; c += ROWS) {
+        float u[ROWS][SPLIT];
+#pragma unroll
+        for (int j = 0; j < ROWS; j++)
+#pragma unroll
+            for (int q = 0; q < SPLIT; q++)
+                if (c + j < to) u[j][q] = ld_cluster(mine + (c + j) * 512, q);
+#pragma unroll
+        for (int j = 0; j < ROWS; j++) {
+            float v = u[j][0];
+#pragma unroll
+            for (int q = 1; q < SPLIT; q++) v += u[j][q];
+            if (c + j < to && inside) put<T, DROP>(L, key, wide, t0 + c + j, n, v);
+        }
+    }
+}
+
+template <typename T, int BN, bool DROP, typename TX>
+__global__ void __launch_bounds__(MX_THREADS) k_mx_product(const __grid_constant__ mx_product_launch L, int tiles_n, int split, int stages) {
+    constexpr bool ROUND = !std::is_same<TX, void>::value;
+    typedef mx_cfg<BN, ROUND> C;
     extern __shared__ uint8_t s_raw[];
-    __shared__ __align__(8) uint64_t s_full[C::STAGES], s_empty[C::STAGES], s_done;
-    __shared__ uint32_t s_tmem, s_failed;
+    __shared__ __align__(8) uint64_t s_full[C::MOST], s_empty[C::MOST], s_done, s_rounded;
+    __shared__ uint32_t s_tmem;
+    __shared__ volatile uint32_t s_failed;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t smem = (smem_u32(s_raw) + 1023) & ~1023u;
+    const uint32_t smem = (smem_u32(s_raw) + 1023) & ~1023u, own = smem + stages * C::STAGE;
     const int rank = blockIdx.x % split, tile = blockIdx.x / split;
     const int64_t n0 = (int64_t)(tile % tiles_n) * 128, t0 = (int64_t)(tile / tiles_n) * BN;
     const int64_t cols = L.a.cols;
@@ -169,11 +239,12 @@ __global__ void __launch_bounds__(MX_THREADS) k_mx_product(const __grid_constant
 
     if (warp == 5) tmem_alloc<C::COLUMNS>(smem_u32(&s_tmem));
     if (threadIdx.x == 0) {
-        for (int i = 0; i < C::STAGES; i++) {
+        for (int i = 0; i < stages; i++) {
             mbar_init(smem_u32(&s_full[i]), 1);
             mbar_init(smem_u32(&s_empty[i]), 1);
         }
         mbar_init(smem_u32(&s_done), 1);
+        mbar_init(smem_u32(&s_rounded), 128);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         s_failed = 0;
     }
@@ -186,40 +257,51 @@ __global__ void __launch_bounds__(MX_THREADS) k_mx_product(const __grid_constant
     if (warp == 4 && elect_one()) {
         const int64_t rows_b = mx_rows8(L.b.rows), rows_a = mx_rows8(L.a.rows);
         const int64_t groups_b = (L.b.rows + 127) / 128, groups_a = (L.a.rows + 127) / 128;
-        const uint32_t nb = (uint32_t)min((int64_t)128, rows_b - n0) * 128, na = (uint32_t)min((int64_t)BN, rows_a - t0) * 128;
-        const uint32_t ga = (uint32_t)min((int64_t)C::GROUPS, groups_a - t0 / 128) * 1024;
-        int issued = p0;
-        for (int p = p0; p < p1; p++) {
-            const int i = p - p0, s = i % C::STAGES;
-            if (i >= C::STAGES && !mbar_wait(smem_u32(&s_empty[s]), (i / C::STAGES - 1) & 1, 4)) {
-                s_failed = 1;
-                break;
-            }
+        const uint32_t nb = (uint32_t)min((int64_t)128, rows_b - n0) * 128, na = ROUND ? 0 : (uint32_t)min((int64_t)BN, rows_a - t0) * 128;
+        const uint32_t ga = ROUND ? 0 : (uint32_t)min((int64_t)C::GROUPS, groups_a - t0 / 128) * 1024;
+        const uint8_t *b = L.b.codes + ((int64_t)p0 * rows_b + n0) * 128, *sb = L.b.scales + ((int64_t)p0 * groups_b + n0 / 128) * 1024;
+        const uint8_t *a = L.a.codes + ((int64_t)p0 * rows_a + t0) * 128, *sa = L.a.scales + ((int64_t)p0 * groups_a + t0 / 128) * 1024;
+        int s = 0, round = 0;   // stage, times round
+        bool ok = true;
+        int p = p0;
+        for (; p < p1; p++, b += rows_b * 128, sb += groups_b * 1024, a += rows_a * 128, sa += groups_a * 1024) {
+            if (round > 0) ok = mbar_wait(smem_u32(&s_empty[s]), (round - 1) & 1, 4);
+            if (!ok) break;
             const uint32_t at = smem + s * C::STAGE, bar = smem_u32(&s_full[s]);
             mbar_expect_tx(bar, nb + na + 1024 + ga);
-            bulk_g2s(at, L.b.codes + ((int64_t)p * rows_b + n0) * 128, nb, bar);
-            bulk_g2s(at + C::B_BYTES, L.a.codes + ((int64_t)p * rows_a + t0) * 128, na, bar);
-            bulk_g2s(at + C::B_BYTES + C::A_BYTES, L.b.scales + ((int64_t)p * groups_b + n0 / 128) * 1024, 1024, bar);
-            bulk_g2s(at + C::B_BYTES + C::A_BYTES + 1024, L.a.scales + ((int64_t)p * groups_a + t0 / 128) * 1024, ga, bar);
-            issued = p + 1;
+            bulk_g2s(at, b, nb, bar);
+            bulk_g2s(at + C::B_BYTES, sb, 1024, bar);
+            if (!ROUND) {
+                bulk_g2s(at + C::B_BYTES + 1024, a, na, bar);
+                bulk_g2s(at + C::B_BYTES + 1024 + C::A_BYTES, sa, ga, bar);
+            }
+            if (++s == stages) {
+                s = 0;
+                round++;
+            }
         }
-        if (s_failed)   // no copy may outlive the CTA
-            for (int i = max(0, issued - p0 - C::STAGES); i < issued - p0; i++)
-                mbar_wait(smem_u32(&s_full[i % C::STAGES]), (i / C::STAGES) & 1, 2);
+        if (!ok) s_failed = 1;
+        // no copy may outlive the CTA, whoever gave up: the last round of each stage
+        for (int left = min(p - p0, stages); left > 0; left--) {
+            if (s-- == 0) {
+                s = stages - 1;
+                round--;
+            }
+            mbar_wait(smem_u32(&s_full[s]), round & 1, 2);
+        }
     }
     if (warp == 5 && elect_one()) {
-        for (int p = p0; p < p1; p++) {
-            const int i = p - p0, s = i % C::STAGES;
-            bool ok = mbar_wait(smem_u32(&s_full[s]), (i / C::STAGES) & 1, 4);
-            // the columns of scales are free once the panel before the last one is done with
-            if (ok && i >= 2) ok = mbar_wait(smem_u32(&s_empty[(i - 2) % C::STAGES]), ((i - 2) / C::STAGES) & 1, 4);
-            if (!ok) {
-                s_failed = 1;
-                break;
-            }
+        bool ok = !ROUND || mbar_wait(smem_u32(&s_rounded), 0, 8);
+        int s = 0, round = 0;   // stage, times round
+        for (int p = p0; p < p1 && ok; p++) {
+            const int i = p - p0;
+            // a full stage is one whose last panel is done with, and so are that panel's columns of scales
+            ok = mbar_wait(smem_u32(&s_full[s]), round & 1, 4);
+            if (!ok) break;
             tc_after_sync();
-            const uint32_t at = smem + s * C::STAGE, sb = at + C::B_BYTES + C::A_BYTES, sa = sb + 1024;
-            const uint32_t cols_b = tmem + BN + (i & 1) * C::SCALES, cols_a = cols_b + 8;
+            const uint32_t at = smem + s * C::STAGE, sb = at + C::B_BYTES;
+            const uint32_t a = ROUND ? own + i * C::A_ALL : sb + 1024, sa = a + C::A_BYTES;
+            const uint32_t cols_b = tmem + BN + s * C::SCALES, cols_a = cols_b + 8;
             const int steps = (int)min((int64_t)4, (cols - (int64_t)p * MX_PANEL + 63) / 64);
 #pragma unroll
             for (int h = 0; h < 2; h++) {
@@ -228,15 +310,27 @@ __global__ void __launch_bounds__(MX_THREADS) k_mx_product(const __grid_constant
                 for (int g = 0; g < C::GROUPS; g++)
                     tc_copy_scales(cols_a + (h * C::GROUPS + g) * 4, desc_scales(sa + g * 1024 + h * 512));
             }
-            const uint64_t db = desc_codes(at), da = desc_codes(at + C::B_BYTES);
+            const uint64_t db = desc_codes(at), da = desc_codes(a);
             for (int j = 0; j < steps; j++) {
                 const uint32_t id = (j & 1) * 2, h = j >> 1;
                 tc_mma(tmem, db + 2 * j, da + 2 * j, C::IDESC | id << 4 | id << 29, cols_b + h * 4,
                        cols_a + h * C::GROUPS * 4, i > 0 || j > 0);
             }
             tc_commit(smem_u32(&s_empty[s]));
+            if (++s == stages) {
+                s = 0;
+                round++;
+            }
         }
+        if (!ok) s_failed = 1;
         tc_commit(smem_u32(&s_done));
+    }
+    if constexpr (ROUND) {
+        if (warp < 4) {
+            round_rows<TX, BN>(L, own, C::A_ALL, p0, p1);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // for the tensor core
+            asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&s_rounded)) : "memory");
+        }
     }
     __syncwarp();
 
@@ -269,20 +363,21 @@ __global__ void __launch_bounds__(MX_THREADS) k_mx_product(const __grid_constant
         if (warp < 4)
             for (int c = 0; c < BN && c < valid; c += 16) {
                 uint32_t r[16];
+                __syncwarp();
                 tc_ld16(mine + c, r);
                 tc_wait_ld();
 #pragma unroll
                 for (int j = 0; j < 16; j++)
                     asm volatile("st.shared.b32 [%0], %1;" ::"r"(smem + ((c + j) * 128 + 32 * warp + lane) * 4), "r"(r[j]) : "memory");
             }
+        __syncwarp();
         cluster_sync();
-        if (warp < 4 && n < L.b.rows) {
+        if (warp < 4) {
             const int from = valid * rank / split, to = valid * (rank + 1) / split;
-            for (int c = from; c < to; c++) {
-                float v = 0.0f;
-                for (int q = 0; q < split; q++) v += ld_cluster(smem + (c * 128 + 32 * warp + lane) * 4, q);
-                put<T, DROP>(L, key, wide, t0 + c, n, v);
-            }
+            const bool inside = n < L.b.rows && fine;
+            if (split == 2) meet<T, 2, DROP>(L, key, wide, smem, t0, n, from, to, inside);
+            else if (split == 4) meet<T, 4, DROP>(L, key, wide, smem, t0, n, from, to, inside);
+            else meet<T, 8, DROP>(L, key, wide, smem, t0, n, from, to, inside);
         }
         __syncwarp();
         cluster_sync();
@@ -697,18 +792,27 @@ static int product_wide(const mx_product_launch &L, int sms, cudaStream_t s) {
     return mx_launch(kern, 2 * pairs, C::THREADS, C::SMEM, 0, s, L, M, (int)tiles_n, (int)tiles);
 }
 
-template <typename T, int BN, bool DROP>
+template <typename T, int BN, bool DROP, typename TX = void>
 static int product_as(const mx_product_launch &L, int sms, cudaStream_t s) {
-    typedef mx_cfg<BN> C;
-    auto kern = k_mx_product<T, BN, DROP>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-    if (e != cudaSuccess) return e;
+    constexpr bool ROUND = !std::is_same<TX, void>::value;
+    typedef mx_cfg<BN, ROUND> C;
     const int64_t tiles_n = (L.b.rows + 127) / 128, tiles_t = (L.a.rows + BN - 1) / BN, tiles = tiles_n * tiles_t;
     const int64_t panels = (L.a.cols + MX_PANEL - 1) / MX_PANEL;
     int split = 1;
     while (split < 8 && tiles * split * 2 <= sms && split * 2 <= panels) split *= 2;
     if (tiles * split > 0x7FFFFFFF) return cudaErrorInvalidValue;
-    return mx_launch(kern, tiles * split, MX_THREADS, C::SMEM, split, s, L, (int)tiles_n, split);
+    // as many stages as the CTAs of an SM have room for, and use for
+    const int64_t ctas = (tiles * split + sms - 1) / sms, each = (panels + split - 1) / split;
+    const int own = 1024 + (ROUND ? (int)each * C::A_ALL : 0), least = split > 1 ? C::SUMS : 1;
+    int stages = (222 * 1024 / (int)(ctas < 3 ? ctas : 3) - own) / C::STAGE;
+    if (stages > each) stages = (int)each;
+    if (stages < least) stages = least;
+    if (stages > C::MOST) stages = C::MOST;
+    const int need = own + stages * C::STAGE, smem = need < C::LEAST ? C::LEAST : need;
+    auto kern = k_mx_product<T, BN, DROP, TX>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 225 * 1024);
+    if (e != cudaSuccess) return e;
+    return mx_launch(kern, tiles * split, MX_THREADS, smem, split, s, L, (int)tiles_n, split, stages);
 }
 
 template <typename T, bool DROP>
@@ -726,6 +830,11 @@ static int product_for(const mx_product_launch &L, int sms, cudaStream_t s) {
 
 template <typename T>
 static int product(const mx_product_launch &L, int sms, cudaStream_t s) {
+    if (L.x) {
+        if (L.x_type == FALCOM_TYPE_F32) return product_as<T, 16, false, float>(L, sms, s);
+        if (L.x_type == FALCOM_TYPE_BF16) return product_as<T, 16, false, __nv_bfloat16>(L, sms, s);
+        return product_as<T, 16, false, __half>(L, sms, s);
+    }
     return L.drop.random.on ? product_for<T, true>(L, sms, s) : product_for<T, false>(L, sms, s);
 }
 

@@ -300,10 +300,12 @@ def product(a: Union[torch.Tensor, Mx4Matrix], b: Mx4Matrix, dtype: torch.dtype 
     device = b.device
     _same_device(device, a=x)
     y = _out(rows, b, dtype, out, a.shape[:-1])
-    work = torch.empty(sum(Mx4Matrix.sizes_of(rows, cols)), dtype=torch.uint8, device=device)
-    _done(_library().falcom_mx4_product_of(x.data_ptr(), _TYPES[x.dtype], rows, x.stride(0) if rows > 1 else cols,
-                                           b._ref, y.data_ptr(), _TYPES[y.dtype], b.rows, work.data_ptr(),
-                                           _stream(device)), "falcom_mx4_product_of")
+    lib = _library()
+    size = lib.falcom_mx4_work_bytes(rows, cols)
+    work = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    _done(lib.falcom_mx4_product_of(x.data_ptr(), _TYPES[x.dtype], rows, x.stride(0) if rows > 1 else cols, b._ref,
+                                    y.data_ptr(), _TYPES[y.dtype], b.rows, work.data_ptr() if size else None,
+                                    _stream(device)), "falcom_mx4_product_of")
     return y
 
 

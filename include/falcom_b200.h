@@ -551,7 +551,9 @@ int falcom_mx4_product(const falcom_mx4_matrix *a, const falcom_mx4_matrix *b, v
                        const falcom_dropout_args *drop, void *stream);
 /* The same with a matrix that is not in 4 bits yet: x (rows x b->cols, rows
  * `ld_x` elements apart) is rounded to the nearest along its rows into `work`,
- * falcom_mx4_work_bytes(rows, b->cols) bytes on a 16-byte boundary. */
+ * falcom_mx4_work_bytes(rows, b->cols) bytes on a 16-byte boundary; 0 bytes
+ * (and NULL) for the few rows of single tokens, which are rounded inside the
+ * product. */
 size_t falcom_mx4_work_bytes(size_t rows, size_t cols);
 int falcom_mx4_product_of(const void *x, int x_type, size_t rows, size_t ld_x, const falcom_mx4_matrix *b, void *out,
                           int dtype, size_t ld, void *work, void *stream);

@@ -114,3 +114,19 @@ def test_encode_and_decode(mx4, n, dtype, rounding, shift):
     assert torch.equal(og.cpu(), (out.float() + torch.tensor(0.3) * v.float()).to(dtype))
     alone = mx4.encode(xg, rounding=rounding, seed=11, counter=counter)
     assert torch.equal(alone.decode().cpu().double(), ref.values(x[None], bits)[0])
+
+
+# rounded inside the product (few rows and columns) or before it: the same bits either way
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("t,n,k", [(1, 1, 1), (1, 50257, 1024), (3, 200, 31), (4, 1024, 4096), (5, 129, 300), (16, 384, 1024), (16, 130, 1025), (16, 200, 2049), (8, 20000, 4096),
+                                   (17, 130, 64), (1, 300, 4097), (2, 70, 8191)])
+def test_product_of_a_tensor(mx4, t, n, k, dtype):
+    b = mx4.quantize(wild(n, k, torch.float32, 2).cuda())
+    whole = wild(t, k + 3, dtype, 1).cuda()
+    if t > 2:
+        whole[1, k // 2] = float("nan")
+    for x in (whole[:, 3:], whole[:, :k].contiguous(), whole[:, 1:k + 1]):
+        for out in TYPES:
+            y = mx4.product(x, b, dtype=out)
+            assert torch.equal(y.nan_to_num(7.5), mx4.product(mx4.quantize(x), b, dtype=out).nan_to_num(7.5))
+    assert y.isnan().any().item() == (t > 2) and mx4.errors() == 0

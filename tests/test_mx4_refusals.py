@@ -46,7 +46,7 @@ def test_sizes(lib):
     for rows, cols in [(1, 1), (8, 256), (9, 257), (128, 32), (129, 1000), (0, 5), (5, 0), (50257, 1024)]:
         codes, scales = lib.falcom_mx4_codes_bytes(rows, cols), lib.falcom_mx4_scales_bytes(rows, cols)
         assert (codes, scales) == Mx4Matrix.sizes_of(rows, cols)
-        assert lib.falcom_mx4_work_bytes(rows, cols) == codes + scales
+        assert lib.falcom_mx4_work_bytes(rows, cols) == (0 if rows <= 16 and cols <= 4096 and rows * cols <= 32768 else codes + scales)
         # 4 bits an element and one byte per 32, filled up to 8 rows (scales: 128) and 256 columns
         if rows and cols:
             assert codes == -(-cols // 256) * 256 * -(-rows // 8) * 8 // 2

@@ -96,13 +96,13 @@ __global__ void __launch_bounds__(MX_TPB) k_mx_encode8(const __grid_constant__ m
         m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
         m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
         const uint32_t s = mx_scale(m);
-        mx_bits bits[4];
+        uint32_t words[4];
         if (RANDOM) {
             const uint32_t start = mx_start(key, (uint64_t)(4 * i));
 #pragma unroll
-            for (int j = 0; j < 4; j++) bits[j] = mx_bits_of(key, start ^ j);
+            for (int j = 0; j < 4; j++) words[j] = mx_word(key, start ^ j);
         }
-        uint32_t codes = row_codes<float, RANDOM, false>(w, mx_inverse(s), 1.0f, bits);
+        uint32_t codes = row_codes<float, RANDOM, false>(w, mx_inverse(s), 1.0f, words);
         if (s == 255u) codes = 0;
         if (BASE) {
             const float unit = mx_scale_value(s);
@@ -181,8 +181,8 @@ __global__ void __launch_bounds__(MX_TPB) k_mx_encode(const __grid_constant__ mx
             const float y = v[b] * mx_inverse(s);
             uint32_t code;
             if (RANDOM) {
-                const mx_bits w = mx_bits_at(key, (uint64_t)(c * 128 + 16 * b + (lane >> 1)));
-                code = mx_code_random(__fmul_rz(fabsf(y), MX_CUT), lane & 1 ? w.high : w.low) | (__float_as_uint(y) >> 31 << 3);
+                const uint32_t w = mx_word_at(key, (uint64_t)(c * 128 + 16 * b + (lane >> 1)));
+                code = mx_code_random(__fmul_rz(fabsf(y), MX_CUT), lane & 1 ? mx_add_high(w) : mx_add_low(w)) | (__float_as_uint(y) >> 31 << 3);
             } else {
                 code = mx_code_near(y);
             }
@@ -286,7 +286,7 @@ struct mx_tile {
 };
 
 template <typename T, bool ROWS, bool COLS, bool RANDOM, bool DROP>
-__global__ void __launch_bounds__(MX_TPB, COLS && sizeof(T) == 4 ? 3 : 4) k_mx_quantize(const __grid_constant__ mx_quantize_launch L) {
+__global__ void __launch_bounds__(MX_TPB, COLS ? (sizeof(T) == 4 ? 3 : 4) : RANDOM ? 4 : 5) k_mx_quantize(const __grid_constant__ mx_quantize_launch L) {
     mx_begin();
     typedef mx_tile<T, COLS, RANDOM> S;
     constexpr int W = 8 * sizeof(T) / 4;   // words of 8 elements
@@ -311,32 +311,27 @@ __global__ void __launch_bounds__(MX_TPB, COLS && sizeof(T) == 4 ? 3 : 4) k_mx_q
     auto one = [&](mx_vec8<T> v, int i, bool inside) {
         const int y = ty + 16 * i;
         uint32_t w[W];
-        mx_bits bits[4];
+        uint32_t words[4];
         if (DROP) {
             const uint32_t start = mx_start(drop, pair);
 #pragma unroll
             for (int j = 0; j < 8; j += 2) {
-                const mx_bits u = mx_bits_of(drop, start ^ (j / 2));
-                if (u.low < L.drop.threshold) memset(&v.x[j], 0, sizeof(T));
-                if (u.high < L.drop.threshold) memset(&v.x[j + 1], 0, sizeof(T));
+                const uint32_t u = mx_word(drop, start ^ (j / 2));
+                if ((u & 0xFFFFu) < L.drop.threshold) memset(&v.x[j], 0, sizeof(T));
+                if ((u >> 16) < L.drop.threshold) memset(&v.x[j + 1], 0, sizeof(T));
             }
         }
         memcpy(w, &v, sizeof(v));
         if (RANDOM) {
             const uint32_t start = mx_start(key, pair);
 #pragma unroll
-            for (int j = 0; j < 4; j++) bits[j] = mx_bits_of(key, start ^ j);
+            for (int j = 0; j < 4; j++) words[j] = mx_word(key, start ^ j);
         }
         if (COLS) {
             uint4 *q = (uint4 *)(s_tile + (y * MX_TILE + 8 * tx) * sizeof(T));
 #pragma unroll
             for (int j = 0; j < W / 4; j++) q[j] = *(const uint4 *)(w + 4 * j);
-            if (RANDOM) {
-                uint32_t u[4];
-#pragma unroll
-                for (int j = 0; j < 4; j++) u[j] = bits[j].high << 16 | bits[j].low;
-                *(uint4 *)(s_words + y * (MX_TILE / 2) + 4 * tx) = *(const uint4 *)u;
-            }
+            if (RANDOM) *(uint4 *)(s_words + y * (MX_TILE / 2) + 4 * tx) = *(const uint4 *)words;
         }
         if (ROWS) {
             uint32_t m = 0;
@@ -346,14 +341,14 @@ __global__ void __launch_bounds__(MX_TPB, COLS && sizeof(T) == 4 ? 3 : 4) k_mx_q
                 m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
                 m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
             } else {
-                m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 1));
-                m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                m = larger(m, __shfl_xor_sync(0xffffffffu, m, 1), T());
+                m = larger(m, __shfl_xor_sync(0xffffffffu, m, 2), T());
             }
             uint32_t top = top_of(m, T());
             // (the largest product is the largest element's)
             if (DROP) top = __float_as_uint(__uint_as_float(top) * L.drop.factor);
             const uint32_t s = mx_scale(top);
-            uint32_t codes = row_codes<T, RANDOM, DROP>(w, mx_inverse(s), L.drop.factor, bits);
+            uint32_t codes = row_codes<T, RANDOM, DROP>(w, mx_inverse(s), L.drop.factor, words);
             if (s == 255u) codes = 0;
             if (inside) *(uint32_t *)(to + i * 16 * 128) = codes;   // (16 rows on the pieces of a row lie alike)
             if ((tx & 3) == 0) s_rows[(y & 31) * 16 + (y >> 5) * 4 + (tx >> 2)] = (uint8_t)s;
@@ -448,7 +443,7 @@ __global__ void __launch_bounds__(MX_TPB, COLS && sizeof(T) == 4 ? 3 : 4) k_mx_q
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             float2 f[2][4];
-            uint32_t bits16[2][8], signs[2] = {0, 0}, w[2][8];
+            uint32_t add[2][8], signs[2] = {0, 0}, w[2][8];
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 float2 x;
@@ -456,19 +451,20 @@ __global__ void __launch_bounds__(MX_TPB, COLS && sizeof(T) == 4 ? 3 : 4) k_mx_q
                     const uint2 u = *(const uint2 *)(q + (8 * i + j) * PITCH);
                     w[0][j] = u.x;
                     w[1][j] = u.y;
-                    x = two_values<T, RANDOM>((const uint32_t *)&u, 0);
+                    x = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
                 } else {
                     w[0][j] = q[(8 * i + j) * PITCH];
-                    x = two_of(RANDOM ? w[0][j] & 0x7FFF7FFFu : w[0][j], T());
+                    x = two_of(w[0][j], T());
                 }
                 if (DROP) x = mx_mul2(x, make_float2(L.drop.factor, L.drop.factor));
-                x = mx_mul2(x, make_float2(inv[0], inv[1]));
+                if (RANDOM) x = make_float2(fabsf(x.x) * inv[0], fabsf(x.y) * inv[1]);   // (one by one the magnitude costs nothing)
+                else x = mx_mul2(x, make_float2(inv[0], inv[1]));
                 if (j & 1) f[0][j / 2].y = x.x, f[1][j / 2].y = x.y;
                 else f[0][j / 2].x = x.x, f[1][j / 2].x = x.y;
                 if (RANDOM) {
                     const uint32_t u = s_words[(32 * b + 8 * i + j) * (MX_TILE / 2) + p];
-                    bits16[1][j] = u >> 16;
-                    bits16[0][j] = u & 0xFFFFu;
+                    add[0][j] = mx_add_low(u);
+                    add[1][j] = mx_add_high(u);
                 }
             }
             if (RANDOM) {
@@ -480,8 +476,8 @@ __global__ void __launch_bounds__(MX_TPB, COLS && sizeof(T) == 4 ? 3 : 4) k_mx_q
                     signs[1] = signs8<3>(w[0]);
                 }
             }
-            codes[0][i] = codes8<RANDOM>(f[0], signs[0], bits16[0]);
-            codes[1][i] = codes8<RANDOM>(f[1], signs[1], bits16[1]);
+            codes[0][i] = codes8<RANDOM>(f[0], signs[0], add[0]);
+            codes[1][i] = codes8<RANDOM>(f[1], signs[1], add[1]);
         }
 #pragma unroll
         for (int h = 0; h < 2; h++) {
@@ -518,10 +514,10 @@ __global__ void __launch_bounds__(MX_TPB) k_mx_dequantize(const __grid_constant_
 
 // -------------------------------------------------------------- dropout
 template <typename T, bool RES>
-__device__ __forceinline__ void drop_pair(const mx_dropout_launch &L, mx_bits w, const T *x, const T *res, T *y) {
+__device__ __forceinline__ void drop_pair(const mx_dropout_launch &L, uint32_t w, const T *x, const T *res, T *y) {
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-        float f = (h ? w.high : w.low) < L.drop.threshold ? 0.0f : mx_f32(x[h]) * L.drop.factor;
+        float f = (h ? w >> 16 : w & 0xFFFFu) < L.drop.threshold ? 0.0f : mx_f32(x[h]) * L.drop.factor;
         if (RES) f = f + mx_f32(res[h]);
         mx_from(&y[h], f);
     }
@@ -553,7 +549,7 @@ __global__ void __launch_bounds__(MX_TPB) k_mx_dropout(const __grid_constant__ m
             const uint32_t start = mx_start(key, (uint64_t)at / 2);
             mx_vec8<T> o;
 #pragma unroll
-            for (int j = 0; j < 8; j += 2) drop_pair<T, RES>(L, mx_bits_of(key, start ^ (j / 2)), v.x + j, z.x + j, o.x + j);
+            for (int j = 0; j < 8; j += 2) drop_pair<T, RES>(L, mx_word(key, start ^ (j / 2)), v.x + j, z.x + j, o.x + j);
 #pragma unroll
             for (int j = 0; j < (int)(sizeof(o) / 16); j++) ((uint4 *)(y + i * 8))[j] = ((const uint4 *)&o)[j];
         }
@@ -570,7 +566,7 @@ __global__ void __launch_bounds__(MX_TPB) k_mx_dropout(const __grid_constant__ m
                 z[0] = res[at];
                 z[1] = two ? res[at + 1] : z[0];
             }
-            drop_pair<T, RES>(L, mx_bits_at(key, (uint64_t)(r * wide + c) / 2), v, z, o);
+            drop_pair<T, RES>(L, mx_word_at(key, (uint64_t)(r * wide + c) / 2), v, z, o);
             y[at] = o[0];
             if (two) y[at + 1] = o[1];
         }

@@ -89,19 +89,13 @@ __device__ __forceinline__ uint32_t mx_start(mx_key k, uint64_t pair) {
     }
     return s;
 }
-// The 16 bits of each of a pair of elements.
-struct mx_bits {
-    uint32_t low, high;
-};
-__device__ __forceinline__ mx_bits mx_bits_of(mx_key k, uint32_t start) {
+// The word of a pair of elements: the even one's 16 bits below, the odd one's above.
+__device__ __forceinline__ uint32_t mx_word(mx_key k, uint32_t start) {
     uint32_t x = start * 0x85EBCA6Bu;
     x = (x ^ (x >> 13) ^ k.b) * 0xC2B2AE35u;
-    mx_bits r;
-    r.high = x >> 16;
-    r.low = (x ^ r.high) & 0xFFFFu;
-    return r;
+    return x ^ (x >> 16);
 }
-__device__ __forceinline__ mx_bits mx_bits_at(mx_key k, uint64_t pair) { return mx_bits_of(k, mx_start(k, pair)); }
+__device__ __forceinline__ uint32_t mx_word_at(mx_key k, uint64_t pair) { return mx_word(k, mx_start(k, pair)); }
 __device__ __forceinline__ int64_t mx_wide(int64_t cols) { return (cols + MX_BLOCK - 1) / MX_BLOCK * MX_BLOCK; }
 
 // ---------------------------------------------------------- 4-bit rounding
@@ -163,19 +157,20 @@ __device__ __forceinline__ float2 mx_mul2_cut(float2 a, float2 b) {   // towards
 // pipe of multiplications, the other one bounds the rounding at random (4099 x
 // 50257 bf16 both ways: 313 us against 295).
 __device__ __constant__ uint32_t mx_p4 = 1u << 4, mx_p8 = 1u << 8, mx_p16 = 1u << 16;
-// The magnitude code of y * 2^-126 with these 16 bits: its bits + 64 * bits16
-// + 32, shifted right by 22.
-__device__ __forceinline__ uint32_t mx_code_random(float cut, uint32_t bits16) {
-    return (__float_as_uint(cut) + ((bits16 << 6) | 32u)) >> 22;
-}
+// What is added for the lower and for the upper 16 bits of a word: 64 times
+// them and 32.
+__device__ __forceinline__ uint32_t mx_add_low(uint32_t word) { return ((word << 6) & 0x3FFFC0u) | 32u; }
+__device__ __forceinline__ uint32_t mx_add_high(uint32_t word) { return ((word >> 10) & 0x3FFFC0u) | 32u; }
+// The magnitude code of y * 2^-126.
+__device__ __forceinline__ uint32_t mx_code_random(float cut, uint32_t add) { return (__float_as_uint(cut) + add) >> 22; }
 // Magnitude codes of 8 elements: y their magnitudes times 1 / scale, two by
-// two, and the bits of each.
-__device__ __forceinline__ uint32_t mx_codes8_random(const float2 *y, const uint32_t *bits16) {
+// two, and what is added to each.
+__device__ __forceinline__ uint32_t mx_codes8_random(const float2 *y, const uint32_t *add) {
     uint32_t p[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const float2 m = mx_mul2_cut(y[i], make_float2(MX_CUT, MX_CUT));
-        p[i] = mx_code_random(m.x, bits16[2 * i]) + mx_code_random(m.y, bits16[2 * i + 1]) * mx_p4;
+        p[i] = mx_code_random(m.x, add[2 * i]) + mx_code_random(m.y, add[2 * i + 1]) * mx_p4;
     }
     return (p[0] + p[1] * mx_p8) + (p[2] + p[3] * mx_p8) * mx_p16;
 }
@@ -216,11 +211,20 @@ __device__ __forceinline__ mx_vec8<T> load8(const T *p) {
     return v;
 }
 
-// What rounding needs of elements: their magnitudes' bits, compared as whole
-// numbers (two at a time where they have 16 bits), and float32 values.
+// What rounding needs of elements: the largest magnitude (of two at a time
+// where they have 16 bits; NaN where one is), as bits, and float32 values.
 __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b, float) { return max(a, b & 0x7FFFFFFFu); }
 template <typename T>
-__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b, T) { return __vmaxu2(a, b & 0x7FFF7FFFu); }
+__device__ __forceinline__ uint32_t larger2(uint32_t a, uint32_t b) {
+    T x, y;
+    memcpy(&x, &a, 4);
+    memcpy(&y, &b, 4);
+    x = __hmax2_nan(x, __habs2(y));   // (the magnitude is a modifier of the operand)
+    memcpy(&a, &x, 4);
+    return a;
+}
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b, __nv_bfloat16) { return larger2<__nv_bfloat162>(a, b); }
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b, __half) { return larger2<__half2>(a, b); }
 // The float32 bits of the largest, by the two halves of a 32-bit word for 16-bit types.
 __device__ __forceinline__ uint32_t top_low(uint32_t m, __nv_bfloat16) { return m << 16; }
 __device__ __forceinline__ uint32_t top_low(uint32_t m, __half) { return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m))); }
@@ -250,42 +254,33 @@ __device__ __forceinline__ uint32_t signs4x2(const uint32_t *w) {
 
 // The codes of 8 elements.  y: values (at random: magnitudes) times 1 / scale, two by two.
 template <bool RANDOM>
-__device__ __forceinline__ uint32_t codes8(const float2 *y, uint32_t signs, const uint32_t *bits16) {
-    if (RANDOM) return mx_codes8_random(y, bits16) | signs;
+__device__ __forceinline__ uint32_t codes8(const float2 *y, uint32_t signs, const uint32_t *add) {
+    if (RANDOM) return mx_codes8_random(y, add) | signs;
     return mx_codes8((const float *)y);
-}
-
-// The values of two words' elements, or of their magnitudes.
-template <typename T, bool RANDOM>
-__device__ __forceinline__ float2 two_values(const uint32_t *w, int i) {
-    if constexpr (sizeof(T) == 4) {
-        const uint32_t m = RANDOM ? 0x7FFFFFFFu : 0xFFFFFFFFu;
-        return make_float2(__uint_as_float(w[2 * i] & m), __uint_as_float(w[2 * i + 1] & m));
-    } else {
-        return two_of(RANDOM ? w[i] & 0x7FFF7FFFu : w[i], T());
-    }
 }
 
 // A row's 8 elements (raw words) to codes.
 template <typename T, bool RANDOM, bool DROP>
-__device__ __forceinline__ uint32_t row_codes(const uint32_t *w, float inv, float factor, const mx_bits *bits) {
+__device__ __forceinline__ uint32_t row_codes(const uint32_t *w, float inv, float factor, const uint32_t *words) {
     float2 y[4];
-    uint32_t bits16[8], signs = 0;
+    uint32_t add[8], signs = 0;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        y[i] = two_values<T, RANDOM>(w, i);
+        if constexpr (sizeof(T) == 4) y[i] = make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+        else y[i] = two_of(RANDOM ? w[i] & 0x7FFF7FFFu : w[i], T());
+        if (sizeof(T) == 4 && RANDOM) y[i] = make_float2(fabsf(y[i].x), fabsf(y[i].y));
         if (DROP) y[i] = mx_mul2(y[i], make_float2(factor, factor));
         y[i] = mx_mul2(y[i], make_float2(inv, inv));
         if (RANDOM) {
-            bits16[2 * i] = bits[i].low;
-            bits16[2 * i + 1] = bits[i].high;
+            add[2 * i] = mx_add_low(words[i]);
+            add[2 * i + 1] = mx_add_high(words[i]);
         }
     }
     if (RANDOM) {
         if constexpr (sizeof(T) == 4) signs = signs8<3>(w);
         else signs = signs4x2(w);
     }
-    return codes8<RANDOM>(y, signs, bits16);
+    return codes8<RANDOM>(y, signs, add);
 }
 
 }  // namespace

@@ -153,8 +153,8 @@ struct mx_cfg {
 template <typename T, bool DROP>
 __device__ __forceinline__ void put(const mx_product_launch &L, mx_key key, int64_t wide, int64_t t, int64_t n, float v) {
     if (DROP) {
-        const mx_bits w = mx_bits_at(key, (uint64_t)(t * wide + n) / 2);
-        v = ((n & 1) ? w.high : w.low) < L.drop.threshold ? 0.0f : v * L.drop.factor;
+        const uint32_t w = mx_word_at(key, (uint64_t)(t * wide + n) / 2);
+        v = ((n & 1) ? w >> 16 : w & 0xFFFFu) < L.drop.threshold ? 0.0f : v * L.drop.factor;
     }
     mx_from((T *)L.out + t * L.ld + n, v);
 }
@@ -723,9 +723,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mx_wide_cfg::THREADS
 #pragma unroll
                     for (int j = 0; j < CHUNK; j += 2) {
                         if (j % 8 == 0) start = mx_start(key, pos + j / 2);
-                        const mx_bits w = mx_bits_of(key, start ^ (j / 2 & 3));
-                        v[j] = w.low < L.drop.threshold ? 0.0f : v[j] * L.drop.factor;
-                        v[j + 1] = w.high < L.drop.threshold ? 0.0f : v[j + 1] * L.drop.factor;
+                        const uint32_t w = mx_word(key, start ^ (j / 2 & 3));
+                        v[j] = (w & 0xFFFFu) < L.drop.threshold ? 0.0f : v[j] * L.drop.factor;
+                        v[j + 1] = (w >> 16) < L.drop.threshold ? 0.0f : v[j + 1] * L.drop.factor;
                     }
                 }
                 bar_pair(1 + quarter);   // the last part has left the buffer

@@ -513,14 +513,33 @@ __global__ void __launch_bounds__(MX_TPB) k_mx_dequantize(const __grid_constant_
 }
 
 // -------------------------------------------------------------- dropout
+template <typename T>
+__device__ __forceinline__ float2 pair_of(const T *x) { return make_float2(mx_f32(x[0]), mx_f32(x[1])); }
+__device__ __forceinline__ void pair_from(float *y, float2 v) {
+    y[0] = v.x;
+    y[1] = v.y;
+}
+__device__ __forceinline__ void pair_from(__nv_bfloat16 *y, float2 v) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(v.x, v.y);
+    y[0] = p.x;
+    y[1] = p.y;
+}
+__device__ __forceinline__ void pair_from(__half *y, float2 v) {
+    const __half2 p = __floats2half2_rn(v.x, v.y);
+    y[0] = p.x;
+    y[1] = p.y;
+}
+
+// Two elements; `w`: their random word.  (The halves are compared in the upper
+// one: below the threshold there is below it here.)
 template <typename T, bool RES>
 __device__ __forceinline__ void drop_pair(const mx_dropout_launch &L, uint32_t w, const T *x, const T *res, T *y) {
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-        float f = (h ? w >> 16 : w & 0xFFFFu) < L.drop.threshold ? 0.0f : mx_f32(x[h]) * L.drop.factor;
-        if (RES) f = f + mx_f32(res[h]);
-        mx_from(&y[h], f);
-    }
+    const uint32_t threshold = L.drop.threshold << 16;
+    float2 f = mx_mul2(pair_of(x), make_float2(L.drop.factor, L.drop.factor));
+    if ((w << 16) < threshold) f.x = 0.0f;
+    if (w < threshold) f.y = 0.0f;
+    if (RES) f = mx_add2(f, pair_of(res));
+    pair_from(y, f);
 }
 
 template <typename T, bool RES>

@@ -139,6 +139,12 @@ __device__ __forceinline__ float2 mx_mul2(float2 a, float2 b) {
         "mov.b64 {%0, %1}, r;}" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return r;
 }
+__device__ __forceinline__ float2 mx_add2(float2 a, float2 b) {
+    float2 r;
+    asm("{.reg .b64 a, b, r;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 r, a, b;\n\t"
+        "mov.b64 {%0, %1}, r;}" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
 __device__ __forceinline__ float2 mx_mul2_cut(float2 a, float2 b) {   // towards 0
     float2 r;
     asm("{.reg .b64 a, b, r;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rz.f32x2 r, a, b;\n\t"

@@ -63,4 +63,6 @@ def dropout(x: torch.Tensor, p: float = 0.5, seed: int = 0, counter: Optional[to
     _mx4._check_p(p)
     if p == 0 and residual is None:
         return x
+    if not (torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad))):
+        return _run(x, residual, float(p), int(seed), counter)
     return _Dropout.apply(x, residual, float(p), int(seed), counter)

@@ -149,7 +149,7 @@ class Mx4Vector:
 class Mx4Matrix:
     """A matrix [rows, cols] in 4 bits, rounded along its rows, in the layout
     of the tensor cores (include/falcom_b200.h): `buffer`, one run of bytes,
-    holds `codes` and `scales`."""
+    holds `codes` and `scales`.  (Padding in it is 0: products count on it.)"""
 
     def __init__(self, rows: int, cols: int, buffer: torch.Tensor):
         codes, scales = self.sizes_of(rows, cols)
@@ -288,7 +288,8 @@ def quantize(x: torch.Tensor, along: str = "rows", rounding: str = "nearest", se
 def product(a: Union[torch.Tensor, Mx4Matrix], b: Mx4Matrix, dtype: torch.dtype = torch.bfloat16,
             out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """a @ b.t() in `dtype`, summed in float32.  A tensor `a` is rounded to the
-    nearest 4-bit values on the way; its leading dimensions stay."""
+    nearest 4-bit values on the way; its leading dimensions stay.  (For
+    answering: no gradients go through it, as they do through linear.)"""
     if not isinstance(b, Mx4Matrix):
         raise TypeError("b is not an Mx4Matrix: quantize it")
     if isinstance(a, Mx4Matrix):
@@ -341,29 +342,33 @@ def errors() -> int:
 
 # ------------------------------------------------------------------- layers
 
+def _linear_forward(x, w, p, seed, counter, need_x, need_w):
+    """y, the layer as the library has it, and what backward needs."""
+    lib, device = _library(), x.device
+    m, v = _rows(x, "x"), _rows(w, "weight")
+    (rows, cols), outs = m.shape, v.shape[0]
+    layer = abi.Mx4LinearC(rows, cols, outs, _TYPES[x.dtype], _TYPES[w.dtype], need_x, need_w, p,
+                           _seeded(seed, counter, device))
+    ref = ctypes.byref(layer)
+    kept = torch.empty(lib.falcom_mx4_linear_kept_bytes(ref), dtype=torch.uint8, device=device)
+    work = torch.empty(lib.falcom_mx4_linear_work_bytes(ref, 0), dtype=torch.uint8, device=device)
+    y = torch.empty((*x.shape[:-1], outs), dtype=x.dtype, device=device)
+    _done(lib.falcom_mx4_linear_forward(ref, m.data_ptr(), m.stride(0) if rows > 1 else cols, v.data_ptr(),
+                                        v.stride(0) if outs > 1 else cols, y.data_ptr(), kept.data_ptr(),
+                                        work.data_ptr(), _stream(device)), "falcom_mx4_linear_forward")
+    return y, layer, kept
+
+
 class _Linear(torch.autograd.Function):
     """falcom_mx4_linear_forward and _backward.  Rounding counts as the
     identity in the gradients; what is kept for them is in 4 bits."""
 
     @staticmethod
     def forward(ctx, x, w, p, seed, counter):
-        lib, device = _library(), x.device
-        m, v = _rows(x, "x"), _rows(w, "weight")
-        (rows, cols), outs = m.shape, v.shape[0]
-        need_x, need_w = ctx.needs_input_grad[:2]
-        random = _seeded(seed, counter, device)
-        layer = abi.Mx4LinearC(rows, cols, outs, _TYPES[x.dtype], _TYPES[w.dtype], need_x, need_w, p, random)
-        ref = ctypes.byref(layer)
-        kept = torch.empty(lib.falcom_mx4_linear_kept_bytes(ref), dtype=torch.uint8, device=device)
-        work = torch.empty(lib.falcom_mx4_linear_work_bytes(ref, 0), dtype=torch.uint8, device=device)
-        y = torch.empty((*x.shape[:-1], outs), dtype=x.dtype, device=device)
-        _done(lib.falcom_mx4_linear_forward(ref, m.data_ptr(), m.stride(0) if rows > 1 else cols, v.data_ptr(),
-                                            v.stride(0) if outs > 1 else cols, y.data_ptr(), kept.data_ptr(),
-                                            work.data_ptr(), _stream(device)), "falcom_mx4_linear_forward")
-        if need_x or need_w:
-            # the counter as it is now, whatever it is when the gradients are asked for
-            ctx.save_for_backward(kept, counter.clone() if counter is not None else None)
-            ctx.layer, ctx.of = layer, (x.shape, x.dtype, w.shape, w.dtype)
+        y, ctx.layer, kept = _linear_forward(x, w, p, seed, counter, *ctx.needs_input_grad[:2])
+        # the counter as it is now, whatever it is when the gradients are asked for
+        ctx.save_for_backward(kept, counter.clone() if counter is not None else None)
+        ctx.of = x.shape, x.dtype, w.shape, w.dtype
         return y
 
     @staticmethod
@@ -398,4 +403,6 @@ def linear(x: torch.Tensor, weight: torch.Tensor, p: float = 0.0, seed: int = 0,
         raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} do not go together")
     _same_device(x.device, weight=weight)
     _check_p(p)
+    if not (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad)):
+        return _linear_forward(x, weight, float(p), int(seed), counter, False, False)[0]
     return _Linear.apply(x, weight, float(p), int(seed), counter)

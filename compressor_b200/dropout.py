@@ -61,8 +61,8 @@ def dropout(x: torch.Tensor, p: float = 0.5, seed: int = 0, counter: Optional[to
             raise ValueError(f"residual is {residual.dtype} {tuple(residual.shape)} on {residual.device}, x {x.dtype} "
                              f"{tuple(x.shape)} on {x.device}")
     _mx4._check_p(p)
-    if p == 0 and residual is None:
-        return x
+    if p == 0:   # the rest is torch's
+        return x if residual is None else x + residual
     if not (torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad))):
         return _run(x, residual, float(p), int(seed), counter)
     return _Dropout.apply(x, residual, float(p), int(seed), counter)

@@ -241,7 +241,11 @@ __global__ void __launch_bounds__(MX_TPB) k_mx_decode(const __grid_constant__ mx
 // whose scales are one 512-byte piece of either layout.  Rows are rounded as
 // they come in (8 elements a thread, 4 threads a block); for the columns the
 // tile goes through shared memory, where a thread has a block of each of two
-// neighbouring columns, which share their random words.
+// neighbouring columns, which share their random words.  To the nearest it is
+// bound by memory (16384 x 4096 bf16: rows 36 us, both ways 50; the bytes at
+// the copy rate 26 and 31), at random by logic operations, some 22 an element
+// (both ways 87 us).  Loads of 4 rows a thread ahead of their use and 4 to 5
+// CTAs an SM made 133 us of it 96.
 #define MX_TILE 128
 
 // 8 elements from any address: the aligned 16-byte pieces that they lie in,
@@ -513,6 +517,8 @@ __global__ void __launch_bounds__(MX_TPB) k_mx_dequantize(const __grid_constant_
 }
 
 // -------------------------------------------------------------- dropout
+// Bound by memory: 16384 x 4096 bf16 in 49 us, with a residual in 65 (the bytes
+// at the copy rate: 41 and 62).
 template <typename T>
 __device__ __forceinline__ float2 pair_of(const T *x) { return make_float2(mx_f32(x[0]), mx_f32(x[1])); }
 __device__ __forceinline__ void pair_from(float *y, float2 v) {

@@ -126,10 +126,12 @@ __device__ uint32_t g_mx_error;   // a wait ran out
 // lanes of the sum), a's rows its N, so that neighbouring lanes are
 // neighbouring elements of a row of `out`, and few rows of a (tokens) cost a
 // narrow instruction instead of an empty one.  What bounds it is the way to b:
-// the stages of the CTAs of an SM (3 at most) take all its shared memory.  The
+// the stages of the CTAs of an SM (3 at most) take all its shared memory (1 x
+// 50257 x 1024 in a graph: 6.8 us, 4.2 of them for the bytes at the copy rate;
+// with 100 KB for each of 2 CTAs 9.3).  The
 // CTAs of a cluster have the same tile and a share of the panels each; their
-// sums meet in the order of the ranks.  TX: a is not in 4 bits yet but has elements of this type; each
-// CTA rounds what it needs (void: it is).
+// sums meet in the order of the ranks.  TX: a is not in 4 bits yet but has
+// elements of this type; each CTA rounds what it needs (void: it is).
 template <int BN, bool ROUND>
 struct mx_cfg {
     static constexpr int GROUPS = BN > 128 ? 2 : 1;                  // of a's rows with scales
@@ -140,9 +142,10 @@ struct mx_cfg {
     static constexpr int COLUMNS = BN <= 64 ? 128 : 2 * BN;
     static constexpr int SLOTS = (COLUMNS - BN) / SCALES, FIT = 222 * 1024 / STAGE;
     static constexpr int MOST = SLOTS < FIT ? SLOTS : FIT;
-    // CTAs that wait for columns may hold up others of their cluster, which have theirs: so whatever CTAs share an SM
-    // have columns for all, each taking at least as large a share of the shared memory (228 KB, 1 KB a CTA) as of the 512.
-    static constexpr int LEAST = BN == 256 ? 200 * 1024 : COLUMNS * 456 - 1024;
+    // CTAs that wait for columns may hold up others of their cluster, which have theirs: so whatever CTAs of these
+    // kernels share an SM have columns for all.  Each takes over a fifth of the SM's 228 KB of shared memory for each
+    // quarter of its 512 columns.
+    static constexpr int LEAST = COLUMNS * 368;
     static_assert(SUMS <= MOST, "");
     // E2M1 both, E8M0 scales, M = 128
     static constexpr uint32_t IDESC = 1u << 7 | 1u << 10 | (uint32_t)(BN / 8) << 17 | 1u << 23 | 1u << 27;
@@ -398,7 +401,9 @@ __global__ void __launch_bounds__(MX_THREADS) k_mx_product(const __grid_constant
 // `out` in its registers, rounds two at a time and stores 16 bytes at a time.
 // Two sums of 256 columns and the scales of 5 panels are more than the 512
 // columns there are, so the sums overlap by 128: those are read first, and the
-// next tile's first instruction waits for that alone.
+// next tile's first instruction waits for that alone.  Bound by the tensor pipe
+// at the clock that the power limit leaves (8192^3: 187 us, 5.9 PFLOP/s; 128 x
+// 256 a CTA 207), or by the way out of the results.
 struct mx_wide_cfg {
     static constexpr int BN = 256, THREADS = 320;                    // warps 0 to 7: results; 8: copies; 9: instructions
     static constexpr int A_BYTES = 128 * 128, B_BYTES = BN / 2 * 128;
@@ -407,7 +412,7 @@ struct mx_wide_cfg {
     static constexpr int SMEM = STAGES * STAGE + 4 * OUT + 1024;
     static constexpr int SECOND = 128, SCALES_AT = 384, SCALES = 24; // columns: a stage's scales have their own
     static constexpr uint32_t IDESC = 1u << 7 | 1u << 10 | (uint32_t)(BN / 8) << 17 | 1u << 23 | 2u << 27;
-    static_assert(SMEM <= 227 * 1024 && SCALES_AT + STAGES * SCALES <= 512 && SECOND + BN <= SCALES_AT, "");
+    static_assert(SMEM <= 227 * 1024 && SMEM >= 512 * 368 && SCALES_AT + STAGES * SCALES <= 512 && SECOND + BN <= SCALES_AT, "");
 };
 
 // The forms for a pair.

@@ -444,7 +444,7 @@ class Downlink:
     got them in full.  What one round rounds away is part of the next one's
     difference, so clients stay within one rounding of the server.  Lay tensors
     out with AggregateLayout.of(..., align=32) or a multiple: 32 consecutive
-    elements share a scale.
+    elements share a scale.  `weights` has to stay where it is.
 
         down = Downlink(weights)
         sent = down.send()                     # a round

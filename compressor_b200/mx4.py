@@ -157,9 +157,14 @@ class Mx4Matrix:
                 or not buffer.is_contiguous():
             raise ValueError(f"the buffer of {rows} x {cols} is {codes + scales} contiguous bytes")
         self.rows, self.cols, self.buffer = rows, cols, buffer
-        at = buffer.data_ptr()
-        self._c = abi.Mx4MatrixC(at, at + codes, rows, cols)
-        self._ref = ctypes.byref(self._c)
+        self._codes, self._c = codes, abi.Mx4MatrixC(None, None, rows, cols)
+
+    @property
+    def _ref(self):
+        """For a call: the buffer as it lies now."""
+        at = self.buffer.data_ptr()
+        self._c.codes, self._c.scales = at, at + self._codes
+        return ctypes.byref(self._c)
 
     @staticmethod
     def sizes_of(rows: int, cols: int) -> Tuple[int, int]:
@@ -174,11 +179,11 @@ class Mx4Matrix:
 
     @property
     def codes(self) -> torch.Tensor:
-        return self.buffer[:self.sizes_of(self.rows, self.cols)[0]]
+        return self.buffer[:self._codes]
 
     @property
     def scales(self) -> torch.Tensor:
-        return self.buffer[self.sizes_of(self.rows, self.cols)[0]:]
+        return self.buffer[self._codes:]
 
     @property
     def shape(self) -> Tuple[int, int]:

@@ -61,7 +61,8 @@ def test_product(mx4, t, n, k, dtype):
 
 # enough tiles for every SM to take several, rows of `out` at all offsets from 16 bytes, sums of one and of many panels
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("t,n,k", [(2048, 4096, 64), (1500, 5001, 300), (4099, 2051, 1025), (300, 20010, 256), (257, 19000, 2048)])
+@pytest.mark.parametrize("t,n,k", [(2048, 4096, 64), (1500, 5001, 300), (4099, 2051, 1025), (300, 20010, 256), (257, 19000, 2048),
+                                   (129, 20001, 300), (20001, 129, 257), (10007, 300, 64), (5000, 2304, 100)])
 def test_product_of_many_tiles(mx4, t, n, k, dtype):
     a, b = mx4.quantize(wild(t, k, torch.float32, 1).cuda()), mx4.quantize(wild(n, k, torch.float32, 2).cuda())
     room = torch.full((t * n + 64,), 7.0, dtype=dtype, device="cuda")

@@ -218,6 +218,28 @@ def test_dropout_in_place_and_refusals(mx4, dropout, product_lib):
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("p", [0.0, 0.3])
+@pytest.mark.parametrize("t,k,n", [(9, 70, 33), (700, 130, 20001)])
+def test_dropout_inside_rounding_and_product(mx4, p, t, k, n):
+    """The C calls' own dropout: the same as before the rounding, or after the
+    product, in the few-rows and the many-tiles form."""
+    import ctypes
+    from compressor_b200 import abi
+    lib, r, s = mx4._library(), ctypes.byref, torch.cuda.current_stream().cuda_stream
+    drop = abi.DropoutArgsC(p, abi.RandomC(5, None))
+    x = wild(t, k, torch.float32, 1)
+    rows, cols = mx4.Mx4Matrix.empty(t, k, "cuda"), mx4.Mx4Matrix.empty(k, t, "cuda")
+    assert lib.falcom_mx4_quantize(x.cuda().data_ptr(), 0, t, k, k, None, r(drop), rows._ref, cols._ref, s) == 0
+    d = ref.dropped(x, p, 5).float().cuda()
+    want = mx4.quantize(d, along="both")
+    assert torch.equal(rows.buffer, want[0].buffer) and torch.equal(cols.buffer, want[1].buffer)
+    b = mx4.quantize(wild(n, k, torch.float32, 2).cuda())
+    y = torch.empty(t, n, device="cuda")
+    assert lib.falcom_mx4_product(rows._ref, b._ref, y.data_ptr(), 0, n, r(drop), s) == 0
+    plain = mx4.product(rows, b, dtype=torch.float32).cpu()
+    assert torch.equal(y.cpu(), ref.dropped(plain, p, 5).float())
+
+
 def test_two_streams_give_the_same_bits(mx4, dropout):
     """Calls in flight at the same time share nothing."""
     x, w = wild(2050, 1030, torch.bfloat16, 1).cuda(), wild(4100, 1030, torch.float32, 2).cuda()

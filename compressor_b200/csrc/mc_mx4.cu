@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(MX_TPB) k_mx_decode(const __grid_constant__ mx
 // 8 elements from any address: the aligned 16-byte pieces that they lie in,
 // and one more, which may lie outside of them by up to 16 bytes at either end.
 template <typename T>
-struct mx_pieces {
+struct __align__(16) mx_pieces {
     uint32_t w[2 * sizeof(T) + 4];
 };
 template <typename T>
@@ -314,8 +314,7 @@ __global__ void __launch_bounds__(MX_TPB, COLS ? (sizeof(T) == 4 ? 3 : 4) : RAND
     // One row's 8 elements; `i` counts 16 rows.
     auto one = [&](mx_vec8<T> v, int i, bool inside) {
         const int y = ty + 16 * i;
-        uint32_t w[W];
-        uint32_t words[4];
+        __align__(16) uint32_t w[W], words[4];
         if (DROP) {
             const uint32_t start = mx_start(drop, pair);
 #pragma unroll

@@ -205,7 +205,7 @@ __device__ __forceinline__ int64_t mx_scale_at(int64_t rows, int64_t r, int64_t 
 
 // ------------------------------------------------------------- elements
 template <typename T>
-struct mx_vec8 {
+struct __align__(16) mx_vec8 {
     T x[8];
 };
 

@@ -54,7 +54,7 @@ static void array(mx_call *c, const char *what, const void *p, size_t bytes, siz
         c->device = at.device;
     }
     const uintptr_t lo = (uintptr_t)p, hi = lo + bytes;
-    if (!p || !check_argument(c->who, what, p, bytes, align, c->device)) {
+    if (!check_argument(c->who, what, p, bytes, align, c->device)) {
         c->ok = 0;
         return;
     }

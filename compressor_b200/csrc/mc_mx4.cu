@@ -639,8 +639,7 @@ static int quantize_as(mx_quantize_launch L, cudaStream_t s) {
     L.tiles = (uint32_t)x;
     const size_t smem = mx_tile<T, COLS, RANDOM>::BYTES;
     if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(k_mx_quantize<T, ROWS, COLS, RANDOM, DROP>,
-                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        const cudaError_t e = mx_allow(k_mx_quantize<T, ROWS, COLS, RANDOM, DROP>, smem);
         if (e != cudaSuccess) return e;
     }
     return mx_launch(k_mx_quantize<T, ROWS, COLS, RANDOM, DROP>, x * y, MX_TPB, smem, 0, s, L);

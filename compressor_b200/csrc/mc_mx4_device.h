@@ -19,6 +19,14 @@ __device__ __forceinline__ void mx_begin() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
+// More dynamic shared memory than a kernel may have unasked.
+template <typename K>
+static cudaError_t mx_allow(K kern, size_t smem) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) (void)cudaGetLastError();
+    return e;
+}
+
 // `cluster` > 0: of so many CTAs.
 template <typename... P, typename... A>
 static cudaError_t mx_launch(void (*kern)(P...), int64_t grid, int threads, size_t smem, int cluster, cudaStream_t s, const A &...args) {

@@ -781,7 +781,7 @@ template <typename T, bool DROP>
 static int product_wide(const mx_product_launch &L, int sms, cudaStream_t s) {
     typedef mx_wide_cfg C;
     auto kern = k_mx_product_wide<T, DROP>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    const cudaError_t e = mx_allow(kern, C::SMEM);
     if (e != cudaSuccess) return e;
     const int64_t tiles_n = (L.b.rows + C::BN - 1) / C::BN, tiles = tiles_n * ((L.a.rows + 255) / 256);
     if (tiles > 0x3FFFFFFF) return cudaErrorInvalidValue;
@@ -815,7 +815,7 @@ static int product_as(const mx_product_launch &L, int sms, cudaStream_t s) {
     if (stages > C::MOST) stages = C::MOST;
     const int need = own + stages * C::STAGE, smem = need < C::LEAST ? C::LEAST : need;
     auto kern = k_mx_product<T, BN, DROP, TX>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 225 * 1024);
+    const cudaError_t e = mx_allow(kern, 225 * 1024);
     if (e != cudaSuccess) return e;
     return mx_launch(kern, tiles * split, MX_THREADS, smem, split, s, L, (int)tiles_n, split, stages);
 }

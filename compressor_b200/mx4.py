@@ -318,7 +318,7 @@ def product(a: Union[torch.Tensor, Mx4Matrix], b: Mx4Matrix, dtype: torch.dtype 
 def _out(rows: int, b: Mx4Matrix, dtype: torch.dtype, out: Optional[torch.Tensor], lead) -> torch.Tensor:
     if out is None:
         _check_type(dtype)
-        return torch.empty((*lead, b.rows), dtype=dtype, device=b.device)
+        return torch.empty(*lead, b.rows, dtype=dtype, device=b.device)
     _check(out, "out")
     if out.numel() != rows * b.rows or not out.is_contiguous():
         raise ValueError(f"out must be {rows} x {b.rows} contiguous values, got {tuple(out.shape)} with strides "
@@ -357,7 +357,7 @@ def _linear_forward(x, w, p, seed, counter, need_x, need_w):
     ref = ctypes.byref(layer)
     kept = torch.empty(lib.falcom_mx4_linear_kept_bytes(ref), dtype=torch.uint8, device=device)
     work = torch.empty(lib.falcom_mx4_linear_work_bytes(ref, 0), dtype=torch.uint8, device=device)
-    y = torch.empty((*x.shape[:-1], outs), dtype=x.dtype, device=device)
+    y = torch.empty(*x.shape[:-1], outs, dtype=x.dtype, device=device)
     _done(lib.falcom_mx4_linear_forward(ref, m.data_ptr(), m.stride(0) if rows > 1 else cols, v.data_ptr(),
                                         v.stride(0) if outs > 1 else cols, y.data_ptr(), kept.data_ptr(),
                                         work.data_ptr(), _stream(device)), "falcom_mx4_linear_forward")

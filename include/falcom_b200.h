@@ -486,10 +486,11 @@ void falcom_adamw_destroy(falcom_adamw *plan);
  *
  * Common rules.  All data is device memory of one device; calls queue work
  * on `stream` (cudaStream_t of that device, NULL = its legacy default
- * stream), whatever device is current, need no workspace, may be captured,
- * and may run at the same time on several streams as long as their outputs
- * are apart.  Results are the same bits every time.  Element types are those
- * above, each array aligned to its element size; codes and scales 16 bytes.
+ * stream), whatever device is current, need no memory but what they are
+ * given, may be captured, and may run at the same time on several streams as
+ * long as their outputs are apart.  Results are the same bits every time.
+ * Element types are those above, each array aligned to its element size; codes
+ * and scales 16 bytes.
  * An output may not overlap anything else, but for dropout's y, which may be
  * x or the residual itself.  Return values: 0; ERROR_INVALID_PARAM for bad
  * arguments; ERROR_COMPRESSION when a launch fails or a CUDA error from

@@ -18,11 +18,13 @@ from . import mx4 as _mx4
 
 def _run(x: torch.Tensor, residual: Optional[torch.Tensor], p: float, seed: int, counter) -> torch.Tensor:
     x = x.contiguous()
+    if residual is not None:   # (as for x: a copy has to live until the call is made)
+        residual = residual.contiguous()
     y = torch.empty_like(x)
     cols = x.shape[-1] if x.dim() else 1
     args = abi.DropoutArgsC(p, _mx4._seeded(seed, counter, x.device))
     _mx4._done(_mx4._library().falcom_dropout(
-        x.data_ptr(), residual.contiguous().data_ptr() if residual is not None else None, y.data_ptr(),
+        x.data_ptr(), residual.data_ptr() if residual is not None else None, y.data_ptr(),
         _mx4._TYPES[x.dtype], x.numel() // cols if cols else 0, cols, ctypes.byref(args), _mx4._stream(x.device)),
         "falcom_dropout")
     return y

@@ -1,0 +1,24 @@
+"""GPU tests of what the 4-bit operators and dropout promise beside their
+values: operands of any strides."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+from tests.test_gpu_mx4 import wild  # noqa: E402
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_dropout_takes_residuals_of_any_strides(dtype):
+    from compressor_b200.dropout import dropout
+    x, whole = wild(65, 96, dtype, 1).cuda(), wild(130, 200, dtype, 2).cuda()
+    for r in (whole[:65, 3:99], whole[::2, 104:], whole.t()[7:72, 5:101], whole[4, :96].expand(65, 96), whole[:65, 9:10].expand(65, 96)):
+        assert not r.is_contiguous()
+        for a in (x, whole.t()[60:125, 20:116]):
+            want = dropout(a.contiguous(), 0.3, seed=4, residual=r.contiguous())
+            assert torch.equal(dropout(a, 0.3, seed=4, residual=r), want)
+            leaf = r.clone().requires_grad_()   # (the clone keeps the strides of views that have any)
+            y = dropout(a, 0.3, seed=4, residual=leaf)
+            assert torch.equal(y, want)
+            g, = torch.autograd.grad(y, leaf, whole.t()[:65, :96])
+            assert torch.equal(g, whole.t()[:65, :96])

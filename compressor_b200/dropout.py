@@ -55,7 +55,8 @@ def dropout(x: torch.Tensor, p: float = 0.5, seed: int = 0, counter: Optional[to
     dimension.  A dropped element is 0 whatever x holds there, infinity and NaN
     included, and so is its gradient.  Give each step and place a seed of its
     own, or a counter (an int64 tensor on the device, read when the work runs)
-    that is counted up.  Without a residual p = 0 returns x itself."""
+    that is counted up.  Without a residual p = 0 returns x itself.  Where p is
+    not 0 tangents of forward mode are refused (NotImplementedError)."""
     _mx4._check(x, "x")
     if residual is not None:
         _mx4._check(residual, "residual")
@@ -65,6 +66,6 @@ def dropout(x: torch.Tensor, p: float = 0.5, seed: int = 0, counter: Optional[to
     _mx4._check_p(p)
     if p == 0:   # the rest is torch's
         return x if residual is None else x + residual
-    if not (torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad))):
+    if not _mx4._differentiated(x, residual):
         return _run(x, residual, float(p), int(seed), counter)
     return _Dropout.apply(x, residual, float(p), int(seed), counter)

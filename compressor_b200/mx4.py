@@ -29,6 +29,7 @@ import ctypes
 from typing import Optional, Tuple, Union
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 from . import abi
 from . import optim as _optim
@@ -89,6 +90,17 @@ def _seeded(seed: int, counter: Optional[torch.Tensor], device) -> abi.RandomC:
             raise ValueError(f"counter must be one int64 on {device}")
         at = counter.data_ptr()
     return abi.RandomC(int(seed), at)
+
+
+def _differentiated(x: torch.Tensor, other: Optional[torch.Tensor]) -> bool:
+    """Whether autograd has to see a call: a gradient is wanted, or a tensor
+    carries a tangent of forward mode (autograd then raises, for want of a
+    rule).  Outside of a dual level there are none, and asking costs 1 us."""
+    if torch.is_grad_enabled() and (x.requires_grad or (other is not None and other.requires_grad)):
+        return True
+    if getattr(_forward_ad, "_current_level", 0) < 0:
+        return False
+    return any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in (x, other))
 
 
 def _check_p(p: float) -> None:
@@ -282,7 +294,8 @@ def quantize(x: torch.Tensor, along: str = "rows", rounding: str = "nearest", se
              counter: Optional[torch.Tensor] = None) -> Union[Mx4Matrix, Tuple[Mx4Matrix, Mx4Matrix]]:
     """x (all but its last dimension are rows) in 4 bits: along its "rows";
     along its "columns", which gives the transposed matrix; or "both", from one
-    read.  Products sum along the dimension that was rounded along."""
+    read.  Products sum along the dimension that was rounded along.  (No
+    gradients go through it, as none do through encode, decode and product.)"""
     if along not in ("rows", "columns", "both"):
         raise ValueError(f"along is 'rows', 'columns' or 'both', got {along!r}")
     x = _rows(x, "x")
@@ -401,13 +414,14 @@ def linear(x: torch.Tensor, weight: torch.Tensor, p: float = 0.0, seed: int = 0,
     """dropout(x, p) @ weight.t() with both factors in 4 bits, in x's type; the
     gradients' products have their factors in 4 bits too (the incoming gradient
     rounded at random).  weight [n, k] may have another type than x [..., k].
-    Give each step and layer a seed of its own, or a counter."""
+    Give each step and layer a seed of its own, or a counter.  Tangents of
+    forward mode are refused (NotImplementedError)."""
     for t, what in ((x, "x"), (weight, "weight")):
         _check(t, what)
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} do not go together")
     _same_device(x.device, weight=weight)
     _check_p(p)
-    if not (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad)):
+    if not _differentiated(x, weight):
         return _linear_forward(x, weight, float(p), int(seed), counter, False, False)[0]
     return _Linear.apply(x, weight, float(p), int(seed), counter)

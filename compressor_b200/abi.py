@@ -635,6 +635,9 @@ def bind_mx4(lib: ctypes.CDLL) -> None:
     P = ctypes.POINTER
     c_vp, size, c_int = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int
     lib.falcom_mx4_encode.argtypes = [c_vp, c_int, size, c_vp, P(RandomC), c_vp, c_vp, c_vp]
+    lib.falcom_mx4_encode_vector.argtypes = [c_vp, c_int, size, c_vp, P(RandomC), c_vp, c_vp]
+    lib.falcom_mx4_vector_bytes.argtypes = [size]
+    lib.falcom_mx4_vector_bytes.restype = size
     lib.falcom_mx4_decode.argtypes = [c_vp, c_vp, size, ctypes.c_float, c_int, c_vp, c_int, c_vp]
     for fn in (lib.falcom_mx4_codes_bytes, lib.falcom_mx4_scales_bytes, lib.falcom_mx4_work_bytes):
         fn.argtypes = [size, size]
@@ -651,7 +654,7 @@ def bind_mx4(lib: ctypes.CDLL) -> None:
     lib.falcom_mx4_product.argtypes = [P(Mx4MatrixC), P(Mx4MatrixC), c_vp, c_int, size, P(DropoutArgsC), c_vp]
     lib.falcom_mx4_errors.argtypes = []
     lib.falcom_dropout.argtypes = [c_vp, c_vp, c_vp, c_int, size, size, P(DropoutArgsC), c_vp]
-    for fn in (lib.falcom_mx4_encode, lib.falcom_mx4_decode, lib.falcom_mx4_quantize, lib.falcom_mx4_dequantize,
+    for fn in (lib.falcom_mx4_encode, lib.falcom_mx4_encode_vector, lib.falcom_mx4_decode, lib.falcom_mx4_quantize, lib.falcom_mx4_dequantize,
                lib.falcom_mx4_product, lib.falcom_mx4_product_of, lib.falcom_mx4_linear_forward,
                lib.falcom_mx4_linear_backward, lib.falcom_mx4_errors, lib.falcom_dropout):
         fn.restype = c_int

@@ -125,11 +125,21 @@ static int drop_of(mx_call *c, mx_drop *out, const falcom_dropout_args *d) {
 
 #define ROUNDING 0x9E3779B9u
 
-MC_EXPORT int falcom_mx4_encode(const void *x, int dtype, size_t n, float *base, const falcom_random *random,
-                                void *codes, void *scales, void *stream) {
-    static const char *who = "falcom_mx4_encode";
+#define VECTOR_ELEMENTS ((size_t)1 << 40)
+
+static size_t codes_of(size_t n) { return (n + 1) / 2; }
+/* Where a vector's scales begin in one run of bytes. */
+static size_t scales_at(size_t n) { return (codes_of(n) + 15) / 16 * 16; }
+
+MC_EXPORT size_t falcom_mx4_vector_bytes(size_t n) {
+    return n <= VECTOR_ELEMENTS ? scales_at(n) + (n + 31) / 32 : 0;
+}
+
+/* `scales` NULL: codes is the whole vector. */
+static int encode(const char *who, const void *x, int dtype, size_t n, float *base, const falcom_random *random,
+                  uint8_t *codes, uint8_t *scales, void *stream) {
     if (!known_type(dtype)) return invalid(who, "unknown type");
-    if (n > (size_t)1 << 40) return invalid(who, "too many elements");
+    if (n > VECTOR_ELEMENTS) return invalid(who, "too many elements");
     if (n == 0) return ERROR_NONE;
     mx_call c;
     mx_encode_launch L;
@@ -137,25 +147,42 @@ MC_EXPORT int falcom_mx4_encode(const void *x, int dtype, size_t n, float *base,
     begin(&c, who);
     array(&c, "x", x, n * g_type_size[dtype], g_type_size[dtype], 0);
     if (base) array(&c, "base", base, n * 4, 4, 1);
-    array(&c, "codes", codes, (n + 1) / 2, 16, 1);
-    array(&c, "scales", scales, (n + 31) / 32, 16, 1);
+    L.unit = scales ? 1 : 16;
+    if (scales) {
+        array(&c, "codes", codes, codes_of(n), 16, 1);
+        array(&c, "scales", scales, (n + 31) / 32, 16, 1);
+    } else {
+        array(&c, "the vector", codes, falcom_mx4_vector_bytes(n), 16, 1);
+    }
     random_of(&c, &L.random, random, ROUNDING);
     int prev, sms, rc = go(&c, &prev, &sms);
     if (rc) return rc;
     L.x = x;
     L.n = (int64_t)n;
     L.base = base;
-    L.codes = (uint8_t *)codes;
-    L.scales = (uint8_t *)scales;
+    L.codes = codes;
+    L.scales = scales ? scales : codes + scales_at(n);
     L.vectors = (((uintptr_t)x | (uintptr_t)base) & 15) == 0;
     return done(&c, prev, mc_launch_mx_encode(&L, dtype, stream));
+}
+
+MC_EXPORT int falcom_mx4_encode(const void *x, int dtype, size_t n, float *base, const falcom_random *random,
+                                void *codes, void *scales, void *stream) {
+    static const char *who = "falcom_mx4_encode";
+    if (n > 0 && !scales) return invalid(who, "no scales");
+    return encode(who, x, dtype, n, base, random, (uint8_t *)codes, (uint8_t *)scales, stream);
+}
+
+MC_EXPORT int falcom_mx4_encode_vector(const void *x, int dtype, size_t n, float *base, const falcom_random *random,
+                                       void *vector, void *stream) {
+    return encode("falcom_mx4_encode_vector", x, dtype, n, base, random, (uint8_t *)vector, NULL, stream);
 }
 
 MC_EXPORT int falcom_mx4_decode(const void *codes, const void *scales, size_t n, float weight, int accumulate,
                                 void *out, int dtype, void *stream) {
     static const char *who = "falcom_mx4_decode";
     if (!known_type(dtype)) return invalid(who, "unknown type");
-    if (n > (size_t)1 << 40 || !isfinite(weight)) return invalid(who, "too many elements, or a weight that is not finite");
+    if (n > VECTOR_ELEMENTS || !isfinite(weight)) return invalid(who, "too many elements, or a weight that is not finite");
     if (n == 0) return ERROR_NONE;
     mx_call c;
     begin(&c, who);

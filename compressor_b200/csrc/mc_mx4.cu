@@ -59,6 +59,10 @@ __device__ __forceinline__ void store_up_to_8(T *p, const float *v, int n) {
         if (j < n) mx_from(&p[j], v[j]);
 }
 
+// Bytes of the codes of n elements, filled up to a multiple of `unit` (1 or 16).
+template <typename I>
+__device__ __forceinline__ I code_bytes(I n, int unit) { return (n + 2 * unit - 1) / 2 & -unit; }
+
 template <typename T, bool BASE, bool RANDOM>
 __global__ void __launch_bounds__(MX_TPB) k_mx_encode8(const __grid_constant__ mx_encode_launch L) {
     mx_begin();
@@ -111,8 +115,8 @@ __global__ void __launch_bounds__(MX_TPB) k_mx_encode8(const __grid_constant__ m
             store_up_to_8(L.base + 8 * i, held.x, left);
         }
         if (left == 8) ((uint32_t *)L.codes)[i] = codes;
-        else
-            for (int j = 0; j < (left + 1) / 2; j++) L.codes[4 * i + j] = (uint8_t)(codes >> (8 * j));
+        else   // (the codes behind the last element are 0, and so is what lies between them and the scales)
+            for (int j = 0, end = min((int)(code_bytes(L.n, L.unit) - 4 * i), 4); j < end; j++) L.codes[4 * i + j] = (uint8_t)(codes >> (8 * j));
         if ((i & 3) == 0 && left > 0) L.scales[i / 4] = (uint8_t)s;
     }
 }
@@ -193,7 +197,7 @@ __global__ void __launch_bounds__(MX_TPB) k_mx_encode(const __grid_constant__ mx
         // lane 8 g + b: elements 8 g .. 8 g + 7 of block b
         codes = transpose8(codes, lane);
         const int word = (lane & 7) * 4 + (lane >> 3);   // of the chunk's 32
-        const int bytes = (left + 1) / 2;
+        const int bytes = code_bytes(left, L.unit);
         uint8_t *out = L.codes + c * 128 + 4 * word;
         if (4 * word + 4 <= bytes) *(uint32_t *)out = codes;
         else

@@ -47,6 +47,7 @@ typedef struct {
     uint8_t *codes, *scales;
     mx_random random;
     int32_t vectors;           /* x and base on 16-byte boundaries */
+    int32_t unit;              /* codes are filled up to a multiple of so many bytes: 1, or 16 where scales follow */
 } mx_encode_launch;
 
 typedef struct {

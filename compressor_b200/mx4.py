@@ -124,7 +124,8 @@ def _scales_from(n: int) -> int:
 
 class Mx4Vector:
     """A vector in 4 bits: `buffer`, one run of bytes (to broadcast, to save),
-    holds `codes` and, from the next multiple of 16 on, `scales`."""
+    holds `codes` and, from the next multiple of 16 on, `scales`.  (The bytes
+    between them, up to 15, are 0.)"""
 
     def __init__(self, n: int, buffer: torch.Tensor):
         if buffer.dtype != torch.uint8 or buffer.dim() != 1 or buffer.numel() != self.size_of(n) \
@@ -146,8 +147,7 @@ class Mx4Vector:
 
     @staticmethod
     def empty(n: int, device) -> "Mx4Vector":
-        """For a receiver: the buffer that a sent one is copied into.  (Zeroed:
-        the bytes between codes and scales, up to 15, are nobody's.)"""
+        """For a receiver: the buffer that a sent one is copied into (zeros until then)."""
         return Mx4Vector(n, torch.zeros(Mx4Vector.size_of(n), dtype=torch.uint8, device=device))
 
     @property
@@ -231,11 +231,10 @@ def encode(x: torch.Tensor, base: Optional[torch.Tensor] = None, rounding: str =
         _same_device(x.device, base=base)
     random = _random(rounding, seed, counter, x.device)
     n = x.numel()
-    # not zeroed: the kernel writes all but the bytes between codes and scales
-    sent = Mx4Vector(n, torch.empty(Mx4Vector.size_of(n), dtype=torch.uint8, device=x.device))
-    at = sent.buffer.data_ptr()
-    _done(_library().falcom_mx4_encode(x.data_ptr(), _TYPES[x.dtype], n, base.data_ptr() if base is not None else None,
-                                       _ref(random), at, at + _scales_from(n), _stream(x.device)), "falcom_mx4_encode")
+    sent = Mx4Vector(n, torch.empty(Mx4Vector.size_of(n), dtype=torch.uint8, device=x.device))   # written whole
+    _done(_library().falcom_mx4_encode_vector(x.data_ptr(), _TYPES[x.dtype], n,
+                                              base.data_ptr() if base is not None else None, _ref(random),
+                                              sent.buffer.data_ptr(), _stream(x.device)), "falcom_mx4_encode_vector")
     if base is not None:
         torch.autograd.graph.increment_version(base)
     return sent

@@ -513,9 +513,15 @@ typedef struct falcom_dropout_args {
  * is part of the next difference.
  * falcom_mx4_decode: v = weight * value (float32, rounded once);
  * out = v, or out = out + v with accumulate (each rounded to float32, then
- * to out's type). */
+ * to out's type).
+ * A vector to send or to save as one run of bytes: the codes, 0 up to the next
+ * multiple of 16, the scales; falcom_mx4_vector_bytes gives the size (0 for
+ * more than 2^40 elements) and falcom_mx4_encode_vector writes every byte. */
 int falcom_mx4_encode(const void *x, int dtype, size_t n, float *base, const falcom_random *random, void *codes,
                       void *scales, void *stream);
+size_t falcom_mx4_vector_bytes(size_t n);
+int falcom_mx4_encode_vector(const void *x, int dtype, size_t n, float *base, const falcom_random *random, void *vector,
+                             void *stream);
 int falcom_mx4_decode(const void *codes, const void *scales, size_t n, float weight, int accumulate, void *out,
                       int dtype, void *stream);
 

@@ -1,5 +1,5 @@
 """GPU tests of what the 4-bit operators and dropout promise beside their
-values: operands of any strides."""
+values: operands of any strides, and every byte of what is sent."""
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -22,3 +22,19 @@ def test_dropout_takes_residuals_of_any_strides(dtype):
             assert torch.equal(y, want)
             g, = torch.autograd.grad(y, leaf, whole.t()[:65, :96])
             assert torch.equal(g, whole.t()[:65, :96])
+
+
+@pytest.mark.parametrize("n", [1, 31, 33, 256, 1000, 5130, 70001])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_every_byte_of_a_vector_is_written(n, shift):
+    """Memory that held something else: the bytes between codes and scales,
+    which are nobody's, are 0, and two encodes give the same buffer."""
+    from compressor_b200 import mx4
+    x = wild(1, n + shift, torch.float32, 3).cuda()[0, shift:]
+    buffers = []
+    for fill in (0xA5, 0x3C):
+        room = [torch.full((mx4.Mx4Vector.size_of(n),), fill, dtype=torch.uint8, device="cuda") for _ in range(4)]
+        del room
+        buffers.append(mx4.encode(x).buffer)
+    codes, scales = (n + 1) // 2, buffers[0].numel() - -(-n // 32)
+    assert torch.equal(buffers[0], buffers[1]) and not buffers[0][codes:scales].any()

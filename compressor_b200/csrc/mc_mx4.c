@@ -492,11 +492,18 @@ MC_EXPORT int falcom_mx4_linear_backward(const falcom_mx4_linear *l, const void 
 }
 
 MC_EXPORT int falcom_mx4_errors(void) {
-    uint32_t word = 0;
-    cudaError_t e = cudaDeviceSynchronize();
-    if (e == cudaSuccess) e = (cudaError_t)mc_mx_errors(&word);
-    if (e != cudaSuccess) return ERROR_COMPRESSION;
-    return word != 0;
+    static uint32_t reported[64];   /* of each device: CTAs that gave up, which the kernels count */
+    uint32_t count = 0, before;
+    int device = -1;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e == cudaSuccess) e = cudaDeviceSynchronize();
+    if (e == cudaSuccess) e = (cudaError_t)mc_mx_errors(&count);
+    if (e != cudaSuccess || device < 0 || device >= 64) return ERROR_COMPRESSION;
+    before = __atomic_load_n(&reported[device], __ATOMIC_RELAXED);
+    do {   /* (a later count that another thread reported stays) */
+        if ((int32_t)(count - before) <= 0) return 0;
+    } while (!__atomic_compare_exchange_n(&reported[device], &before, count, 0, __ATOMIC_RELAXED, __ATOMIC_RELAXED));
+    return 1;
 }
 
 MC_EXPORT int falcom_dropout(const void *x, const void *residual, void *y, int dtype, size_t rows, size_t cols,

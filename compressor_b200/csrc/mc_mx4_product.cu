@@ -27,6 +27,9 @@ __device__ __forceinline__ void bulk_g2s(uint32_t dst, const void *src, uint32_t
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
 __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
     uint32_t done;
     asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
@@ -34,8 +37,8 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
     return done != 0;
 }
 // Every wait is bounded: false when it ran out (some seconds).  The clock is
-// looked at late and rarely.
-__device__ __noinline__ bool mbar_wait_long(uint32_t bar, uint32_t parity, uint32_t seconds) {
+// looked at late and rarely, and so is `failed` (or NULL), which ends the wait.
+__device__ __noinline__ bool mbar_wait_long(uint32_t bar, uint32_t parity, uint32_t seconds, const volatile uint32_t *failed) {
     uint64_t t0, t;
     for (int i = 0; i < 256; i++)
         if (mbar_try_wait(bar, parity)) return true;
@@ -43,12 +46,12 @@ __device__ __noinline__ bool mbar_wait_long(uint32_t bar, uint32_t parity, uint3
     for (uint32_t i = 0; i < 1u << 26; i++) {
         if (mbar_try_wait(bar, parity)) return true;
         asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-        if (t - t0 > seconds * 1000000000ull) return false;
+        if (t - t0 > seconds * 1000000000ull || (failed && *failed)) return false;
     }
     return false;
 }
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint32_t seconds) {
-    return mbar_try_wait(bar, parity) || mbar_wait_long(bar, parity, seconds);
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint32_t seconds, const volatile uint32_t *failed = NULL) {
+    return mbar_try_wait(bar, parity) || mbar_wait_long(bar, parity, seconds, failed);
 }
 
 // The same for a barrier at which threads of another CTA of the cluster arrive.
@@ -59,7 +62,7 @@ __device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t par
     return done != 0;
 }
 __device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, uint32_t seconds) {
-    return mbar_try_wait_cluster(bar, parity) || (mbar_wait_long(bar, parity, seconds) && mbar_try_wait_cluster(bar, parity));
+    return mbar_try_wait_cluster(bar, parity) || (mbar_wait_long(bar, parity, seconds, NULL) && mbar_try_wait_cluster(bar, parity));
 }
 
 __device__ __forceinline__ bool elect_one() {
@@ -119,7 +122,10 @@ __device__ __forceinline__ uint64_t desc_scales(uint32_t at) {
     return (uint64_t)(at >> 4 & 0x3FFF) | 1ull << 16 | 8ull << 32 | 1ull << 46;
 }
 
-__device__ uint32_t g_mx_error;   // a wait ran out
+// CTAs in which a wait ran out.  Sums that may lack a part are then never said
+// to be done, and who waits for them leaves NaN.
+__device__ uint32_t g_mx_error;
+#define MX_NAN 0x7FFFFFFFu
 
 // ------------------------------------------------------------------ narrow
 // Few tiles.  One tile of 128 x BN a CTA: b's rows are the instruction's M (128
@@ -224,12 +230,21 @@ __device__ __forceinline__ void meet(const mx_product_launch &L, mx_key key, int
     }
 }
 
+// What failed leaves NaN.
+__device__ __noinline__ void nan_sums(uint32_t at, int rows) {
+    for (int c = 0; c < rows; c++) asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + c * 512), "r"(MX_NAN) : "memory");
+}
+template <typename T, bool DROP>
+__device__ __noinline__ void nan_out(const mx_product_launch &L, mx_key key, int64_t wide, int64_t t0, int64_t n, int rows) {
+    for (int c = 0; c < rows; c++) put<T, DROP>(L, key, wide, t0 + c, n, __uint_as_float(MX_NAN));
+}
+
 template <typename T, int BN, bool DROP, typename TX>
 __global__ void __launch_bounds__(MX_THREADS) k_mx_product(const __grid_constant__ mx_product_launch L, int tiles_n, int split, int stages) {
     constexpr bool ROUND = !std::is_same<TX, void>::value;
     typedef mx_cfg<BN, ROUND> C;
     extern __shared__ uint8_t s_raw[];
-    __shared__ __align__(8) uint64_t s_full[C::MOST], s_empty[C::MOST], s_done, s_rounded;
+    __shared__ __align__(8) uint64_t s_full[C::MOST], s_empty[C::MOST], s_done, s_quiet, s_stopped, s_rounded;
     __shared__ uint32_t s_tmem;
     __shared__ volatile uint32_t s_failed;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -247,6 +262,8 @@ __global__ void __launch_bounds__(MX_THREADS) k_mx_product(const __grid_constant
             mbar_init(smem_u32(&s_empty[i]), 1);
         }
         mbar_init(smem_u32(&s_done), 1);
+        mbar_init(smem_u32(&s_quiet), 1);
+        mbar_init(smem_u32(&s_stopped), 1);
         mbar_init(smem_u32(&s_rounded), 128);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         s_failed = 0;
@@ -292,6 +309,7 @@ __global__ void __launch_bounds__(MX_THREADS) k_mx_product(const __grid_constant
             }
             mbar_wait(smem_u32(&s_full[s]), round & 1, 2);
         }
+        mbar_arrive(smem_u32(&s_quiet));
     }
     if (warp == 5 && elect_one()) {
         bool ok = !ROUND || mbar_wait(smem_u32(&s_rounded), 0, 8);
@@ -325,21 +343,29 @@ __global__ void __launch_bounds__(MX_THREADS) k_mx_product(const __grid_constant
                 round++;
             }
         }
-        if (!ok) s_failed = 1;
-        tc_commit(smem_u32(&s_done));
+        if (ok) {
+            tc_commit(smem_u32(&s_done));
+        } else {   // what was issued ends before the memory goes
+            s_failed = 1;
+            tc_commit(smem_u32(&s_stopped));
+            mbar_wait(smem_u32(&s_stopped), 0, 2);
+        }
     }
     if constexpr (ROUND) {
         if (warp < 4) {
             round_rows<TX, BN>(L, own, C::A_ALL, p0, p1);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // for the tensor core
-            asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&s_rounded)) : "memory");
+            mbar_arrive(smem_u32(&s_rounded));
         }
     }
     __syncwarp();
 
-    bool fine = true;
-    if (warp < 4) fine = mbar_wait(smem_u32(&s_done), 0, 16);
-    if (!fine) s_failed = 1;
+    bool failed = false;
+    if (warp < 4) failed = !mbar_wait(smem_u32(&s_done), 0, 16, &s_failed);
+    if (failed) {
+        s_failed = 1;
+        mbar_wait(smem_u32(&s_quiet), 0, 60);   // no copy that is late may come over what is left instead of the sums
+    }
     tc_after_sync();
     const int64_t n = n0 + 32 * warp + lane;
     const int valid = (int)min((int64_t)BN, L.a.rows - t0);
@@ -355,11 +381,12 @@ __global__ void __launch_bounds__(MX_THREADS) k_mx_product(const __grid_constant
                 __syncwarp();
                 tc_ld16(mine + c, r);
                 tc_wait_ld();
-                if (n < L.b.rows && fine)
+                if (n < L.b.rows && !failed)
 #pragma unroll
                     for (int j = 0; j < 16; j++)
                         if (c + j < valid) put<T, DROP>(L, key, wide, t0 + c + j, n, panels ? __uint_as_float(r[j]) : 0.0f);
             }
+            if (failed && n < L.b.rows) nan_out<T, DROP>(L, key, wide, t0, n, valid);
         }
     } else {
         // [BN][128] float32 over the stages, which are all used up
@@ -373,11 +400,12 @@ __global__ void __launch_bounds__(MX_THREADS) k_mx_product(const __grid_constant
                 for (int j = 0; j < 16; j++)
                     asm volatile("st.shared.b32 [%0], %1;" ::"r"(smem + ((c + j) * 128 + 32 * warp + lane) * 4), "r"(r[j]) : "memory");
             }
+        if (failed) nan_sums(smem + threadIdx.x * 4, valid);
         __syncwarp();
         cluster_sync();
         if (warp < 4) {
             const int from = valid * rank / split, to = valid * (rank + 1) / split;
-            const bool inside = n < L.b.rows && fine;
+            const bool inside = n < L.b.rows;
             if (split == 2) meet<T, 2, DROP>(L, key, wide, smem, t0, n, from, to, inside);
             else if (split == 4) meet<T, 4, DROP>(L, key, wide, smem, t0, n, from, to, inside);
             else meet<T, 8, DROP>(L, key, wide, smem, t0, n, from, to, inside);
@@ -387,7 +415,7 @@ __global__ void __launch_bounds__(MX_THREADS) k_mx_product(const __grid_constant
     }
     tc_before_sync();
     __syncthreads();
-    if (threadIdx.x == 0 && s_failed) atomicExch(&g_mx_error, 1u);
+    if (threadIdx.x == 0 && s_failed) atomicAdd(&g_mx_error, 1u);
     if (warp == 5) tmem_free<C::COLUMNS>(tmem);
 }
 
@@ -444,6 +472,11 @@ __device__ __forceinline__ void tc_commit_pair(uint32_t bar) {
 __device__ __forceinline__ void mbar_arrive_first(uint32_t bar) {
     asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, 0;\n\t"
                  "mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [a];\n\t}" ::"r"(bar) : "memory");
+}
+// A word of the second CTA's.
+__device__ __forceinline__ void st_second(uint32_t at, uint32_t v) {
+    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, 1;\n\tst.shared::cluster.b32 [a], %1;\n\t}"
+                 ::"r"(at), "r"(v) : "memory");
 }
 // A box of rows from `row` on to this CTA's shared memory, which the first
 // CTA's barrier is told.
@@ -571,7 +604,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mx_wide_cfg::THREADS
     constexpr int CHUNK = 128 / sizeof(T), PARTS = 64 / CHUNK, E = 16 / sizeof(T), BN = C::BN, COPIES = 8, ISSUE = 9;
     extern __shared__ uint8_t s_raw[];
     // s_full: both CTAs' copies, at the first; s_done, s_free: for even and for odd tiles
-    __shared__ __align__(8) uint64_t s_full[C::STAGES], s_empty[C::STAGES], s_done[2], s_free[2];
+    __shared__ __align__(8) uint64_t s_full[C::STAGES], s_empty[C::STAGES], s_done[2], s_free[2], s_stopped;
     __shared__ uint32_t s_tmem;
     __shared__ volatile uint32_t s_failed;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -589,6 +622,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mx_wide_cfg::THREADS
             mbar_init(smem_u32(&s_done[i]), 1);
             mbar_init(smem_u32(&s_free[i]), 16);   // the result warps of both
         }
+        mbar_init(smem_u32(&s_stopped), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         s_failed = 0;
     }
@@ -679,15 +713,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mx_wide_cfg::THREADS
                     parity ^= 1;
                 }
             }
-            if (!ok) {
-                s_failed = 1;
-                break;
-            }
+            if (!ok) break;
             tc_commit_pair(smem_u32(&s_done[count & 1]));
         }
         if (!ok) {   // what was issued ends before the memory goes
-            tc_commit_pair(smem_u32(&s_done[count & 1]));
-            mbar_wait(smem_u32(&s_done[count & 1]), count >> 1 & 1, 2);
+            s_failed = 1;
+            st_second(smem_u32((const void *)&s_failed), 1);
+            tc_commit_pair(smem_u32(&s_stopped));
+            mbar_wait(smem_u32(&s_stopped), 0, 2);
         }
     }
     __syncwarp();
@@ -699,11 +732,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mx_wide_cfg::THREADS
         mx_key key = {};
         if (DROP) key = mx_key_of(L.drop.random);
         int count = 0;
+        bool failed = false;   // the tiles that follow are not summed either
         for (int tile = pair; tile < tiles; tile += pairs, count++) {
             const int64_t n0 = (int64_t)(tile % tiles_n) * BN, t0 = (int64_t)(tile / tiles_n) * 256 + 128 * rank + 32 * quarter;
             const int rows = (int)max((int64_t)0, min((int64_t)32, L.a.rows - t0)), columns = (int)min((int64_t)BN, L.b.rows - n0);
             uint8_t *out = (uint8_t *)L.out + t0 * ld_bytes + n0 * (int64_t)sizeof(T);
-            if (!s_failed && !mbar_wait(smem_u32(&s_done[count & 1]), count >> 1 & 1, 20)) s_failed = 1;
+            if (!failed) failed = !mbar_wait(smem_u32(&s_done[count & 1]), count >> 1 & 1, 20, &s_failed);
+            if (failed) s_failed = 1;
             tc_after_sync();
             const uint32_t mine = tmem + (count & 1) * C::SECOND + ((uint32_t)(32 * quarter) << 16);
             // first the overlap: columns 128 on of even tiles, the first 128 of odd ones
@@ -715,6 +750,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mx_wide_cfg::THREADS
 #pragma unroll
                     for (int j = 0; j < CHUNK; j += 16) tc_ld16(mine + c + j, (uint32_t *)v + j);
                     tc_wait_ld();
+                    if (failed)
+#pragma unroll
+                        for (int j = 0; j < CHUNK; j++) v[j] = __uint_as_float(MX_NAN);
                 }
                 if (k == PARTS - 1) {   // the overlap is read, and all of the tile before
                     tc_before_sync();
@@ -737,14 +775,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mx_wide_cfg::THREADS
 #pragma unroll
                 for (int j = 0; j < CHUNK; j += E) st_shared16(buf + lane * C::PITCH + (set * CHUNK + j) * sizeof(T), pack16(v + j, T()));
                 bar_pair(1 + quarter);
-                if (!s_failed)
-                    rows_out<T>(buf, out + both * (int64_t)sizeof(T), ld_bytes, rows, min(2 * CHUNK, columns - both), set, lane, even);
+                rows_out<T>(buf, out + both * (int64_t)sizeof(T), ld_bytes, rows, min(2 * CHUNK, columns - both), set, lane, even);
             }
         }
     }
     tc_before_sync();
     __syncthreads();
-    if (threadIdx.x == 0 && s_failed) atomicExch(&g_mx_error, 1u);
+    if (threadIdx.x == 0 && s_failed) atomicAdd(&g_mx_error, 1u);
     cluster_sync();   // nothing of the pair is in use any more
     tc_after_sync();
     if (warp == ISSUE) tmem_free_pair(tmem);

@@ -351,9 +351,9 @@ def _product(a: Mx4Matrix, b: Mx4Matrix, dtype: torch.dtype, out: Optional[torch
 
 
 def errors() -> int:
-    """Nonzero once a product on the current device gave up waiting for its own
-    copies (never seen): what it left is then not to be used.  Waits for the
-    device."""
+    """Nonzero when a product on the current device gave up waiting for its own
+    copies since the last call that said so (never seen): results that may lack
+    a part are NaN then.  Waits for the device."""
     return _library().falcom_mx4_errors()
 
 

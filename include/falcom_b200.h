@@ -593,8 +593,9 @@ int falcom_mx4_linear_forward(const falcom_mx4_linear *layer, const void *x, siz
 int falcom_mx4_linear_backward(const falcom_mx4_linear *layer, const void *dy, size_t ld_dy, const void *kept, void *dx,
                                void *dw, void *work, void *stream);
 /* 1 when a product on the current device gave up waiting for its own copies
- * (some seconds; its result is then not to be used), else 0; negative when
- * the device cannot be asked.  Waits for the device, so it does not belong
+ * (some seconds) since the last call that said so, else 0; negative when the
+ * device cannot be asked.  Results that may lack a part are NaN then (but for
+ * elements that dropout makes 0).  Waits for the device, so it does not belong
  * inside a stream capture. */
 int falcom_mx4_errors(void);
 

@@ -61,7 +61,8 @@ extern "C" int mc_launch_mx_product(const mx_product_launch *L, int type, int sm
         }
     return 0;
 }
-extern "C" int mc_mx_errors(uint32_t *word) { *word = 0; return 0; }
+extern "C" __attribute__((visibility("default"))) uint32_t emu_mx4_gave_up = 0;   // CTAs, for a test to count up
+extern "C" int mc_mx_errors(uint32_t *word) { *word = emu_mx4_gave_up; return 0; }
 """
 
 

@@ -35,7 +35,13 @@ BODIES = {
     "mbar_expect_tx": " emu_arrive(bar, -1, (int)bytes); ",
     "bulk_g2s": " emu_copy(dst, (const uint8_t *)src, bytes, bar, -1); ",
     "mbar_try_wait": " return emu_done(bar, parity, 0); ",
-    "mbar_wait_long": " return emu_done(bar, parity, seconds); ",
+    "mbar_wait_long": """
+    for (double t = 0; t < seconds; t += 0.25) {
+        if (emu_done(bar, parity, 0.25)) return true;
+        if (failed && *failed) return false;
+    }
+    return false;
+""",
     "mbar_try_wait_cluster": " return emu_done(bar, parity, 0); ",
     "elect_one": " return (threadIdx.x & 31) == 0; ",
     "tmem_alloc": " emu_tmem_alloc(dst, COLUMNS); ",
@@ -49,6 +55,8 @@ BODIES = {
     "tc_ld16": " emu_tmem_load(at, r, 16); ",
     "cluster_sync": " emu_cluster->all.wait(); ",
     "ld_cluster": " return emu_load<float>(at, (int)rank); ",
+    "mbar_arrive": " emu_arrive(bar, -1); ",
+    "st_second": " emu_store<uint32_t>(at, v, 1); ",
     "tmem_alloc_pair": " emu_tmem_alloc(dst, 512); ",
     "tmem_free_pair": " emu_tmem_free(at, 512); ",
     "tc_copy_scales_pair": " for (int c = 0; c < 2; c++) emu_copy_scales(emu_cluster->cta[c].get(), c, tmem, desc); ",
@@ -64,7 +72,6 @@ BODIES = {
 # instructions that kernels use in place
 INLINE = [
     (r'asm volatile\("fence\.[\w.:]+;" ::: "memory"\);', ";"),
-    (r'asm volatile\("mbarrier\.arrive\.shared::cta\.b64 _, \[%0\];" ::"r"\((.*)\) : "memory"\);', r"emu_arrive(\1, -1);"),
     (r'asm volatile\("st\.shared\.b32 \[%0\], %1;" ::"r"\((.*)\), "r"\((.*)\) : "memory"\);', r"emu_store<uint32_t>(\1, \2);"),
     (r'asm volatile\("st\.shared\.b8 \[%0\], %1;" ::"r"\((.*)\), "r"\((.*)\) : "memory"\);', r"emu_store<uint8_t>(\1, (uint8_t)(\2));"),
     (r'asm volatile\("ld\.shared\.b32 %0, \[%1\];" : "=r"\((.*)\) : "r"\((.*)\) : "memory"\);', r"\1 = emu_load<uint32_t>(\2);"),

@@ -134,3 +134,67 @@ def test_nan_stays_in_its_rows(lib, size, sms):
     y, _ = call(lib, a, b, torch.float32, sms)
     want[1], want[:, 3] = float("nan"), float("nan")
     assert torch.equal(y.isnan(), want.isnan()) and torch.equal(y.nan_to_num(0.5), want.nan_to_num(0.5))
+
+
+# ((t, n, k), SMs, the rank that loses its copies, from which one on)
+LATE = [
+    ((5, 200, 600), 1, 0, 0),        # no cluster: nothing arrives
+    ((5, 200, 600), 1, 0, 4),        # the second panel does not
+    ((100, 130, 1800), 1, 0, 24),    # after the stages went round
+    ((3, 100, 2400), 8, 5, 0),       # one rank of a cluster of 8
+    ((40, 100, 1300), 2, 0, 4),      # of 2
+    ((260, 120, 2400), 4, 1, 8),
+    ((300, 520, 700), 2, 0, 0),      # a pair, either CTA: from its first tile on
+    ((300, 520, 700), 2, 1, 0),
+    ((300, 520, 700), 2, 1, 12),     # from its second one
+    ((300, 520, 700), 2, 0, 42),     # in the middle of its fourth
+]
+
+
+@pytest.mark.parametrize("size,sms,rank,first", LATE)
+def test_sums_that_are_not_complete_are_nan(lib, size, sms, rank, first):
+    """Copies that never arrive: the waits end, each result is right or NaN, and
+    what depends on the lost copies is NaN; none is left unwritten."""
+    t, n, k = size
+    a, b = exact.matrix(t, k, 1), exact.matrix(n, k, 2)
+    want = exact.product(a, b)
+    assert lib.emu_product_errors() == 0
+    lib.emu_product_lose(rank, first, 0.05)
+    try:
+        y, alone = call(lib, a, b, torch.float32, sms, shift=1)
+    finally:
+        lib.emu_product_lose(-1, 0, 0.0)
+    assert alone and lib.emu_product_errors() > 0 and lib.emu_product_errors() == 0
+    assert (y.isnan() | (y.double() == want)).all()
+    whole = 0   # tiles of 256 x 256, row by row, whose copies all arrived (a pair's panel is 4 copies)
+    if t > 128 and n > 128:
+        whole = first // (4 * -(-k // 256))
+    for i, (r, c) in enumerate((r, c) for r in range(0, t, 256) for c in range(0, n, 256)):
+        tile = y[r:r + 256, c:c + 256]
+        assert i < whole or tile.isnan().all()
+    y, _ = call(lib, a, b, torch.float32, sms)   # and the next call is as ever
+    assert torch.equal(y.double(), want) and lib.emu_product_errors() == 0
+
+
+def test_rounding_inside_with_late_copies(lib):
+    b = exact.matrix(40, 600, 2)
+    lib.emu_product_lose(0, 2, 0.05)
+    try:
+        y, _ = call(lib, None, b, torch.bfloat16, 1, x=exact.matrix(3, 600, 1))
+    finally:
+        lib.emu_product_lose(-1, 0, 0.0)
+    assert y.isnan().all() and lib.emu_product_errors() > 0
+
+
+def test_errors_are_reported_once():
+    """falcom_mx4_errors: what gave up since the last call that said so."""
+    from tests.emu import build_mx4
+    lib = ctypes.CDLL(build_mx4.build())
+    abi.bind_mx4(lib)
+    count = ctypes.c_uint32.in_dll(lib, "emu_mx4_gave_up")
+    start = count.value
+    assert lib.falcom_mx4_errors() == 0
+    for more in (1, 5, 2 ** 31 - 1, 2 ** 31 - 1, 3):   # (the count may go round)
+        count.value += more
+        assert lib.falcom_mx4_errors() == 1 and lib.falcom_mx4_errors() == 0
+    assert count.value != start

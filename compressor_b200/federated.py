@@ -22,7 +22,7 @@ from __future__ import annotations
 import ctypes
 import math
 from dataclasses import dataclass
-from typing import List, Sequence
+from typing import List, Optional, Sequence
 
 import numpy as np
 
@@ -448,8 +448,12 @@ class Downlink:
 
         down = Downlink(weights)
         sent = down.send()                     # a round
-        broadcast(sent, dist)                  # one run of bytes
-        Downlink.receive(sent, mine)           # a client: its float32 copy
+        broadcast(sent, dist)                  # one run of bytes, and the round's number
+        Downlink.receive(sent, mine, round=t)  # a client: its float32 copy, brought forward t times so far
+
+    Each vector is a difference from the one before: a client takes every one
+    once, in order.  One that missed a round needs `held` in full, and the
+    number to go on from; `round` is how it is told.
 
     rounding: "nearest", or "random" (from `seed` and the round's number,
     which is on the device: send() may be captured in a CUDA graph).  After a
@@ -472,24 +476,38 @@ class Downlink:
         self.round = torch.zeros(1, dtype=torch.int64, device=weights.device)
 
     def send(self):
-        """The difference (mx4.Mx4Vector), queued on the current stream; held
-        is brought forward by it."""
+        """The difference (mx4.Mx4Vector, its `round` the number of this
+        call), queued on the current stream; held is brought forward by it."""
         sent = self._mx4.encode(self.weights, base=self.held, rounding=self.rounding, seed=self.seed, counter=self.round)
+        sent.round = self.round.clone()
         self.round += 1
         return sent
 
     @staticmethod
-    def receive(sent, weights):
-        """Adds what was sent to a client's weights (returned)."""
+    def receive(sent, weights, round: Optional[int] = None):
+        """Adds what was sent to a client's weights (returned).  With `round`,
+        the number of vectors that these weights have had, ValueError for any
+        other than the next one (the number is read, so this waits for it)."""
         from . import mx4
+        if round is not None:
+            number = int(sent.round) if sent.round is not None else -1
+            if number != round:
+                raise ValueError(f"the vector is of {f'round {number}' if number >= 0 else 'no round'}, these weights want "
+                                 f"that of round {round}: who missed one needs the model in full")
         return mx4.decode(sent, out=weights, accumulate=True)
 
 
 def broadcast(sent, dist, src: int = 0, group=None) -> None:
     """A 4-bit vector or matrix to every rank: those other than `src` pass an
-    empty one of the same size (mx4.Mx4Vector.empty)."""
+    empty one of the same size (mx4.Mx4Vector.empty).  A vector's round goes
+    with it (-1 for none)."""
     if dist is not None and dist.is_initialized() and dist.get_world_size(group) > 1:
         dist.broadcast(sent.buffer, src=src, group=group)
+        if hasattr(sent, "round"):
+            import torch
+            if sent.round is None:
+                sent.round = torch.full((1,), -1, dtype=torch.int64, device=sent.device)
+            dist.broadcast(sent.round, src=src, group=group)
 
 
 class _DeviceFloats:

@@ -1,5 +1,6 @@
 """GPU tests of what the 4-bit operators and dropout promise beside their
-values: operands of any strides, and every byte of what is sent."""
+values: operands of any strides, every byte of what is sent, and the rounds of
+the way down."""
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -38,3 +39,32 @@ def test_every_byte_of_a_vector_is_written(n, shift):
         buffers.append(mx4.encode(x).buffer)
     codes, scales = (n + 1) // 2, buffers[0].numel() - -(-n // 32)
     assert torch.equal(buffers[0], buffers[1]) and not buffers[0][codes:scales].any()
+
+
+@pytest.mark.parametrize("rounding", ["nearest", "random"])
+def test_rounds_of_the_way_down(rounding):
+    """Each vector has its round's number, in a replayed graph too, and a client
+    that is given another one is told before its weights change."""
+    from compressor_b200 import federated as fed
+    weights = wild(1, 5000, torch.bfloat16, 1).cuda()[0]
+    held = torch.zeros(5000, device="cuda")
+    down, mine = fed.Downlink(weights, held=held, rounding=rounding, seed=3), held.clone()
+    for t in range(2):
+        sent = down.send()
+        assert int(sent.round) == t
+        fed.Downlink.receive(sent, mine, round=t)
+    before = mine.clone()
+    with pytest.raises(ValueError, match="round 1, .* round 2"):
+        fed.Downlink.receive(sent, mine, round=2)
+    assert torch.equal(mine, before) and torch.equal(mine, down.held)
+    graph = torch.cuda.CUDAGraph()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=side):
+        sent = down.send()
+    for t in range(2, 5):
+        weights.add_(1)
+        graph.replay()
+        assert int(sent.round) == t and int(down.round) == t + 1
+        fed.Downlink.receive(sent, mine, round=t)
+        assert torch.equal(mine, down.held)

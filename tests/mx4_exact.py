@@ -5,16 +5,16 @@ import torch
 from tests import mx4_reference as ref
 
 
-def matrix(rows, cols, seed):
+def matrix(rows, cols, seed, device="cpu"):
     """float32 values that 4 bits hold: scales of 1/2, 1 and 2, elements of all
     codes, in each block one of 6 times the scale."""
-    g = torch.Generator().manual_seed(seed)
+    g = torch.Generator(device).manual_seed(seed)
     blocks = -(-cols // 32)
-    code = torch.randint(0, 8, (rows, blocks, 32), generator=g)
+    code = torch.randint(0, 8, (rows, blocks, 32), generator=g, device=device)
     code[:, :, 0] = 7
-    sign = 1.0 - 2.0 * torch.randint(0, 2, code.shape, generator=g)
-    scale = torch.exp2(torch.randint(-1, 2, (rows, blocks, 1), generator=g).float())
-    return (ref.VALUES[code].float() * sign * scale).view(rows, -1)[:, :cols].contiguous()
+    sign = 1.0 - 2.0 * torch.randint(0, 2, code.shape, generator=g, device=device)
+    scale = torch.exp2(torch.randint(-1, 2, (rows, blocks, 1), generator=g, device=device).float())
+    return (ref.VALUES.to(device)[code].float() * sign * scale).view(rows, -1)[:, :cols].contiguous()
 
 
 def product(a, b):

@@ -1,6 +1,7 @@
 // mc_mx4.cu -- 4-bit rounding (vectors with what their receivers hold,
-// matrices along rows and columns), reading back, and dropout.  All of it is
-// bound by memory: every element is read once and written once.
+// matrices along rows and columns), reading back, and dropout.  Every element
+// is read once and written once.  On whole aligned rows vectors and dropout
+// are bound by memory, the rounding of matrices by instructions.
 
 #include "mc_mx4_device.h"
 
@@ -245,11 +246,15 @@ __global__ void __launch_bounds__(MX_TPB) k_mx_decode(const __grid_constant__ mx
 // whose scales are one 512-byte piece of either layout.  Rows are rounded as
 // they come in (8 elements a thread, 4 threads a block); for the columns the
 // tile goes through shared memory, where a thread has a block of each of two
-// neighbouring columns, which share their random words.  To the nearest it is
-// bound by memory (16384 x 4096 bf16: rows 36 us, both ways 50; the bytes at
-// the copy rate 26 and 31), at random by logic operations, some 22 an element
-// (both ways 87 us).  Loads of 4 rows a thread ahead of their use and 4 to 5
-// CTAs an SM made 133 us of it 96.
+// neighbouring columns, which share their random words.  To the nearest 16384 x
+// 4096 bf16 take 36 us along rows, 50 both ways (the bytes at the copy rate: 26
+// and 31): both ways 3.4 TB/s with the logic pipe 69 and the issue slots 72 %
+// busy, more instructions than memory.  At random logic operations bound it, 84
+// % busy with some 22 an element (both ways 87 us).  Dropout in front costs
+// 16384 x 1024 both ways 2.5 us (12.6 and 15.1 in a graph).  Loads of 4 rows a
+// thread ahead of their use and 4 to 5 CTAs an SM made 133 us of it 96; to have
+// registers for so many CTAs 14 of the 36 instances keep up to 48 bytes a thread
+// in local memory.
 #define MX_TILE 128
 
 // 8 elements from any address: the aligned 16-byte pieces that they lie in,
@@ -504,6 +509,8 @@ __global__ void __launch_bounds__(MX_TPB, COLS ? (sizeof(T) == 4 ? 3 : 4) : RAND
         ((uint32_t *)(L.along_cols.scales + mx_scale_at(L.cols, c0, r0 / MX_BLOCK)))[tid - 128] = ((const uint32_t *)s_cols)[tid - 128];
 }
 
+// For looking at a matrix: 8 elements a thread, stored one by one (16384 x 4096
+// to bf16 170 us, to float32 226; the bytes at the copy rate 26 and 47).
 template <typename T>
 __global__ void __launch_bounds__(MX_TPB) k_mx_dequantize(const __grid_constant__ mx_dequantize_launch L) {
     mx_begin();
@@ -520,8 +527,9 @@ __global__ void __launch_bounds__(MX_TPB) k_mx_dequantize(const __grid_constant_
 }
 
 // -------------------------------------------------------------- dropout
-// Bound by memory: 16384 x 4096 bf16 in 49 us, with a residual in 65 (the bytes
-// at the copy rate: 41 and 62).
+// Bound by memory where rows are whole 16-byte vectors: 16384 x 4096 bf16 in 49
+// us, with a residual in 65 (the bytes at the copy rate: 41 and 62).  Other rows
+// go two elements a thread: 16384 x 4097 in 116 and 126.
 template <typename T>
 __device__ __forceinline__ float2 pair_of(const T *x) { return make_float2(mx_f32(x[0]), mx_f32(x[1])); }
 __device__ __forceinline__ void pair_from(float *y, float2 v) {

@@ -76,7 +76,13 @@ typedef struct {
 } mx_dequantize_launch;
 
 /* Few enough rows and columns to be rounded inside the product, by every CTA
- * for itself. */
+ * for itself, which saves a launch.  Rounding inside and before, in a graph,
+ * bf16: 1 x 1024 times 4096 rows of weights 3.3 and 5.4 us, 1 x 4096 5.2 and
+ * 7.7, 8 x 4096 7.6 and 7.9, 16 x 2048 6.8 and 6.8: at 32768 elements they
+ * meet.  (4096 columns: 48 KB of rounded rows in a CTA of its own.)  The sizes
+ * of x alone decide, as they do about the workspace; with many more rows of
+ * weights the CTAs round over and over, and 8 x 4096 times 20000 takes 22 us
+ * instead of 12, 16 x 1024 times 50257 12.5 instead of 9.9. */
 #define MX_ROUND_ROWS 16
 #define MX_ROUND_COLS 4096
 #define MX_ROUND_ELEMENTS 32768

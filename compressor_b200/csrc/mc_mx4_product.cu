@@ -132,9 +132,10 @@ __device__ uint32_t g_mx_error;
 // lanes of the sum), a's rows its N, so that neighbouring lanes are
 // neighbouring elements of a row of `out`, and few rows of a (tokens) cost a
 // narrow instruction instead of an empty one.  What bounds it is the way to b:
-// the stages of the CTAs of an SM (3 at most) take all its shared memory (1 x
-// 50257 x 1024 in a graph: 6.8 us, 4.2 of them for the bytes at the copy rate;
-// with 100 KB for each of 2 CTAs 9.3).  The
+// an SM's shared memory is shared out in stages to the CTAs that it gets, 3 at
+// most (1 x 50257 x 1024 in a graph: 6.8 us, 4.2 of them for the bytes at the
+// copy rate; with 100 KB for each of 2 CTAs 9.3).  From 65 rows of a on tensor
+// memory admits 2 CTAs of an SM, from 129 on one, and the rest stays empty.  The
 // CTAs of a cluster have the same tile and a share of the panels each; their
 // sums meet in the order of the ranks.  TX: a is not in 4 bits yet but has
 // elements of this type; each CTA rounds what it needs (void: it is).
@@ -531,7 +532,7 @@ __device__ __forceinline__ uint4 joined(uint4 a, uint4 b, uint32_t from) {
 // memory to `out` (of the first row), from row `first` (0 or 1) on.  16 lanes
 // have a row, 16 bytes each.  A row that does not begin on a 16-byte boundary
 // leaves in the 15 whole pieces that lie in it, put together from two, and 16 /
-// SIZE elements at its two ends, one a lane (8192 x 50257 x 1024 to bf16: 304
+// SIZE elements at its two ends, one a lane (8192 x 50257 x 1024 to bf16: 295
 // us; with 4-byte stores of whole rows 750, on boundaries 225, at the rate of
 // a fill 213).
 template <typename T>

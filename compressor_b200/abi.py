@@ -654,9 +654,10 @@ def bind_mx4(lib: ctypes.CDLL) -> None:
     lib.falcom_mx4_product.argtypes = [P(Mx4MatrixC), P(Mx4MatrixC), c_vp, c_int, size, P(DropoutArgsC), c_vp]
     lib.falcom_mx4_errors.argtypes = []
     lib.falcom_dropout.argtypes = [c_vp, c_vp, c_vp, c_int, size, size, P(DropoutArgsC), c_vp]
-    for fn in (lib.falcom_mx4_encode, lib.falcom_mx4_encode_vector, lib.falcom_mx4_decode, lib.falcom_mx4_quantize, lib.falcom_mx4_dequantize,
-               lib.falcom_mx4_product, lib.falcom_mx4_product_of, lib.falcom_mx4_linear_forward,
-               lib.falcom_mx4_linear_backward, lib.falcom_mx4_errors, lib.falcom_dropout):
+    for fn in (lib.falcom_mx4_encode, lib.falcom_mx4_encode_vector, lib.falcom_mx4_decode, lib.falcom_mx4_quantize,
+               lib.falcom_mx4_dequantize, lib.falcom_mx4_product, lib.falcom_mx4_product_of,
+               lib.falcom_mx4_linear_forward, lib.falcom_mx4_linear_backward, lib.falcom_mx4_errors,
+               lib.falcom_dropout):
         fn.restype = c_int
 
 

@@ -5,6 +5,7 @@
  */
 #include <cuda_runtime_api.h>
 #include <math.h>
+#include <pthread.h>
 #include <stdio.h>
 #include <string.h>
 
@@ -492,18 +493,20 @@ MC_EXPORT int falcom_mx4_linear_backward(const falcom_mx4_linear *l, const void 
 }
 
 MC_EXPORT int falcom_mx4_errors(void) {
+    static pthread_mutex_t lock = PTHREAD_MUTEX_INITIALIZER;
     static uint32_t reported[64];   /* of each device: CTAs that gave up, which the kernels count */
-    uint32_t count = 0, before;
-    int device = -1;
+    uint32_t count = 0;
+    int device = -1, rc = ERROR_COMPRESSION;
+    pthread_mutex_lock(&lock);
     cudaError_t e = cudaGetDevice(&device);
     if (e == cudaSuccess) e = cudaDeviceSynchronize();
     if (e == cudaSuccess) e = (cudaError_t)mc_mx_errors(&count);
-    if (e != cudaSuccess || device < 0 || device >= 64) return ERROR_COMPRESSION;
-    before = __atomic_load_n(&reported[device], __ATOMIC_RELAXED);
-    do {   /* (a later count that another thread reported stays) */
-        if ((int32_t)(count - before) <= 0) return 0;
-    } while (!__atomic_compare_exchange_n(&reported[device], &before, count, 0, __ATOMIC_RELAXED, __ATOMIC_RELAXED));
-    return 1;
+    if (e == cudaSuccess && device >= 0 && device < 64) {
+        rc = count != reported[device] && count != 0;   /* (0 again: the device was reset) */
+        reported[device] = count;
+    }
+    pthread_mutex_unlock(&lock);
+    return rc;
 }
 
 MC_EXPORT int falcom_dropout(const void *x, const void *residual, void *y, int dtype, size_t rows, size_t cols,

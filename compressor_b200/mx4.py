@@ -128,12 +128,13 @@ class Mx4Vector:
     between them, up to 15, are 0.)  `round` goes beside it: the number, an
     int64 tensor, of the federated.Downlink round that it was sent in, or None."""
 
+    round: Optional[torch.Tensor] = None
+
     def __init__(self, n: int, buffer: torch.Tensor):
         if buffer.dtype != torch.uint8 or buffer.dim() != 1 or buffer.numel() != self.size_of(n) \
                 or not buffer.is_contiguous():
             raise ValueError(f"the buffer of {n} elements is {self.size_of(n)} contiguous bytes")
         self.n, self.buffer = n, buffer
-        self.round: Optional[torch.Tensor] = None
 
     @property
     def codes(self) -> torch.Tensor:
